@@ -177,6 +177,73 @@ int slm_hip_attend(slm_hip* ctx, float* y, float* scores, const float* q, const 
 int slm_hip_attend_noalloc(slm_hip* ctx, float* y, float* scores, const float* q, const float* k,
                            const float* v, const slm_attn* a);
 
+/* ---- several sequences over paged caches (no trait counterpart: the reference answers one
+ *      request at a time, src/serve.rs; beside store and attend, for a server that steps
+ *      several conversations together) ----
+ * Keys and values lie in pages, [pages][key_heads][page][dh], that the caller hands out: token
+ * t of a sequence is in slot t % page of the page that its row of a page table names for
+ * t / page. A page has as many slots as the caller likes; dh is a multiple of 4 up to 256. The
+ * buffers are fp32 (slm_hip_alloc) or hold fp16 values (slm_hip_alloc_pages with half), whose
+ * keys and values are widened exactly. All calls may be made inside a recorded step and
+ * outside; under a caller's own capture of the stream they return SLM_E_UNSUPPORTED. */
+typedef struct slm_seqs slm_seqs;
+typedef struct slm_pages {
+    size_t pages, page, key_heads, dh;
+    float *k, *v;    /* [pages][key_heads][page][dh], both fp32 or both fp16, 16-byte aligned */
+    float* mass;     /* [pages][key_heads][page]: attention weight each key has received, or NULL */
+    uint32_t* born;  /* [pages][key_heads][page]: position of each slot's token, or NULL */
+} slm_pages;
+/* A zeroed [pages][key_heads][page][dh] buffer; half: of fp16 values, in fp16 mode and outside
+ * it (slm_hip_upload rounds into it, slm_hip_read widens). Freed with slm_hip_free. */
+int slm_hip_alloc_pages(slm_hip* ctx, size_t pages, size_t key_heads, size_t page, size_t dh, int half,
+                        float** out);
+/* Room for a batch of up to max_n sequences of up to max_pages pages of `page` slots. */
+int slm_hip_seqs_new(slm_hip* ctx, size_t page, size_t max_n, size_t max_pages, slm_seqs** out);
+int slm_hip_seqs_free(slm_hip* ctx, slm_seqs* seqs);
+/* The batch from now on: n sequences of len[b] tokens, of which the last fresh[b] are new (fresh
+ * NULL: one each, none where len is 0), with seen[b] tokens in all (NULL: len[b]; more where an
+ * eviction has taken some), in the pages table[b·width + 0 ..]. Host arrays, copied; entries of the
+ * table behind a sequence's last page are not looked at. The newest token's position is
+ * seen[b] − 1. A step being recorded runs what it holds first. SLM_E_BOUNDS: more sequences or
+ * pages than there is room for. */
+int slm_hip_seqs_set(slm_hip* ctx, slm_seqs* seqs, size_t n, const uint32_t* len, const uint32_t* fresh,
+                     const uint32_t* seen, const uint32_t* table, size_t width);
+/* The new tokens' keys and values ([rows][key_heads][dh] fp32, the sequences' new tokens one
+ * after another) into the last slots of their sequences, rounded to nearest even into fp16
+ * pages; their mass (where the cache has it) becomes 0, their born the position. No other slot
+ * changes. SLM_E_INVALID where a page that takes new tokens is in the table twice. */
+int slm_hip_paged_store(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, const float* k, const float* v);
+/* Softmax attention of the newest token of each sequence over its slots: q and y are
+ * [n][heads][dh]; query head h reads key head h / (heads / key_heads), at most 16 to one. Seen are
+ * the tokens of position seen[b] − 1 − gap and before: by `born` where the cache has it, else
+ * slot t holds position t (as long as nothing was evicted). A sequence that sees no token gets
+ * zeros. mass_out (NULL: none): mass plus the weights that the key received from the heads that
+ * read it, for all the sequences' slots, those not seen included; it may be `mass` itself. Other
+ * slots of it stay as they were. The weights are fp32, in fp16 mode too; y is rounded there as
+ * slm_hip_attend rounds it. A sequence's result has the same bits in any batch. SLM_E_INVALID for
+ * mass_out where a page is in the table twice (without it, sequences may share pages). */
+int slm_hip_paged_attend(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* y, float* mass_out,
+                         const float* q, size_t heads, size_t gap, float scale);
+/* Leaves every sequence of more than `keep` (≥ 1) tokens its `keep` most wanted under each key
+ * head: first the newest `recent` (≤ keep) by position, then those of largest mass, of equal mass
+ * the lower slot (NaN counts as less than any number). Kept tokens in slots from `keep` on move,
+ * the r-th of them into the r-th of the slots below that were given up, with their mass and
+ * position; slots from `keep` on stay as they were, and their pages are free once the caller has
+ * set the batch's lengths to min(len, keep). mass_out and born_out are the cache's own mass and
+ * born, or other buffers, which then receive both for the slots that hold tokens (and the cache's
+ * stay as they were). SLM_E_INVALID where a page is in the table twice. */
+int slm_hip_paged_evict(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* mass_out, uint32_t* born_out,
+                        size_t keep, size_t recent);
+/* What rows of logits x ([m][n]) say of given tokens (beside slm_hip_argmax; sample.rs keeps no
+ * probabilities): lp[i] = x[i][ids[i]] − log Σ e^x[i]; entropy[i] = −Σ p log p in nats (NULL:
+ * none); and the `top` (0 to 32, at most n) likeliest tokens with their log probabilities,
+ * [m][top] (both NULL with top 0): larger logits first, of equal ones the lower token, NaNs
+ * last. `ids` is host memory, as slm_hip_gather's. Logits of −infinity are impossible tokens;
+ * a row of nothing else has lp −infinity and entropy 0. A NaN or +infinity in a row goes where
+ * the formulas take it. The outputs are fp32 in fp16 mode too. */
+int slm_hip_logprobs(slm_hip* ctx, float* lp, float* entropy, uint32_t* top_ids, float* top_lp, size_t top,
+                     const float* x, const uint32_t* ids, size_t m, size_t n);
+
 /* ---- steps (no trait counterpart; backend settings like cuda.rs's one stream) ----
  * With step graphs or fusion on (both are by default), the operations of one advance —
  * from rope_table to flush — are recorded instead of launched. At flush the planner

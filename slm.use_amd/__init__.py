@@ -46,6 +46,13 @@ class Attn(C.Structure):
         ("scale", C.c_float)]
 
 
+class Pages(C.Structure):
+    """slm_pages: a paged cache, its buffers as pointers (Buffer.ptr)."""
+
+    _fields_ = [(n, C.c_size_t) for n in ("pages", "page", "key_heads", "dh")] + [
+        (n, C.c_void_p) for n in ("k", "v", "mass", "born")]
+
+
 if not LIB_PATH.exists():
     raise ImportError(f"{LIB_PATH} is not built: run `python slm.use_amd/build.py` "
                       "(or __graft_entry__.build())")
@@ -115,6 +122,14 @@ _SIGS = {
     "slm_hip_alloc_cache": (_i, [_p, _sz, _sz, _sz, C.POINTER(_p)]),
     "slm_hip_grow_cache": (_i, [_p, _p, _p, _sz, _sz, _sz]),
     "slm_hip_mem_info": (_i, [_p, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
+    "slm_hip_alloc_pages": (_i, [_p, _sz, _sz, _sz, _sz, _i, C.POINTER(_p)]),
+    "slm_hip_seqs_new": (_i, [_p, _sz, _sz, _sz, C.POINTER(_p)]),
+    "slm_hip_seqs_free": (_i, [_p, _p]),
+    "slm_hip_seqs_set": (_i, [_p, _p, _sz, _u32p, _u32p, _u32p, _u32p, _sz]),
+    "slm_hip_paged_store": (_i, [_p, _p, C.POINTER(Pages), _p, _p]),
+    "slm_hip_paged_attend": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _p, _sz, _sz, _f]),
+    "slm_hip_paged_evict": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _sz, _sz]),
+    "slm_hip_logprobs": (_i, [_p, _p, _p, _p, _p, _sz, _p, _u32p, _sz, _sz]),
     "slm_model_load": (_i, [_p, C.c_char_p, C.POINTER(_p)]),
     "slm_model_free": (None, [_p]),
     "slm_model_error": (C.c_char_p, [_p]),
@@ -383,6 +398,30 @@ class Hip:
         args = Attn(**a)
         self.check(lib.slm_hip_attend_noalloc(self.ctx, y, None, q, k, v, C.byref(args)))
 
+    def alloc_pages(self, pages: int, key_heads: int, page: int, dh: int, half: bool = False) -> Buffer:
+        """A zeroed [pages][key_heads][page][dh] buffer of a paged cache; half: of fp16 values."""
+        p = _p()
+        self.check(lib.slm_hip_alloc_pages(self.ctx, pages, key_heads, page, dh, int(half), C.byref(p)))
+        return Buffer(self, p.value, max(pages * key_heads * page * dh, 1))
+
+    def seqs(self, page: int, max_n: int, max_pages: int) -> "Seqs":
+        """Room for a batch of sequences over paged caches."""
+        return Seqs(self, page, max_n, max_pages)
+
+    def paged_store(self, seqs: "Seqs", pages: Pages, k, v):
+        self.check(lib.slm_hip_paged_store(self.ctx, seqs.h, C.byref(pages), k, v))
+
+    def paged_attend(self, seqs: "Seqs", pages: Pages, y, q, heads, scale, gap=0, mass_out=None):
+        self.check(lib.slm_hip_paged_attend(self.ctx, seqs.h, C.byref(pages), y, mass_out, q, heads, gap, scale))
+
+    def paged_evict(self, seqs: "Seqs", pages: Pages, mass_out, born_out, keep, recent):
+        self.check(lib.slm_hip_paged_evict(self.ctx, seqs.h, C.byref(pages), mass_out, born_out, keep, recent))
+
+    def logprobs(self, lp, x, ids, n, entropy=None, top=0, top_ids=None, top_lp=None):
+        """x: rows of n logits, one a token of ids."""
+        ids = np.ascontiguousarray(ids, dtype=np.uint32)
+        self.check(lib.slm_hip_logprobs(self.ctx, lp, entropy, top_ids, top_lp, top, x, _up(ids), ids.size, n))
+
     def stream(self) -> int:
         s = _p()
         self.check(lib.slm_hip_stream(self.ctx, C.byref(s)))
@@ -408,6 +447,37 @@ class Hip:
 
     def probe_mfma(self, out, a, b):
         self.check(lib.slm_hip_probe_mfma(self.ctx, out, a, b))
+
+
+class Seqs:
+    """A batch of sequences over paged caches (slm_seqs)."""
+
+    def __init__(self, hip: Hip, page: int, max_n: int, max_pages: int):
+        self.hip, self.page, self.h = hip, page, None
+        h = _p()
+        hip.check(lib.slm_hip_seqs_new(hip.ctx, page, max_n, max_pages, C.byref(h)))
+        self.h = h.value
+
+    def set(self, lens, table, fresh=None, seen=None):
+        """lens [n]; table [n][width]: the pages; fresh [n]: new tokens (None: one each); seen [n]:
+        tokens in all (None: lens)."""
+        def u32(a):
+            return None if a is None else np.ascontiguousarray(a, dtype=np.uint32)
+
+        lens, table, fresh, seen = u32(lens), u32(table), u32(fresh), u32(seen)
+        n, width = table.shape
+        if any(a is not None and a.shape != (n,) for a in (lens, fresh, seen)):
+            raise ValueError(f"seqs: arrays of {n} sequences are wanted")
+        self.hip.check(lib.slm_hip_seqs_set(self.hip.ctx, self.h, n, *(None if a is None else _up(a) for a in (
+            lens, fresh, seen)), _up(table), width))
+
+    def free(self):
+        if self.h and self.hip.ctx:
+            self.hip.check(lib.slm_hip_seqs_free(self.hip.ctx, self.h))
+        self.h = None
+
+    def __del__(self):
+        self.free()
 
 
 class Model:

@@ -1,5 +1,5 @@
-"""Builds the backend in place: the gfx950 code object (hipcc --genco), embedded as a byte
-array into libslm_hip.so together with the host runtime (runtime.cpp, the C ABI of
+"""Builds the backend in place: the gfx950 code objects (hipcc --genco), embedded as byte
+arrays into libslm_hip.so together with the host runtime (runtime.cpp, the C ABI of
 include/slm_hip.h), the model twin (model.cpp, include/slm_model.h) and the fixed device
 scratch of the allocation-free entry points (scratch.hip, a HIP translation unit of its own).
 
@@ -39,39 +39,42 @@ def run(cmd):
     return out
 
 
-def embed(co: Path, dst: Path):
+def embed(co: Path, dst: Path, name: str):
     data = co.read_bytes()
     rows = []
     for i in range(0, len(data), 24):
         rows.append(",".join(str(b) for b in data[i:i + 24]))
     dst.write_text(
-        "// generated by slm.use_amd/build.py from the gfx950 code object\n"
+        "// generated by slm.use_amd/build.py from a gfx950 code object\n"
         "#include <stddef.h>\n"
         "extern \"C\" {\n"
-        f"extern const unsigned char slm_code_object[{len(data)}];\n"
-        "extern const size_t slm_code_object_size;\n"
-        f"alignas(4096) const unsigned char slm_code_object[{len(data)}] = {{\n"
+        f"extern const unsigned char {name}[{len(data)}];\n"
+        f"extern const size_t {name}_size;\n"
+        f"alignas(4096) const unsigned char {name}[{len(data)}] = {{\n"
         + ",\n".join(rows) + "\n};\n"
-        f"const size_t slm_code_object_size = {len(data)};\n"
+        f"const size_t {name}_size = {len(data)};\n"
         "}\n")
 
 
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
-    co = BUILD / "kernels.co"
-    run([HIPCC, "--genco", *DEVICE_FLAGS, str(CSRC / "kernels.hip"), "-o", str(co)])
-    blob = BUILD / "kernels_blob.cpp"
-    embed(co, blob)
+    blobs = []
+    for src, name in (("kernels", "slm_code_object"), ("batch", "slm_batch_object")):
+        co = BUILD / f"{src}.co"
+        run([HIPCC, "--genco", *DEVICE_FLAGS, str(CSRC / f"{src}.hip"), "-o", str(co)])
+        blobs.append(BUILD / f"{src}_blob.cpp")
+        embed(co, blobs[-1], name)
     objs = [BUILD / "scratch.o"]
     run([HIPCC, "-c", "-fPIC", *DEVICE_FLAGS, str(CSRC / "scratch.hip"), "-o", str(objs[0])])
-    for src in (CSRC / "runtime.cpp", CSRC / "model.cpp", blob):
+    for src in (CSRC / "runtime.cpp", CSRC / "model.cpp", *blobs):
         objs.append(BUILD / (src.stem + ".o"))
         run([HIPCC, *HOST_FLAGS, "-c", "-I", str(ROOT / "include"), str(src), "-o", str(objs[-1])])
     tmp = LIB.with_suffix(".so.tmp")
     run([HIPCC, "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)])
     os.replace(tmp, LIB)
     if verbose:
-        print(f"built {LIB} ({LIB.stat().st_size} bytes; code object {co.stat().st_size} bytes)")
+        sizes = ", ".join(f"{p.name} {p.stat().st_size}" for p in sorted(BUILD.glob("*.co")))
+        print(f"built {LIB} ({LIB.stat().st_size} bytes; {sizes})")
     return LIB
 
 

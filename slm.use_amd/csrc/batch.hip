@@ -1,0 +1,590 @@
+// gfx950 (CDNA4) kernels for several sequences over paged caches, and for the scores of rows
+// of logits: a code object of its own, loaded by the host runtime beside kernels.hip's and
+// compiled with the same flags (expressions round as written).
+//
+// A paged cache is [pages][key heads][page][dh]: token t of a sequence lies in slot t % page of
+// page table[t / page]. Every result is computed in an order that depends on the sequence
+// alone, not on the batch around it or on how the launch is cut: the bits of a sequence's
+// attention are the same whatever it is batched with.
+
+#include <float.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "batch.h"
+
+#define KERNEL extern "C" __global__
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+static constexpr float NEG_INF = -__builtin_inff();
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+// Sums and maxima over a row of 16 lanes (in every lane): lane pairs, quads, then the mirrored
+// lane of eight and of sixteen.
+__device__ __forceinline__ float row_sum(float x) {
+    x += dpp<0xB1>(x);
+    x += dpp<0x4E>(x);
+    x += dpp<0x141>(x);
+    return x + dpp<0x140>(x);
+}
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));
+    return fmaxf(x, dpp<0x140>(x));
+}
+// The same over lanes 16 (32) apart, by register lane swaps.
+__device__ __forceinline__ float sum16(float v) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float sum32(float v) {
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float max16(float v) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float max32(float v) {
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float wave_sum(float v) { return sum32(sum16(row_sum(v))); }
+__device__ __forceinline__ float wave_max(float v) { return max32(max16(row_max(v))); }
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {  // set bits below this lane
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// fp16 mode's rounding of what an operation writes (the fp32 value rounds: the register is
+// opaque, so the compiler does not fold the product before it into the conversion).
+__device__ __forceinline__ float r16(float v) {
+    asm volatile("" : "+v"(v));
+    return (float)(_Float16)v;
+}
+
+__device__ __forceinline__ f4 load4(const float* p) { return *(const f4*)p; }
+__device__ __forceinline__ f4 load4(const _Float16* p) {
+    h4 v = *(const h4*)p;
+    return f4{(float)v.x, (float)v.y, (float)v.z, (float)v.w};
+}
+
+// Row of a sequence's token t under key head h, over [pages][kh][page].
+__device__ __forceinline__ uint32_t row_of(const SeqsDev& s, int b, uint32_t t, int h, int kh, int page) {
+    uint32_t pg = t / (uint32_t)page;
+    return (s.table[(int64_t)b * s.width + pg] * (uint32_t)kh + (uint32_t)h) * (uint32_t)page + (t - pg * (uint32_t)page);
+}
+
+// ---------------------------------------------------------------------------------------
+// store: the new tokens' keys and values into the pages
+// ---------------------------------------------------------------------------------------
+
+// Rows of new tokens lie one sequence after another; a row's sequence is found by bisection of
+// the batch's row offsets. One thread an element: a row of 64 floats is one wave's store of 256
+// bytes. A slot's noted weight starts at zero, its position is the token's.
+template <typename T>
+__device__ __forceinline__ void store_body(const PStoreArgs& a) {
+    const int64_t per = (int64_t)a.kh * a.dh, total = (int64_t)a.rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        uint32_t row = (uint32_t)(i / per);
+        int e = (int)(i - row * per), h = e / a.dh, d = e - h * a.dh;
+        int lo = 0, hi = a.s.n;  // first[lo] <= row < first[hi]
+        while (hi - lo > 1) {
+            int mid = (lo + hi) >> 1;
+            if (a.s.first[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        uint32_t behind = a.s.first[lo + 1] - row;  // 1: the newest
+        uint32_t to = row_of(a.s, lo, a.s.len[lo] - behind, h, a.kh, a.page);
+        ((T*)a.k)[(int64_t)to * a.dh + d] = (T)a.ksrc[i];
+        ((T*)a.v)[(int64_t)to * a.dh + d] = (T)a.vsrc[i];
+        if (d == 0) {
+            if (a.mass) a.mass[to] = 0.0f;
+            if (a.born) a.born[to] = a.s.seen[lo] - behind;
+        }
+    }
+}
+KERNEL void __launch_bounds__(256) slm_paged_store(PStoreArgs a) { store_body<float>(a); }
+KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<_Float16>(a); }
+
+// ---------------------------------------------------------------------------------------
+// attend: one new token a sequence
+// ---------------------------------------------------------------------------------------
+
+// y_g = sum_t softmax_t(scale · q_g·k_t) v_t for the query heads g of one key head, over one
+// superblock of SLM_PG_KEYS slots: the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
+// x = (scale · log2 e) q·k. slm_paged_join adds the superblocks up. A superblock none of whose
+// slots is visible has m = -inf, one with a visible slot at least -FLT_MAX.
+extern __shared__ char lds_[];
+
+template <typename T, int NT>
+__device__ __forceinline__ void attn_body(const PAttnArgs& a) {
+    constexpr int DP = 64 * NT;
+    const int h = blockIdx.x % a.kh, item = blockIdx.x / a.kh;
+    const uint32_t b = a.s.items[2 * item], sb = a.s.items[2 * item + 1];
+    if (b == SLM_NO_SEQ) return;
+    const int G = a.heads / a.kh, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, dh = a.dh;
+    const uint32_t len = a.s.len[b], base = sb * SLM_PG_KEYS;
+    // slots to look at: all where positions are given, else those before the gap
+    const uint32_t most = a.born ? len : (int64_t)len > a.gap ? (uint32_t)(len - a.gap) : 0;
+    if (base >= most && !(a.direct && sb == 0)) return;
+
+    float* sq = (float*)lds_;                // [G][DP]
+    float* ss = sq + G * DP;                 // [G][SLM_PG_KEYS]
+    float* so = ss + G * SLM_PG_KEYS;        // [4][G][DP]
+    float* sml = so + 4 * G * DP;            // [G][2]
+    uint32_t* srow = (uint32_t*)(sml + 2 * G);  // [SLM_PG_KEYS], the top bit: not visible
+    {
+        uint32_t t = base + tid, row = 0x80000000u;
+        if (len) {
+            row = row_of(a.s, b, min(t, len - 1), h, a.kh, a.page);
+            bool sees = t < most;
+            if (sees && a.born) sees = (uint64_t)a.born[row] + (uint64_t)a.gap < a.s.seen[b];
+            if (!sees) row |= 0x80000000u;
+        }
+        srow[tid] = row;
+    }
+    for (int i = tid; i < G * DP; i += 256) {
+        int g = i / DP, d = i % DP;
+        sq[i] = d < dh ? a.q[((int64_t)b * a.heads + h * G + g) * dh + d] : 0.0f;
+    }
+    __syncthreads();
+    const bool any_key = len > 0;
+    {  // scores: sixteen lanes a key
+        const int r = lane >> 4, c = lane & 15;
+#pragma unroll 4
+        for (int j = 0; j < 16; j++) {
+            int key = w * 64 + 4 * j + r;
+            uint32_t row = srow[key];
+            f4 kv[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                int d = 64 * t + 4 * c;
+                kv[t] = any_key && d < dh ? load4((const T*)a.k + (int64_t)(row & 0x7fffffffu) * dh + d) : f4{0, 0, 0, 0};
+            }
+            for (int g = 0; g < G; g++) {
+                float s = 0.0f;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    f4 q = *(const f4*)(sq + g * DP + 64 * t + 4 * c);
+                    s = fmaf(q.x, kv[t].x, s);
+                    s = fmaf(q.y, kv[t].y, s);
+                    s = fmaf(q.z, kv[t].z, s);
+                    s = fmaf(q.w, kv[t].w, s);
+                }
+                s = row_sum(s) * a.scale;
+                if (c == 0) ss[g * SLM_PG_KEYS + key] = (int)row < 0 ? NEG_INF : s;
+            }
+        }
+    }
+    __syncthreads();
+    for (int g = w; g < G; g += 4) {  // softmax: a wave a head
+        float x[4], m = NEG_INF;
+        bool sees = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[i] = ss[g * SLM_PG_KEYS + lane + 64 * i];
+            sees |= (int)srow[lane + 64 * i] >= 0;
+            m = fmaxf(m, x[i]);
+        }
+        m = wave_max(m);
+        if (__ballot(sees)) m = fmaxf(m, -FLT_MAX);
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (a.sc) a.sc[((int64_t)item * a.heads + h * G + g) * SLM_PG_KEYS + lane + 64 * i] = x[i];
+            float p = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m);
+            ss[g * SLM_PG_KEYS + lane + 64 * i] = p;
+            l += p;
+        }
+        l = wave_sum(l);
+        if (lane == 0) {
+            sml[2 * g] = m;
+            sml[2 * g + 1] = l;
+        }
+    }
+    __syncthreads();
+    {  // values: 16·NT threads a key
+        constexpr int C = 16 * NT, KG = 256 / C;
+        const int c = tid % C, kg = tid / C, d = 4 * c;
+        for (int g0 = 0; g0 < G; g0 += 4) {
+            f4 acc[4] = {};
+#pragma unroll 8
+            for (int key = kg; key < SLM_PG_KEYS; key += KG) {
+                uint32_t row = srow[key];
+                f4 v = f4{0, 0, 0, 0};
+                if ((int)row >= 0 && d < dh) v = load4((const T*)a.v + (int64_t)row * dh + d);
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    if (g0 + g >= G) break;
+                    float p = ss[(g0 + g) * SLM_PG_KEYS + key];
+                    acc[g].x = fmaf(p, v.x, acc[g].x);
+                    acc[g].y = fmaf(p, v.y, acc[g].y);
+                    acc[g].z = fmaf(p, v.z, acc[g].z);
+                    acc[g].w = fmaf(p, v.w, acc[g].w);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (g0 + g >= G) break;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float o = acc[g][e];
+                    if (NT == 1) o = sum16(o);
+                    if (NT <= 2) o = sum32(o);
+                    if (lane < C) so[(w * G + g0 + g) * DP + (tid % C) * 4 + e] = o;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < G * dh; i += 256) {
+        int g = i / dh, d = i - g * dh, H = h * G + g;
+        float o = 0.0f;
+        if (NT <= 2) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) o += so[(k * G + g) * DP + d];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) o += so[(k * G + g) * DP + d];
+        }
+        float m = sml[2 * g], l = sml[2 * g + 1];
+        if (a.direct) {
+            float y = m == NEG_INF ? 0.0f : o / l;
+            a.y[((int64_t)b * a.heads + H) * dh + d] = a.r16 ? r16(y) : y;
+        } else {
+            a.po[((int64_t)item * a.heads + H) * dh + d] = o;
+            if (d == 0) {
+                a.ml[2 * ((int64_t)item * a.heads + H)] = m;
+                a.ml[2 * ((int64_t)item * a.heads + H) + 1] = l;
+            }
+        }
+    }
+    if (a.direct && a.mass_out && base + tid < len) {
+        uint32_t row = srow[tid] & 0x7fffffffu;
+        float add = 0.0f;
+        for (int g = 0; g < G; g++)
+            if (sml[2 * g] != NEG_INF) add += ss[g * SLM_PG_KEYS + tid] / sml[2 * g + 1];
+        a.mass_out[row] = a.mass[row] + add;
+    }
+}
+
+#define PAGED_ATTN(name, T, NT) \
+    KERNEL void __launch_bounds__(256) name(PAttnArgs a) { attn_body<T, NT>(a); }
+PAGED_ATTN(slm_paged_attn_1, float, 1)
+PAGED_ATTN(slm_paged_attn_2, float, 2)
+PAGED_ATTN(slm_paged_attn_4, float, 4)
+PAGED_ATTN(slm_paged_attn16_1, _Float16, 1)
+PAGED_ATTN(slm_paged_attn16_2, _Float16, 2)
+PAGED_ATTN(slm_paged_attn16_4, _Float16, 4)
+
+// The superblocks of a sequence that a call looks at.
+__device__ __forceinline__ int superblocks(const PAttnArgs& a, int b) {
+    uint32_t len = a.s.len[b];
+    uint32_t most = a.born ? len : (int64_t)len > a.gap ? (uint32_t)(len - a.gap) : 0;
+    return (int)((most + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
+}
+
+// M = max m_z and L = sum l_z 2^(m_z - M) over a sequence's nz superblocks for one head, by a
+// workgroup of 256 (every thread gets both): threads stride over z, then one fixed tree.
+__device__ __forceinline__ float2 join_ml(const float* ml, int heads, int nz, float* red) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    float m = NEG_INF;
+    for (int z = tid; z < nz; z += 256) m = fmaxf(m, ml[2 * (int64_t)z * heads]);
+    m = wave_max(m);
+    __syncthreads();
+    if (lane == 0) red[w] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float l = 0.0f, ms = m == NEG_INF ? 0.0f : m;
+    for (int z = tid; z < nz; z += 256)
+        l = fmaf(ml[2 * (int64_t)z * heads + 1], __builtin_amdgcn_exp2f(ml[2 * (int64_t)z * heads] - ms), l);
+    l = wave_sum(l);
+    if (lane == 0) red[4 + w] = l;
+    __syncthreads();
+    return make_float2(m, (red[4] + red[5]) + (red[6] + red[7]));
+}
+
+// y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), the superblocks dealt to
+// 256 / (dh / 4) groups of threads, whose sums add in order. Behind them, with mass_out, a
+// workgroup a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g.
+KERNEL void __launch_bounds__(256) slm_paged_join(PAttnArgs a) {
+    __shared__ float red[8];
+    __shared__ float so[256 * 4];
+    const int tid = threadIdx.x, H = a.heads;
+    if ((int)blockIdx.x < a.s.n * H) {
+        const int b = blockIdx.x / H, g = blockIdx.x % H, nz = superblocks(a, b);
+        const int64_t z0 = a.s.ifirst[b];
+        float2 ML = join_ml(a.ml + 2 * (z0 * H + g), H, nz, red);
+        const int C = a.dh / 4, KG = 256 / C, c = tid % C, zg = tid / C;
+        float ms = ML.x == NEG_INF ? 0.0f : ML.x;
+        f4 o = {0, 0, 0, 0};
+        if (zg < KG)
+            for (int z = zg; z < nz; z += KG) {
+                float wz = __builtin_amdgcn_exp2f(a.ml[2 * ((z0 + z) * H + g)] - ms);
+                f4 v = *(const f4*)(a.po + ((z0 + z) * H + g) * a.dh + 4 * c);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = fmaf(v[e], wz, o[e]);
+            }
+        *(f4*)(so + 4 * tid) = o;
+        __syncthreads();
+        if (tid < a.dh) {
+            float s = 0.0f;
+            for (int k = 0; k < KG; k++) s += so[4 * C * k + tid];
+            float y = ML.x == NEG_INF ? 0.0f : s / ML.y;
+            a.y[((int64_t)b * H + g) * a.dh + tid] = a.r16 ? r16(y) : y;
+        }
+        return;
+    }
+    const int k = blockIdx.x - a.s.n * H, item = k / a.kh, h = k % a.kh, G = H / a.kh;
+    const uint32_t b = a.s.items[2 * item], sb = a.s.items[2 * item + 1];
+    if (b == SLM_NO_SEQ) return;
+    const uint32_t t = sb * SLM_PG_KEYS + tid, len = a.s.len[b];
+    const int nz = superblocks(a, b);
+    float add = 0.0f;
+    for (int g = 0; g < G && (int)sb < nz; g++) {
+        float2 ML = join_ml(a.ml + 2 * ((int64_t)a.s.ifirst[b] * H + h * G + g), H, nz, red);
+        if (ML.x != NEG_INF)
+            add += __builtin_amdgcn_exp2f(a.sc[((int64_t)item * H + h * G + g) * SLM_PG_KEYS + tid] - ML.x) / ML.y;
+    }
+    if (t < len) {
+        uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+        a.mass_out[row] = a.mass[row] + add;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// evict: which slots stay, then the moves
+// ---------------------------------------------------------------------------------------
+
+// A slot's rank as a number: the newest above all, then by weight (NaN below all, -0 as 0).
+__device__ __forceinline__ uint32_t mass_key(float m, uint32_t born, uint32_t recent, uint32_t seen) {
+    if ((uint64_t)born + recent >= seen) return 0xffffffffu;
+    if (m != m) return 0;
+    uint32_t u = __float_as_uint(m + 0.0f);
+    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// Exclusive prefix of one value a wave over the workgroup's 16 waves, and the total.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v, uint32_t* s, uint32_t* total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __syncthreads();
+    if (lane == 0) s[w] = v;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < 16; i++) {
+        if (i < w) before += s[i];
+        all += s[i];
+    }
+    *total = all;
+    return before;
+}
+
+// A workgroup of 1024 a (sequence, key head): the keep-th largest key by three rounds of
+// counting its digits (11, 11 and 10 bits), ties by slot; then, over the slots in order, which
+// of the first `keep` are left and which of those behind move there.
+KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
+    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t red[16];
+    __shared__ uint32_t pick[2];
+    const int h = blockIdx.x % a.kh, b = blockIdx.x / a.kh, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t len = a.s.len[b], seen = a.s.seen[b];
+    if (len <= a.keep) {  // nothing goes
+        if (tid == 0) a.count[blockIdx.x] = 0;
+        if (!a.in_place)
+            for (uint32_t t = tid; t < len; t += 1024) {
+                uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+                a.mass_out[row] = a.mass[row];
+                a.born_out[row] = a.born[row];
+            }
+        return;
+    }
+    auto key_of = [&](uint32_t t) {
+        uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+        return mass_key(a.mass[row], a.born[row], a.recent, seen);
+    };
+    uint32_t prefix = 0, need = a.keep;  // keys that share the digits so far: `need` of them stay
+    for (int round = 0; round < 3; round++) {
+        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+        for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
+        __syncthreads();
+        for (uint32_t t = tid; t < len; t += 1024) {
+            uint32_t k = key_of(t);
+            if (round == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        // the digit at which the count from above reaches `need`: each thread two bins, from above
+        uint32_t h1 = hist[2047 - 2 * tid], h0 = hist[2046 - 2 * tid], mine = h1 + h0;
+        uint32_t incl = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            uint32_t v = __shfl_up(incl, o);
+            if (lane >= o) incl += v;
+        }
+        uint32_t total, before = wave_prefix(__shfl(incl, 63), red, &total) + incl - mine;
+        if (before < need && before + mine >= need) {
+            bool first = before + h1 >= need;
+            pick[0] = 2047 - 2 * tid - (first ? 0 : 1);
+            pick[1] = need - before - (first ? 0 : h1);
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | pick[0];
+        need = pick[1];
+        __syncthreads();
+    }
+    // keys above `prefix` stay, and the first `need` of those equal to it. A wave takes a run of
+    // whole 64s of slots.
+    const uint32_t run = (len + 1024 - 1) / 1024 * 64, lo = min(len, w * run), hi = min(len, lo + run);
+    uint32_t ties = 0;
+    for (uint32_t t0 = lo; t0 < hi; t0 += 64)
+        ties += __popcll(__ballot(t0 + lane < hi && key_of(t0 + lane) == prefix));
+    uint32_t total, tie0 = wave_prefix(ties, red, &total);
+    auto kept_of = [&](uint32_t t0, uint32_t& tie) {
+        uint32_t k = t0 + lane < hi ? key_of(t0 + lane) : 0;
+        bool in = t0 + lane < hi, eq = in && k == prefix;
+        uint64_t em = __ballot(eq);
+        bool kept = in && (k > prefix || (eq && tie + lanes_below(em) < need));
+        tie += __popcll(em);
+        return kept;
+    };
+    uint32_t holes = 0, movers = 0, tie = tie0;
+    for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
+        bool kept = kept_of(t0, tie), in = t0 + lane < hi;
+        holes += __popcll(__ballot(in && !kept && t0 + lane < a.keep));
+        movers += __popcll(__ballot(kept && t0 + lane >= a.keep));
+    }
+    uint32_t nh, nm, hole0 = wave_prefix(holes, red, &nh), mover0 = wave_prefix(movers, red, &nm);
+    uint32_t* to = a.moves + (int64_t)blockIdx.x * 2 * a.most;
+    uint32_t* from = to + a.most;
+    if (tid == 0) a.count[blockIdx.x] = nm;
+    tie = tie0;
+    for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
+        uint32_t t = t0 + lane;
+        bool kept = kept_of(t0, tie), in = t < hi;
+        bool hole = in && !kept && t < a.keep, mover = kept && t >= a.keep;
+        uint64_t hm = __ballot(hole), mm = __ballot(mover);
+        if (hole) to[hole0 + lanes_below(hm)] = t;
+        if (mover) from[mover0 + lanes_below(mm)] = t;
+        hole0 += __popcll(hm);
+        mover0 += __popcll(mm);
+        if (kept && !mover && !a.in_place) {
+            uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+            a.mass_out[row] = a.mass[row];
+            a.born_out[row] = a.born[row];
+        }
+    }
+}
+
+// The moves of a (sequence, key head), 64 of them a workgroup: sixteen lanes a row.
+template <typename V>
+__device__ __forceinline__ void move_body(const PEvictArgs& a, uint32_t blocks) {
+    const uint32_t pair = blockIdx.x / blocks, r0 = blockIdx.x % blocks * 64;
+    const uint32_t n = a.count[pair];
+    if (r0 >= n) return;
+    const int h = pair % a.kh, b = pair / a.kh, tid = threadIdx.x;
+    const uint32_t* to = a.moves + (int64_t)pair * 2 * a.most;
+    const uint32_t* from = to + a.most;
+    const int vecs = a.dh * a.unit / (int)sizeof(V);  // a row
+    for (uint32_t r = r0 + tid / 16; r < min(n, r0 + 64); r += 16) {
+        uint32_t d = row_of(a.s, b, to[r], h, a.kh, a.page), s = row_of(a.s, b, from[r], h, a.kh, a.page);
+        for (int c = tid % 16; c < vecs; c += 16) {
+            V kv = ((const V*)a.k)[(int64_t)s * vecs + c], vv = ((const V*)a.v)[(int64_t)s * vecs + c];
+            ((V*)a.k)[(int64_t)d * vecs + c] = kv;
+            ((V*)a.v)[(int64_t)d * vecs + c] = vv;
+        }
+        if (tid % 16 == 0) {
+            a.mass_out[d] = a.mass[s];
+            a.born_out[d] = a.born[s];
+        }
+    }
+}
+KERNEL void __launch_bounds__(256) slm_paged_move16(PMoveArgs a) { move_body<f4>(a.e, a.blocks); }
+KERNEL void __launch_bounds__(256) slm_paged_move8(PMoveArgs a) { move_body<h4>(a.e, a.blocks); }
+
+// ---------------------------------------------------------------------------------------
+// logprobs
+// ---------------------------------------------------------------------------------------
+
+// A logit's rank as a number: NaN below all, -0 as 0.
+__device__ __forceinline__ uint32_t logit_key(float x) {
+    if (x != x) return 0;
+    uint32_t u = __float_as_uint(x + 0.0f);
+    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.0f;
+    for (int i = 0; i < 16; i++) s += red[i];
+    return s;
+}
+
+// A workgroup of 1024 a row: its maximum, then L = c + S and E = sum e^(x-M) (x-M), where c
+// logits are the maximum M and S sums e^(x-M) over the others, so that log L = log c +
+// log1p(S / c) keeps its digits where one token has nearly all the probability. Then the
+// alternatives, one search of the row each.
+KERNEL void __launch_bounds__(1024) slm_logprobs(LogpArgs a) {
+    __shared__ float red[16];
+    __shared__ uint64_t best[16];
+    const int64_t row = blockIdx.x;
+    const float* x = a.x + row * a.n;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    float m = NEG_INF;
+    for (int64_t i = tid; i < a.n; i += 1024) m = fmaxf(m, x[i]);
+    m = wave_max(m);
+    if (lane == 0) red[w] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; i++) m = fmaxf(m, red[i]);
+    float c = 0.0f, S = 0.0f, E = 0.0f;
+    for (int64_t i = tid; i < a.n; i += 1024) {
+        float v = x[i];
+        if (v == m) {
+            c += 1.0f;
+        } else {
+            float d = v - m, e = m == NEG_INF ? v - v : __builtin_amdgcn_exp2f(d * 1.44269504f);
+            S += e;
+            E = fmaf(e, fmaxf(d, -1e4f), E);
+        }
+    }
+    c = block_sum(c, red);
+    S = block_sum(S, red);
+    E = block_sum(E, red);
+    const bool none = m == NEG_INF && S == 0.0f;  // no logit above -inf (and no NaN)
+    float logl = logf(c) + log1pf(S / c);
+    if (tid == 0) {
+        float v = x[a.ids[row]];
+        a.lp[row] = none ? NEG_INF : (v - m) - logl;
+        if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - E / (c + S);
+    }
+    uint64_t last = ~0ull;  // the rank of the one before: key, then the lower index
+    for (int k = 0; k < a.top; k++) {
+        uint64_t mine = 0;
+        for (int64_t i = tid; i < a.n; i += 1024) {
+            uint64_t r = (uint64_t)logit_key(x[i]) << 32 | (0xffffffffu - (uint32_t)i);
+            if (r < last && r > mine) mine = r;
+        }
+        for (int o = 32; o; o >>= 1) {
+            uint64_t v = __shfl_xor(mine, o);
+            if (v > mine) mine = v;
+        }
+        __syncthreads();
+        if (lane == 0) best[w] = mine;
+        __syncthreads();
+        for (int i = 0; i < 16; i++)
+            if (best[i] > mine) mine = best[i];
+        last = mine;
+        if (tid == 0) {
+            uint32_t id = 0xffffffffu - (uint32_t)mine;
+            a.top_ids[row * a.top + k] = id;
+            a.top_lp[row * a.top + k] = none ? NEG_INF : (x[id] - m) - logl;
+        }
+    }
+}

@@ -30,12 +30,14 @@
 
 #include <emmintrin.h>
 
+#include "batch.h"
 #include "fusion.h"
 #include "scratch.h"
 #include "slm_hip.h"
 
 extern "C" const unsigned char slm_code_object[];
 extern "C" const size_t slm_code_object_size;
+extern "C" const unsigned char slm_batch_object[];
 
 namespace {
 
@@ -62,7 +64,7 @@ constexpr int64_t CU_COUNT = 256;           // MI355X compute units
 enum OpKind : uint32_t {
     OP_GATHER = 1, OP_COPY, OP_SHIFT, OP_COLUMNS, OP_LINEAR, OP_ADD, OP_ADD_ROW, OP_SCALE_ROWS,
     OP_MIX, OP_RMS, OP_SILU_MUL, OP_ROPE_TABLE, OP_ROPE, OP_L2NORM, OP_GLA, OP_STORE, OP_ATTEND,
-    OP_ARGMAX, OP_GROW
+    OP_ARGMAX, OP_GROW, OP_PSTORE, OP_PATTEND, OP_PEVICT, OP_LOGPROBS
 };
 
 // One operation, by value. p[] are device pointers (outputs first), n[] sizes, f[]
@@ -149,14 +151,39 @@ struct Kernels {
     hipFunction_t gemm2_48;                  // 48-row tiles, four waves of three row blocks
     hipFunction_t gemm2hk_16, gemm2hwk_16, gemm2h_48, gemm2hw_48;  // the same in fp16 mode
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
+    // several sequences over paged caches (batch.hip): fp32 and fp16 pages, head sizes to 64, 128, 256
+    hipFunction_t pstore[2], pattn[2][3], pjoin, pselect, pmove[2], logprobs;
 };
 
 }  // namespace
 
+// A batch of sequences over paged caches: what slm_hip_seqs_set was last given, and its device
+// copy — lengths, tokens seen, offsets of the new tokens' rows and of the superblocks, the
+// superblocks themselves ([n, sb] pairs) and the page table, in one block whose address stays.
+struct slm_seqs {
+    size_t page = 0, max_n = 0, max_pages = 0, max_items = 0;
+    unsigned char* dev = nullptr;
+    unsigned char* pin[2] = {nullptr, nullptr};  // two pinned uploads, as the step values
+    hipEvent_t ev[2] = {nullptr, nullptr};
+    int flip = 0;
+    size_t n = 0, width = 0, rows = 0, items = 0;
+    uint32_t max_len = 0, max_page = 0;
+    bool shared = false;        // a page that two places of the table name
+    bool fresh_shared = false;  // ... and new tokens go into
+    std::vector<uint32_t> len;
+    std::vector<uint8_t> uses;  // per page, while a table is read
+    size_t at_seen() const { return 4 * max_n; }
+    size_t at_first() const { return 8 * max_n; }
+    size_t at_ifirst() const { return 12 * max_n + 4; }
+    size_t at_items() const { return 16 * max_n + 8; }
+    size_t at_table() const { return at_items() + 8 * max_items; }
+    size_t bytes() const { return at_table() + 4 * max_n * max_pages; }
+};
+
 struct slm_hip {
     int device = 0;
     hipStream_t stream = nullptr;
-    hipModule_t mod = nullptr;
+    hipModule_t mod = nullptr, mod_batch = nullptr;
     Kernels k{};
     std::string err;
     char name[256] = {0};
@@ -190,6 +217,9 @@ struct slm_hip {
     size_t part_bytes = 0;
     float* gpart = nullptr;              // split partials of prompt GEMMs
     size_t gpart_bytes = 0;
+    float* pws = nullptr;                // paged attention's partials and scores, eviction's moves
+    size_t pws_bytes = 0;
+    std::map<uintptr_t, slm_seqs*> seqs; // live batches, by their device block
     std::vector<void*> retired;          // replaced internal buffers (launched work or cached
                                          // graphs may still use them): freed at close
     std::vector<void*> free_after_step;  // buffers freed while a step was recorded
@@ -843,6 +873,120 @@ int lower_attn_dec(slm_hip* c, const Op& o, std::vector<Rec>& out, bool defer) {
     return SLM_OK;
 }
 
+// ---- several sequences over paged caches, rows of logits ----
+
+SeqsDev seqs_dev(const slm_seqs* s, int64_t n, int64_t width) {
+    SeqsDev d{};
+    d.len = (const uint32_t*)s->dev;
+    d.seen = (const uint32_t*)(s->dev + s->at_seen());
+    d.first = (const uint32_t*)(s->dev + s->at_first());
+    d.ifirst = (const uint32_t*)(s->dev + s->at_ifirst());
+    d.items = (const uint32_t*)(s->dev + s->at_items());
+    d.table = (const uint32_t*)(s->dev + s->at_table());
+    d.n = (int32_t)n;
+    d.width = (int32_t)width;
+    return d;
+}
+
+// Bytes of the workspace that a paged attention of `items` superblocks uses.
+size_t pattend_bytes(size_t items, size_t heads, size_t dh, bool mass) {
+    return items * heads * (2 + dh + (mass ? SLM_PG_KEYS : 0)) * 4;
+}
+
+int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
+    const Kernels& k = c->k;
+    const float* const* p = o.p;
+    const int64_t* n = o.n;
+    if (o.kind == OP_LOGPROBS) {  // p0 lp, p1 entropy, p2 top ids, p3 top lp, p4 x; n0 m, n1 n, n2 top; dyn ids
+        LogpArgs a{};
+        a.x = p[4];
+        a.ids = (const uint32_t*)o.dyn;
+        a.lp = (float*)p[0];
+        a.ent = (float*)p[1];
+        a.top_ids = (uint32_t*)p[2];
+        a.top_lp = (float*)p[3];
+        a.m = n[0];
+        a.n = n[1];
+        a.top = (int32_t)n[2];
+        out.push_back(mk_desc(k.logprobs, (uint32_t)n[0], 1024, 0, a));
+        out.back().abytes = 4.0 * (double)n[0] * (double)(n[1] + 3 + 2 * n[2]);
+        return SLM_OK;
+    }
+    if (o.kind != OP_PSTORE && o.kind != OP_PATTEND && o.kind != OP_PEVICT)
+        return fail(c, SLM_E_INVALID, "unknown op %u", o.kind);
+    const void* dev = o.kind == OP_PSTORE ? p[6] : p[o.kind == OP_PATTEND ? 7 : 6];
+    auto it = c->seqs.find((uintptr_t)dev);
+    if (it == c->seqs.end()) return fail(c, SLM_E_INVALID, "paged: the batch is gone");
+    const SeqsDev s = seqs_dev(it->second, n[0], n[o.kind == OP_PSTORE ? 7 : 9]);
+    const int half = n[6] ? 1 : 0;
+    if (o.kind == OP_PSTORE) {  // p0 k, p1 v, p2 mass, p3 born, p4 and p5 new rows; n0 n, n1 rows, n2 kh, n3 page, n4 dh
+        PStoreArgs a{s, (void*)p[0], (void*)p[1], (float*)p[2], (uint32_t*)p[3], p[4], p[5],
+                     (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4]};
+        out.push_back(mk_desc(k.pstore[half], blocks_for((size_t)(n[1] * n[2] * n[4])), 256, 0, a));
+        return SLM_OK;
+    }
+    if (o.kind == OP_PATTEND) {
+        // p0 y, p1 mass out, p2 q, p3 k, p4 v, p5 mass, p6 born; n0 n, n1 heads, n2 kh, n3 page, n4 dh,
+        // n5 pages, n6 fp16, n7 superblocks, n8 gap; f0 scale, f1 one superblock each
+        PAttnArgs a{};
+        a.s = s;
+        a.y = (float*)p[0];
+        a.mass_out = (float*)p[1];
+        a.q = p[2];
+        a.k = p[3];
+        a.v = p[4];
+        a.mass = p[5];
+        a.born = (const uint32_t*)p[6];
+        a.heads = (int32_t)n[1];
+        a.kh = (int32_t)n[2];
+        a.page = (int32_t)n[3];
+        a.dh = (int32_t)n[4];
+        a.gap = n[8];
+        a.scale = o.f[0];
+        a.direct = o.f[1] != 0.0f;
+        a.r16 = c->fp16 ? 1 : 0;
+        if (!a.direct) {
+            a.ml = c->pws;
+            a.po = a.ml + 2 * n[7] * n[1];
+            if (a.mass_out) a.sc = a.po + n[7] * n[1] * n[4];
+        }
+        int nt = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
+        int64_t G = n[1] / n[2], dp = (int64_t)64 << nt;
+        uint32_t lds = (uint32_t)(4 * (G * dp + G * SLM_PG_KEYS + 4 * G * dp + 2 * G + SLM_PG_KEYS));
+        out.push_back(mk_desc(k.pattn[half][nt], (uint32_t)(n[7] * n[2]), 256, lds, a));
+        if (!a.direct)
+            out.push_back(mk_desc(k.pjoin, (uint32_t)(n[0] * n[1] + (a.mass_out ? n[7] * n[2] : 0)), 256, 0, a));
+        return SLM_OK;
+    }
+    // p0 k, p1 v, p2 mass out, p3 born out, p4 mass, p5 born; n0 n, n1 keep, n2 kh, n3 page, n4 dh, n5 pages,
+    // n6 fp16, n7 recent, n8 most moves
+    PEvictArgs a{};
+    a.s = s;
+    a.k = (void*)p[0];
+    a.v = (void*)p[1];
+    a.mass_out = (float*)p[2];
+    a.born_out = (uint32_t*)p[3];
+    a.mass = p[4];
+    a.born = (const uint32_t*)p[5];
+    a.kh = (int32_t)n[2];
+    a.page = (int32_t)n[3];
+    a.dh = (int32_t)n[4];
+    a.keep = (uint32_t)n[1];
+    a.recent = (uint32_t)n[7];
+    a.most = (uint32_t)n[8];
+    a.in_place = p[2] == p[4] && p[3] == p[5];
+    a.unit = half ? 2 : 4;
+    a.count = (uint32_t*)c->pws;
+    a.moves = a.count + n[0] * n[2];
+    out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, 0, a));
+    if (a.most) {
+        uint32_t blocks = (a.most + 63) / 64;
+        Rec r = mk_desc(k.pmove[half], (uint32_t)(n[0] * n[2]) * blocks, 256, 0, PMoveArgs{a, blocks});
+        out.push_back(r);
+    }
+    return SLM_OK;
+}
+
 int lower_one(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const Kernels& k = c->k;
     const float* const* p = o.p;
@@ -1004,7 +1148,7 @@ int lower_one(slm_hip* c, const Op& o, std::vector<Rec>& out) {
             return SLM_OK;
         }
     }
-    return fail(c, SLM_E_INVALID, "unknown op %u", o.kind);
+    return lower_batch(c, o, out);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1097,7 +1241,46 @@ int64_t wfloats(const Op& o) { return o.n[4] ? (o.n[0] * o.n[1] + 1) / 2 : o.n[0
 void op_ranges(const Op& o, std::vector<Range>& rd, std::vector<Range>& wr) {
     const float* const* p = o.p;
     const int64_t* n = o.n;
+    // what a paged op writes of a buffer of `count` floats (some of its slots: the rest stays)
+    auto slots = [&](const float* b, int64_t count) {
+        if (!b) return;
+        wr.push_back(rng(b, count));
+        rd.push_back(rng(b, count));
+    };
     switch (o.kind) {
+        case OP_PSTORE: {
+            int64_t sl = n[5] * n[2] * n[3];
+            slots(p[0], ring_floats(sl * n[4], n[6]));
+            slots(p[1], ring_floats(sl * n[4], n[6]));
+            slots(p[2], sl);
+            slots(p[3], sl);
+            for (int q = 4; q < 6; q++) rd.push_back(rng(p[q], n[1] * n[2] * n[4]));
+            break;
+        }
+        case OP_PATTEND: {
+            int64_t sl = n[5] * n[2] * n[3];
+            wr.push_back(rng(p[0], n[0] * n[1] * n[4]));
+            slots(p[1], sl);
+            rd.push_back(rng(p[2], n[0] * n[1] * n[4]));
+            for (int q = 3; q < 5; q++) rd.push_back(rng(p[q], ring_floats(sl * n[4], n[6])));
+            for (int q = 5; q < 7; q++)
+                if (p[q]) rd.push_back(rng(p[q], sl));
+            break;
+        }
+        case OP_PEVICT: {
+            int64_t sl = n[5] * n[2] * n[3];
+            for (int q = 0; q < 2; q++) slots(p[q], ring_floats(sl * n[4], n[6]));
+            for (int q = 2; q < 4; q++) slots(p[q], sl);
+            for (int q = 4; q < 6; q++) rd.push_back(rng(p[q], sl));
+            break;
+        }
+        case OP_LOGPROBS:
+            for (int q = 0; q < 2; q++)
+                if (p[q]) wr.push_back(rng(p[q], n[0]));
+            for (int q = 2; q < 4; q++)
+                if (p[q]) wr.push_back(rng(p[q], n[0] * n[2]));
+            rd.push_back(rng(p[4], n[0] * n[1]));
+            break;
         case OP_GATHER: wr.push_back(rng(p[0], n[0] * n[1])); rd.push_back(rng(p[1], 1)); break;
         case OP_ARGMAX:
             wr.push_back(rng(p[0], 2));
@@ -2954,6 +3137,25 @@ int need_ws(slm_hip* c, size_t bytes) {
     return SLM_OK;
 }
 
+int need_pws(slm_hip* c, size_t bytes) {
+    if (bytes <= c->pws_bytes) return SLM_OK;
+    size_t nb = std::max(bytes, c->pws_bytes * 2);
+    TRY(internal_realloc(c, (void**)&c->pws, nb));
+    c->pws_bytes = nb;
+    return SLM_OK;
+}
+
+// A batch's memory (nothing queued may still use it).
+void free_seqs(slm_hip* c, slm_seqs* s) {
+    if (s->dev && c->pooled.count((uintptr_t)s->dev)) dev_free(c, s->dev);
+    else if (s->dev) hipFree(s->dev);
+    for (int i = 0; i < 2; i++) {
+        if (s->pin[i]) hipHostFree(s->pin[i]);
+        if (s->ev[i]) hipEventDestroy(s->ev[i]);
+    }
+    delete s;
+}
+
 // ---- prompt lanes: running a step on one ----
 
 // The live allocation holding address a: its start and size (false: none does).
@@ -3044,8 +3246,8 @@ int run_lane_step(slm_hip* c, int* handled) {
     std::vector<Range> rd, wr;
     for (size_t i = 0; i < ops.size(); i++) {
         const Op& o = ops[i];
-        if (o.kind == OP_ARGMAX || o.kind == OP_GROW || (o.kind == OP_ATTEND && o.n[1] == 1))
-            return lane_fallback(c);
+        if (o.kind == OP_ARGMAX || o.kind >= OP_GROW || (o.kind == OP_ATTEND && o.n[1] == 1))
+            return lane_fallback(c);  // (the paged ops share the context's workspace)
         if (o.dyn && ((uintptr_t)o.dyn < dyn_a || (uintptr_t)o.dyn >= dyn_b)) return lane_fallback(c);
         rd.clear();
         wr.clear();
@@ -3627,6 +3829,21 @@ int load_kernels(slm_hip* c) {
         }
         TRY(get(&k.lin_small1[nv], "slm_linear_small_s" + n));
     }
+    struct {
+        hipFunction_t* f;
+        const char* n;
+    } batch[] = {{&k.pstore[0], "slm_paged_store"},      {&k.pstore[1], "slm_paged_store16"},
+                 {&k.pattn[0][0], "slm_paged_attn_1"},   {&k.pattn[0][1], "slm_paged_attn_2"},
+                 {&k.pattn[0][2], "slm_paged_attn_4"},   {&k.pattn[1][0], "slm_paged_attn16_1"},
+                 {&k.pattn[1][1], "slm_paged_attn16_2"}, {&k.pattn[1][2], "slm_paged_attn16_4"},
+                 {&k.pjoin, "slm_paged_join"},           {&k.pselect, "slm_paged_select"},
+                 {&k.pmove[0], "slm_paged_move16"},      {&k.pmove[1], "slm_paged_move8"},
+                 {&k.logprobs, "slm_logprobs"}};
+    for (auto& f : batch) {
+        hipError_t e = hipModuleGetFunction(f.f, c->mod_batch, f.n);
+        if (e != hipSuccess) return fail(c, SLM_E_HIP, "kernel %s: %s", f.n, hipGetErrorString(e));
+        c->fname[*f.f] = f.n;
+    }
     return SLM_OK;
 }
 
@@ -3670,6 +3887,7 @@ int slm_hip_open(int device, slm_hip** out) {
     OPEN_HIP(hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking));
     OPEN_HIP(slm_scratch_address((void**)&c->scratch));  // this device current (hipSetDevice above)
     OPEN_HIP(hipModuleLoadData(&c->mod, slm_code_object));
+    OPEN_HIP(hipModuleLoadData(&c->mod_batch, slm_batch_object));
     int rc = load_kernels(c);
     if (rc) return bail(rc);
     OPEN_HIP(hipHostMalloc((void**)&c->stage_host, STAGE_CAP, hipHostMallocDefault));
@@ -3749,6 +3967,8 @@ void slm_hip_close(slm_hip* c) {
     if (c->pick) hipFree(c->pick);
     release(c->part);
     release(c->gpart);
+    release(c->pws);
+    for (auto& q : c->seqs) free_seqs(c, q.second);
     for (int l = 1; l < (int)c->lanes.size(); l++) {
         auto& L = c->lanes[l];
         for (auto& cp : L.copies) release(cp.second.first);
@@ -3783,6 +4003,7 @@ void slm_hip_close(slm_hip* c) {
         if (c->read_ev[i]) hipEventDestroy(c->read_ev[i]);
     }
     if (c->mod) hipModuleUnload(c->mod);
+    if (c->mod_batch) hipModuleUnload(c->mod_batch);
     if (c->stream) hipStreamDestroy(c->stream);
     delete c;
 }
@@ -4712,6 +4933,407 @@ int slm_hip_attend_noalloc(slm_hip* c, float* y, float* scores, const float* q, 
     return SLM_OK;
 }
 
+// ---- several sequences over paged caches, rows of logits ----
+
+}  // extern "C"
+
+namespace {
+
+// A caller's own capture of the context's stream: the calls below are not part of it (their
+// launches are sized by the batch's lengths, and host arrays go up beside them).
+int refuse_capture(slm_hip* c, const char* op) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIPC(c, hipStreamIsCapturing(c->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+        return fail(c, SLM_E_UNSUPPORTED, "%s: the context's stream is being captured by the caller", op);
+    return SLM_OK;
+}
+
+bool meet(const void* p, size_t np, const void* q, size_t nq) {  // two byte ranges with a byte in common
+    return p && q && (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+}
+
+// The checks every paged call makes of its batch and its cache; *half: fp16 pages, *slots: the
+// slots of all pages and key heads.
+int check_pages(slm_hip* c, const char* op, const slm_seqs* s, const slm_pages* g, bool* half, size_t* slots) {
+    if (!c || !s || !g) return SLM_E_INVALID;
+    bool live = false;
+    for (auto& q : c->seqs) live = live || q.second == s;
+    if (!live) return fail(c, SLM_E_INVALID, "%s: not a batch of this context", op);
+    TRY(refuse_capture(c, op));
+    if (!g->pages || !g->page || !g->key_heads || !g->dh) return fail(c, SLM_E_INVALID, "%s: an empty cache", op);
+    if (g->page != s->page)
+        return fail(c, SLM_E_INVALID, "%s: pages of %zu slots, the batch's have %zu", op, g->page, s->page);
+    if (g->dh > 256 || g->dh % 4)
+        return fail(c, SLM_E_UNSUPPORTED, "%s: head size %zu (a multiple of 4 up to 256)", op, g->dh);
+    if (s->n && s->max_len && s->max_page >= g->pages)
+        return fail(c, SLM_E_BOUNDS, "%s: page %u of %zu", op, s->max_page, g->pages);
+    size_t n = 0;
+    if (g->key_heads > 65536 || __builtin_mul_overflow(g->pages, g->page * g->key_heads, &n) || n >= (size_t)1 << 31)
+        return fail(c, SLM_E_UNSUPPORTED, "%s: %zu pages of %zu slots and %zu key heads (2^31 rows or more)", op,
+                    g->pages, g->page, g->key_heads);
+    *slots = n;
+    size_t hk = half_count(c, g->k), hv = half_count(c, g->v);
+    *half = hk != 0;
+    if ((hk != 0) != (hv != 0)) return fail(c, SLM_E_INVALID, "%s: one fp16 buffer and one fp32 buffer", op);
+    if (hk) {
+        if (hk < n * g->dh || hv < n * g->dh)
+            return fail(c, SLM_E_BOUNDS, "%s: %zu rows of %zu in %zu and %zu halves", op, n, g->dh, hk, hv);
+    } else {
+        NEED(c, op, g->k, n * g->dh);
+        NEED(c, op, g->v, n * g->dh);
+    }
+    if (!aligned16(g->k) || !aligned16(g->v))
+        return fail(c, SLM_E_UNSUPPORTED, "%s: k and v must be 16-byte aligned", op);
+    if (g->mass) NEED(c, op, g->mass, n);
+    if (g->born) NEED(c, op, (const float*)g->born, n);
+    const size_t kb = n * g->dh * (hk ? 2 : 4);
+    if (meet(g->k, kb, g->v, kb) || meet(g->mass, n * 4, g->born, n * 4) || meet(g->k, kb, g->mass, n * 4) ||
+        meet(g->k, kb, g->born, n * 4) || meet(g->v, kb, g->mass, n * 4) || meet(g->v, kb, g->born, n * 4))
+        return fail(c, SLM_E_INVALID, "%s: the cache's buffers overlap", op);
+    return SLM_OK;
+}
+
+// Does [p, p + bytes) meet one of the cache's buffers?
+bool meets_cache(const slm_pages* g, size_t slots, bool half, const void* p, size_t bytes) {
+    size_t kb = slots * g->dh * (half ? 2 : 4);
+    return meet(p, bytes, g->k, kb) || meet(p, bytes, g->v, kb) || meet(p, bytes, g->mass, slots * 4) ||
+           meet(p, bytes, g->born, slots * 4);
+}
+
+}  // namespace
+
+extern "C" {
+
+int slm_hip_alloc_pages(slm_hip* c, size_t pages, size_t key_heads, size_t page, size_t dh, int half, float** out) {
+    if (!c || !out) return SLM_E_INVALID;
+    size_t n = 0;
+    if (__builtin_mul_overflow(pages, key_heads, &n) || __builtin_mul_overflow(n, page, &n) ||
+        __builtin_mul_overflow(n, dh, &n) || n > (size_t)1 << 46)
+        return fail(c, SLM_E_MEMORY, "alloc_pages: %zu x %zu x %zu x %zu", pages, key_heads, page, dh);
+    return half ? slm_hip_alloc_half(c, n, out) : slm_hip_alloc(c, n, out);
+}
+
+int slm_hip_seqs_new(slm_hip* c, size_t page, size_t max_n, size_t max_pages, slm_seqs** out) {
+    if (!c || !out) return SLM_E_INVALID;
+    *out = nullptr;
+    if (!page || !max_n || !max_pages) return fail(c, SLM_E_INVALID, "seqs_new: a size of 0");
+    size_t slots = 0, cells = 0;
+    if (max_n > 65536 || __builtin_mul_overflow(page, max_pages, &slots) || slots >= (size_t)1 << 31 ||
+        __builtin_mul_overflow(max_n, max_pages, &cells) || cells > (size_t)1 << 26 ||
+        max_n * ((slots + SLM_PG_KEYS - 1) / SLM_PG_KEYS) > (size_t)1 << 26)
+        return fail(c, SLM_E_UNSUPPORTED, "seqs_new: %zu sequences of %zu pages of %zu slots", max_n, max_pages, page);
+    TRY(refuse_capture(c, "seqs_new"));
+    slm_seqs* s = new slm_seqs();
+    s->page = page;
+    s->max_n = max_n;
+    s->max_pages = max_pages;
+    // (the count of superblocks in a launch is rounded up by at most an eighth)
+    s->max_items = max_n * ((slots + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
+    s->max_items += s->max_items / 8 + 1;
+    hipError_t e = dev_alloc(c, s->bytes(), (void**)&s->dev);
+    for (int i = 0; i < 2 && e == hipSuccess; i++) {
+        e = hipHostMalloc((void**)&s->pin[i], s->bytes(), hipHostMallocDefault);
+        if (e == hipSuccess) e = hipEventCreateWithFlags(&s->ev[i], hipEventDisableTiming);
+    }
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        free_seqs(c, s);
+        return fail(c, SLM_E_MEMORY, "seqs_new: %s", hipGetErrorString(e));
+    }
+    c->seqs[(uintptr_t)s->dev] = s;
+    *out = s;
+    return SLM_OK;
+}
+
+int slm_hip_seqs_free(slm_hip* c, slm_seqs* s) {
+    if (!c) return SLM_E_INVALID;
+    if (!s) return SLM_OK;
+    for (auto it = c->seqs.begin(); it != c->seqs.end(); ++it) {
+        if (it->second != s) continue;
+        TRY(taint(c));  // a step's calls recorded so far run first
+        drop_graphs(c);
+        HIPC(c, hipStreamSynchronize(mstream(c)));
+        c->seqs.erase(it);
+        free_seqs(c, s);
+        return SLM_OK;
+    }
+    return fail(c, SLM_E_INVALID, "seqs_free: not a batch of this context");
+}
+
+int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, const uint32_t* fresh, const uint32_t* seen,
+                     const uint32_t* table, size_t width) {
+    if (!c || !s || (n && (!len || !table))) return SLM_E_INVALID;
+    bool live = false;
+    for (auto& q : c->seqs) live = live || q.second == s;
+    if (!live) return fail(c, SLM_E_INVALID, "seqs_set: not a batch of this context");
+    TRY(refuse_capture(c, "seqs_set"));
+    if (n > s->max_n) return fail(c, SLM_E_BOUNDS, "seqs_set: %zu sequences, room for %zu", n, s->max_n);
+    size_t used_max = 1, rows = 0, items = 0;
+    uint32_t max_len = 0, max_page = 0;
+    auto pages_of = [&](uint32_t l) { return (l + s->page - 1) / s->page; };
+    auto fresh_of = [&](size_t b) { return fresh ? fresh[b] : len[b] ? 1u : 0u; };
+    for (size_t b = 0; b < n; b++) {
+        size_t used = pages_of(len[b]);
+        if (used > s->max_pages)
+            return fail(c, SLM_E_BOUNDS, "seqs_set: sequence %zu has %u tokens, room for %zu", b, len[b], s->max_pages * s->page);
+        if (used > width) return fail(c, SLM_E_BOUNDS, "seqs_set: %zu pages of sequence %zu in a table of %zu", used, b, width);
+        if (fresh_of(b) > len[b])
+            return fail(c, SLM_E_INVALID, "seqs_set: %u new tokens of %u in sequence %zu", fresh_of(b), len[b], b);
+        if (seen && seen[b] < len[b])
+            return fail(c, SLM_E_INVALID, "seqs_set: sequence %zu has seen %u tokens and holds %u", b, seen[b], len[b]);
+        for (size_t i = 0; i < used; i++) max_page = std::max(max_page, table[b * width + i]);
+        used_max = std::max(used_max, used);
+        max_len = std::max(max_len, len[b]);
+        rows += fresh_of(b);
+        items += std::max<size_t>(1, ((size_t)len[b] + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
+    }
+    if (max_page >= (uint32_t)1 << 27) return fail(c, SLM_E_UNSUPPORTED, "seqs_set: page %u (2^27 or more)", max_page);
+    if (rows >= (size_t)1 << 31) return fail(c, SLM_E_UNSUPPORTED, "seqs_set: %zu new tokens", rows);
+    TRY(taint(c));  // a step's calls recorded so far run with the batch as it was
+    // Launches are sized by these, and a kept step is kept for its launches: the table's width
+    // and the count of superblocks go up in steps, so that a batch that grows by a token changes
+    // neither most of the time.
+    size_t w = std::min(s->max_pages, (used_max + 15) / 16 * 16);
+    size_t step = 1;
+    while (step * 16 <= items) step *= 2;
+    size_t all = (items + step - 1) / step * step;
+
+    s->uses.assign(n ? max_page + 1 : 0, 0);
+    s->shared = s->fresh_shared = false;
+    for (size_t b = 0; b < n; b++)
+        for (size_t i = 0; i < pages_of(len[b]); i++) {
+            uint8_t& u = s->uses[table[b * width + i]];
+            if (u) s->shared = true;
+            u = u ? 2 : 1;
+        }
+    if (s->shared)
+        for (size_t b = 0; b < n; b++)
+            if (uint32_t f = fresh_of(b))
+                for (size_t i = (len[b] - f) / s->page; i < pages_of(len[b]); i++)
+                    if (s->uses[table[b * width + i]] > 1) s->fresh_shared = true;
+
+    int k = s->flip ^= 1;
+    HIPC(c, hipEventSynchronize(s->ev[k]));
+    unsigned char* h = s->pin[k];
+    uint32_t* hl = (uint32_t*)h;
+    uint32_t* hs = (uint32_t*)(h + s->at_seen());
+    uint32_t* hf = (uint32_t*)(h + s->at_first());
+    uint32_t* hi = (uint32_t*)(h + s->at_ifirst());
+    uint32_t* ht = (uint32_t*)(h + s->at_items());
+    uint32_t* hp = (uint32_t*)(h + s->at_table());
+    uint32_t row = 0, item = 0;
+    for (size_t b = 0; b < n; b++) {
+        hl[b] = len[b];
+        hs[b] = seen ? seen[b] : len[b];
+        hf[b] = row;
+        hi[b] = item;
+        row += fresh_of(b);
+        uint32_t nsb = (uint32_t)std::max<size_t>(1, ((size_t)len[b] + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
+        for (uint32_t z = 0; z < nsb; z++, item++) {
+            ht[2 * item] = (uint32_t)b;
+            ht[2 * item + 1] = z;
+        }
+        size_t used = pages_of(len[b]);
+        std::memcpy(hp + b * w, table + b * width, used * 4);
+        std::memset(hp + b * w + used, 0, (w - used) * 4);
+    }
+    hf[n] = row;
+    hi[n] = item;
+    for (size_t i = items; i < all; i++) ht[2 * i] = ht[2 * i + 1] = SLM_NO_SEQ;
+    hipStream_t st = mstream(c);
+    s->n = 0;  // (nothing until both copies are queued)
+    HIPC(c, hipMemcpyAsync(s->dev, h, s->at_items() + 8 * all, hipMemcpyHostToDevice, st));
+    if (n) HIPC(c, hipMemcpyAsync(s->dev + s->at_table(), hp, 4 * n * w, hipMemcpyHostToDevice, st));
+    HIPC(c, hipEventRecord(s->ev[k], st));
+    s->n = n;
+    s->width = w;
+    s->rows = rows;
+    s->items = all;
+    s->max_len = max_len;
+    s->max_page = max_page;
+    s->len.assign(len, len + n);
+    return SLM_OK;
+}
+
+int slm_hip_paged_store(slm_hip* c, slm_seqs* s, const slm_pages* g, const float* k, const float* v) {
+    bool half = false;
+    size_t slots = 0;
+    TRY(check_pages(c, "paged_store", s, g, &half, &slots));
+    if (!s->n || !s->rows) return SLM_OK;
+    size_t n = s->rows * g->key_heads * g->dh;
+    NEED(c, "paged_store", k, n);
+    NEED(c, "paged_store", v, n);
+    if (meets_cache(g, slots, half, k, n * 4) || meets_cache(g, slots, half, v, n * 4))
+        return fail(c, SLM_E_INVALID, "paged_store: the new rows lie in the cache");
+    if (s->fresh_shared)
+        return fail(c, SLM_E_INVALID, "paged_store: a page that takes new tokens is in the table twice");
+    Op o = op(OP_PSTORE);
+    o.p[0] = g->k;
+    o.p[1] = g->v;
+    o.p[2] = g->mass;
+    o.p[3] = (const float*)g->born;
+    o.p[4] = k;
+    o.p[5] = v;
+    o.p[6] = (const float*)s->dev;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)s->rows;
+    o.n[2] = (int64_t)g->key_heads;
+    o.n[3] = (int64_t)g->page;
+    o.n[4] = (int64_t)g->dh;
+    o.n[5] = (int64_t)g->pages;
+    o.n[6] = half;
+    o.n[7] = (int64_t)s->width;
+    return submit(c, o);
+}
+
+int slm_hip_paged_attend(slm_hip* c, slm_seqs* s, const slm_pages* g, float* y, float* mass_out, const float* q,
+                         size_t heads, size_t gap, float scale) {
+    bool half = false;
+    size_t slots = 0;
+    TRY(check_pages(c, "paged_attend", s, g, &half, &slots));
+    if (!heads || heads % g->key_heads)
+        return fail(c, SLM_E_INVALID, "paged_attend: %zu heads over %zu key heads", heads, g->key_heads);
+    if (heads / g->key_heads > 16)
+        return fail(c, SLM_E_UNSUPPORTED, "paged_attend: %zu query heads per key head", heads / g->key_heads);
+    if (!s->n) return SLM_OK;
+    size_t n = s->n * heads * g->dh;
+    NEED(c, "paged_attend", y, n);
+    NEED(c, "paged_attend", q, n);
+    if (!aligned16(q)) return fail(c, SLM_E_UNSUPPORTED, "paged_attend: q must be 16-byte aligned");
+    if (meet(y, n * 4, q, n * 4) || meets_cache(g, slots, half, y, n * 4))
+        return fail(c, SLM_E_INVALID, "paged_attend: y lies in an input");
+    if (mass_out) {
+        if (!g->mass) return fail(c, SLM_E_INVALID, "paged_attend: weights to add to nothing (the cache has no mass)");
+        NEED(c, "paged_attend", mass_out, slots);
+        slm_pages rest = *g;
+        rest.mass = mass_out == g->mass ? nullptr : g->mass;
+        if (meets_cache(&rest, slots, half, mass_out, slots * 4) || meet(mass_out, slots * 4, y, n * 4) ||
+            meet(mass_out, slots * 4, q, n * 4))
+            return fail(c, SLM_E_INVALID, "paged_attend: mass_out lies in an input other than mass, or in y");
+        if (s->shared) return fail(c, SLM_E_INVALID, "paged_attend: weights for pages that are in the table twice");
+    }
+    bool direct = s->max_len <= SLM_PG_KEYS;
+    if (s->items * std::max(heads, (size_t)1) >= (size_t)1 << 31)
+        return fail(c, SLM_E_UNSUPPORTED, "paged_attend: %zu superblocks of %zu heads", s->items, heads);
+    if (!direct) TRY(need_pws(c, pattend_bytes(s->items, heads, g->dh, mass_out != nullptr)));
+    Op o = op(OP_PATTEND);
+    o.p[0] = y;
+    o.p[1] = mass_out;
+    o.p[2] = q;
+    o.p[3] = g->k;
+    o.p[4] = g->v;
+    o.p[5] = mass_out ? g->mass : nullptr;
+    o.p[6] = gap ? (const float*)g->born : nullptr;  // (positions matter to a gap alone)
+    o.p[7] = (const float*)s->dev;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)heads;
+    o.n[2] = (int64_t)g->key_heads;
+    o.n[3] = (int64_t)g->page;
+    o.n[4] = (int64_t)g->dh;
+    o.n[5] = (int64_t)g->pages;
+    o.n[6] = half;
+    o.n[7] = (int64_t)s->items;
+    o.n[8] = (int64_t)std::min(gap, (size_t)1 << 50);
+    o.n[9] = (int64_t)s->width;
+    // scores in powers of two (fp16 mode: the dtype's scalar first, as slm_hip_attend)
+    o.f[0] = (float)((double)(c->fp16 ? round16(scale) : scale) * 1.4426950408889634);
+    o.f[1] = direct ? 1.0f : 0.0f;
+    return submit(c, o);
+}
+
+int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass_out, uint32_t* born_out, size_t keep,
+                        size_t recent) {
+    bool half = false;
+    size_t slots = 0;
+    TRY(check_pages(c, "paged_evict", s, g, &half, &slots));
+    if (!mass_out || !born_out || !g->mass || !g->born)
+        return fail(c, SLM_E_INVALID, "paged_evict: weights and positions are needed");
+    if (!keep || recent > keep) return fail(c, SLM_E_INVALID, "paged_evict: %zu kept, %zu of them the newest", keep, recent);
+    NEED(c, "paged_evict", mass_out, slots);
+    NEED(c, "paged_evict", (const float*)born_out, slots);
+    slm_pages rest = *g;
+    if (mass_out == g->mass && born_out == g->born) rest.mass = nullptr, rest.born = nullptr;
+    if (meets_cache(&rest, slots, half, mass_out, slots * 4) || meets_cache(&rest, slots, half, born_out, slots * 4) ||
+        meet(mass_out, slots * 4, born_out, slots * 4))
+        return fail(c, SLM_E_INVALID, "paged_evict: mass_out and born_out are the cache's own, or lie in no input");
+    if (s->shared) return fail(c, SLM_E_INVALID, "paged_evict: a page is in the table twice");
+    if (!s->n) return SLM_OK;
+    keep = std::min(keep, (size_t)UINT32_MAX);
+    recent = std::min(recent, (size_t)UINT32_MAX);
+    uint64_t most = 0;
+    for (uint32_t l : s->len)
+        if (l > keep) most = std::max<uint64_t>(most, std::min<uint64_t>(keep, l - keep));
+    bool in_place = !rest.mass;
+    if (!most && in_place) return SLM_OK;
+    // (a kept step's launches hold for its most moves: it goes up in steps)
+    uint64_t step = 64;
+    while (step * 8 <= most) step *= 2;
+    most = (most + step - 1) / step * step;
+    size_t pairs = s->n * g->key_heads;
+    if (pairs >= (size_t)1 << 24 || pairs * ((most + 63) / 64) >= (size_t)1 << 31)
+        return fail(c, SLM_E_UNSUPPORTED, "paged_evict: %zu sequences of %zu key heads", s->n, g->key_heads);
+    TRY(need_pws(c, pairs * 4 + pairs * 2 * most * 4));
+    Op o = op(OP_PEVICT);
+    o.p[0] = g->k;
+    o.p[1] = g->v;
+    o.p[2] = mass_out;
+    o.p[3] = (const float*)born_out;
+    o.p[4] = g->mass;
+    o.p[5] = (const float*)g->born;
+    o.p[6] = (const float*)s->dev;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)keep;
+    o.n[2] = (int64_t)g->key_heads;
+    o.n[3] = (int64_t)g->page;
+    o.n[4] = (int64_t)g->dh;
+    o.n[5] = (int64_t)g->pages;
+    o.n[6] = half;
+    o.n[7] = (int64_t)recent;
+    o.n[8] = (int64_t)most;
+    o.n[9] = (int64_t)s->width;
+    return submit(c, o);
+}
+
+int slm_hip_logprobs(slm_hip* c, float* lp, float* entropy, uint32_t* top_ids, float* top_lp, size_t top, const float* x,
+                     const uint32_t* ids, size_t m, size_t n) {
+    if (!c || (m && !ids)) return SLM_E_INVALID;
+    TRY(refuse_capture(c, "logprobs"));
+    if (!m) return SLM_OK;
+    if (!n || (top && (!top_ids || !top_lp)) || top > n)
+        return fail(c, SLM_E_INVALID, "logprobs: %zu alternatives of %zu logits", top, n);
+    if (top > SLM_TOP_MAX) return fail(c, SLM_E_UNSUPPORTED, "logprobs: %zu alternatives (at most %d)", top, SLM_TOP_MAX);
+    if (n > (size_t)1 << 28 || m >= (size_t)1 << 22 || m * n > (size_t)1 << 40)  // (a launch's 32-bit count of threads)
+        return fail(c, SLM_E_UNSUPPORTED, "logprobs: %zu rows of %zu", m, n);
+    NEED(c, "logprobs", x, m * n);
+    NEED(c, "logprobs", lp, m);
+    if (entropy) NEED(c, "logprobs", entropy, m);
+    if (top) {
+        NEED(c, "logprobs", (const float*)top_ids, m * top);
+        NEED(c, "logprobs", top_lp, m * top);
+    }
+    const void* outs[4] = {lp, entropy, top ? top_ids : nullptr, top ? top_lp : nullptr};
+    const size_t bytes[4] = {m * 4, m * 4, m * top * 4, m * top * 4};
+    for (int i = 0; i < 4; i++) {
+        bool bad = meet(outs[i], bytes[i], x, m * n * 4);
+        for (int j = 0; j < i; j++) bad = bad || meet(outs[i], bytes[i], outs[j], bytes[j]);
+        if (bad) return fail(c, SLM_E_INVALID, "logprobs: the outputs overlap each other or the logits");
+    }
+    for (size_t i = 0; i < m; i++)
+        if (ids[i] >= n) return fail(c, SLM_E_BOUNDS, "logprobs: token %u of %zu logits", ids[i], n);
+    Op o = op(OP_LOGPROBS);
+    o.p[0] = lp;
+    o.p[1] = entropy;
+    o.p[2] = top ? (const float*)top_ids : nullptr;
+    o.p[3] = top ? top_lp : nullptr;
+    o.p[4] = x;
+    o.n[0] = (int64_t)m;
+    o.n[1] = (int64_t)n;
+    o.n[2] = (int64_t)top;
+    TRY(stage(c, ids, m * 4, &o.dyn));
+    return submit(c, o);
+}
+
 // ---- diagnostics ----
 
 int slm_hip_stream(slm_hip* c, void** out) {
@@ -4734,6 +5356,8 @@ int slm_hip_mem_info(slm_hip* c, size_t* free_bytes, size_t* total_bytes, size_t
     direct(c->ws, c->ws_bytes);
     direct(c->part, c->part_bytes);
     direct(c->gpart, c->gpart_bytes);
+    direct(c->pws, c->pws_bytes);
+    for (auto& q : c->seqs) direct(q.second->dev, q.second->bytes());
     *held_bytes = held;
     return SLM_OK;
 }
