@@ -517,74 +517,224 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < 16; i++) s += red[i];
-    return s;
+__device__ __forceinline__ float logit_of(uint32_t key) {  // (a number, not a NaN's key)
+    return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// A workgroup of 1024 a row: its maximum, then L = c + S and E = sum e^(x-M) (x-M), where c
-// logits are the maximum M and S sums e^(x-M) over the others, so that log L = log c +
-// log1p(S / c) keeps its digits where one token has nearly all the probability. Then the
-// alternatives, one search of the row each.
-KERNEL void __launch_bounds__(1024) slm_logprobs(LogpArgs a) {
-    __shared__ float red[16];
-    __shared__ uint64_t best[16];
-    const int64_t row = blockIdx.x;
-    const float* x = a.x + row * a.n;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    float m = NEG_INF;
-    for (int64_t i = tid; i < a.n; i += 1024) m = fmaxf(m, x[i]);
-    m = wave_max(m);
-    if (lane == 0) red[w] = m;
-    __syncthreads();
-    for (int i = 0; i < 16; i++) m = fmaxf(m, red[i]);
-    float c = 0.0f, S = 0.0f, E = 0.0f;
-    for (int64_t i = tid; i < a.n; i += 1024) {
-        float v = x[i];
-        if (v == m) {
-            c += 1.0f;
-        } else {
-            float d = v - m, e = m == NEG_INF ? v - v : __builtin_amdgcn_exp2f(d * 1.44269504f);
-            S += e;
-            E = fmaf(e, fmaxf(d, -1e4f), E);
+// Part of a row's sums: its maximum m, the count c of logits equal to it, and over the others
+// S = sum e^(x-m) and E = sum e^(x-m) (x-m); so log L = log c + log1p(S / c) keeps its digits
+// where one token has nearly all the probability. A NaN is in S.
+struct RowSum {
+    float m, c, S, E;
+    __device__ __forceinline__ void raise(float to) {  // the same sum about a maximum `to` >= m
+        if (!(to > m)) return;
+        if (m > NEG_INF) {
+            float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f), all = c + S;
+            E = f * fmaf(fmaxf(d, -1e4f), all, E);
+            S = f * all;
         }
+        c = 0.0f;
+        m = to;
     }
-    c = block_sum(c, red);
-    S = block_sum(S, red);
-    E = block_sum(E, red);
-    const bool none = m == NEG_INF && S == 0.0f;  // no logit above -inf (and no NaN)
-    float logl = logf(c) + log1pf(S / c);
-    if (tid == 0) {
-        float v = x[a.ids[row]];
-        a.lp[row] = none ? NEG_INF : (v - m) - logl;
-        if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - E / (c + S);
+    __device__ __forceinline__ void add(float x) {  // x <= m, or a NaN; m > -inf
+        float d = x - m, e = __builtin_amdgcn_exp2f(d * 1.44269504f);
+        S += x == m ? 0.0f : e;
+        c += x == m ? 1.0f : 0.0f;
+        E = fmaf(e, fmaxf(d, -1e4f), E);  // (e^-1e4 is 0: an impossible token adds nothing)
     }
-    uint64_t last = ~0ull;  // the rank of the one before: key, then the lower index
-    for (int k = 0; k < a.top; k++) {
-        uint64_t mine = 0;
-        for (int64_t i = tid; i < a.n; i += 1024) {
-            uint64_t r = (uint64_t)logit_key(x[i]) << 32 | (0xffffffffu - (uint32_t)i);
-            if (r < last && r > mine) mine = r;
-        }
-        for (int o = 32; o; o >>= 1) {
-            uint64_t v = __shfl_xor(mine, o);
-            if (v > mine) mine = v;
-        }
-        __syncthreads();
-        if (lane == 0) best[w] = mine;
-        __syncthreads();
-        for (int i = 0; i < 16; i++)
-            if (best[i] > mine) mine = best[i];
-        last = mine;
-        if (tid == 0) {
-            uint32_t id = 0xffffffffu - (uint32_t)mine;
-            a.top_ids[row * a.top + k] = id;
-            a.top_lp[row * a.top + k] = none ? NEG_INF : (x[id] - m) - logl;
-        }
+};
+
+// The largest t (to 20 bits) such that at least `want` of the wave's 64 keys are >= t: by its
+// bits from above, a ballot each; two wants at once.
+__device__ __forceinline__ void wave_nth(uint32_t key, int want0, int want1, uint32_t& t0, uint32_t& t1) {
+    t0 = t1 = 0;
+    for (int bit = 31; bit >= 12; bit--) {
+        uint32_t c0 = t0 | (1u << bit), c1 = t1 | (1u << bit);
+        if (__popcll(__ballot(key >= c0)) >= want0) t0 = c0;
+        if (__popcll(__ballot(key >= c1)) >= want1) t1 = c1;
     }
 }
+
+// A workgroup of W waves a row, in panels of W·2048 logits that a wave holds in registers while
+// it adds them up: the row is read once. The alternatives are those of largest rank (key, then
+// the lower index), found without a second look at the row: `top` logits at least as large as
+// a bound T exist if every wave has ceil(top / W) lanes whose own maximum reaches it (the least
+// over the waves of that lane's maximum), or one wave has `top` of them (the most over the
+// waves): T is the larger of the two, from the first panel. Whatever reaches T goes into the
+// wave's list, which is cut to its `top` best when more than 64 are in it (T rises with it);
+// about 5·top of a row of 32000 reach T. Of what the lists hold at the end, those that reach a
+// second bound of the same kind are ranked by counting the better ones.
+template <int W>
+__device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
+    __shared__ uint64_t list[W][128], fin[W * 64];
+    __shared__ uint32_t cnts[W], bound[W][2], nfin;
+    __shared__ float sums[W][4];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.top;
+    const float* x = a.x + row * a.n;
+    // whole 16 bytes from the last such address at or before the row's first logit
+    const int a0 = (int)(((uintptr_t)x >> 2) & 3), end = (int)a.n + a0;
+    const float* xa = x - a0;
+    const int fair = (top + W - 1) / W;
+    const float given = x[a.ids[row]];
+    if (tid == 0) nfin = 0;
+
+    auto threshold = [&](uint32_t key) -> uint32_t {
+        uint32_t t0, t1;
+        wave_nth(key, top, fair, t0, t1);
+        if (lane == 0) {
+            bound[w][0] = t0;
+            bound[w][1] = t1;
+        }
+        __syncthreads();
+        uint32_t most = bound[0][0], least = bound[0][1];
+#pragma unroll
+        for (int i = 1; i < W; i++) {
+            most = max(most, bound[i][0]);
+            least = min(least, bound[i][1]);
+        }
+        __syncthreads();
+        return max(most, least);
+    };
+
+    RowSum s{NEG_INF, 0.0f, 0.0f, 0.0f};
+    uint64_t least = 0;  // what a logit's rank must pass to be listed
+    float least_x = NEG_INF;
+    int cnt = 0;
+    auto cut = [&]() {  // the list's `top` best, best first
+        uint64_t e0 = lane < cnt ? list[w][lane] : 0, e1 = lane + 64 < cnt ? list[w][lane + 64] : 0;
+        int r0 = 0, r1 = 0;
+        for (int i = 0; i < cnt; i++) {
+            uint64_t o = list[w][i];
+            r0 += o > e0;
+            r1 += o > e1;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (e0 && r0 < top) list[w][r0] = e0;
+        if (e1 && r1 < top) list[w][r1] = e1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (cnt >= top) {
+            cnt = top;
+            least = list[w][top - 1];
+            least = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(least >> 32)) << 32 |
+                    (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)least);
+            least_x = least >> 32 ? logit_of((uint32_t)(least >> 32)) : NEG_INF;
+        }
+    };
+
+    for (int p0 = 0; p0 < end; p0 += W * 2048) {
+        f4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            int at = p0 + ((j >> 2) * W + w) * 1024 + (j & 3) * 256 + lane * 4;
+            if (at >= a0 && at + 4 <= end) {
+                v[j] = *(const f4*)(xa + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[j][e] = at + e >= a0 && at + e < end ? xa[at + e] : NEG_INF;
+            }
+        }
+        float m = NEG_INF;
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(fmaxf(m, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
+        s.raise(m);
+        if (s.m > NEG_INF) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s.add(v[j][e]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s.S += v[j][e] == NEG_INF ? 0.0f : v[j][e];  // (a NaN)
+        }
+        if (top) {
+            if (p0 == 0) {
+                // (a lane of nothing but NaNs and -infinities bounds nothing)
+                uint32_t t = threshold(m > NEG_INF ? logit_key(m) : 0);
+                least = t ? ((uint64_t)t << 32) - 1 : 0;
+                least_x = t ? logit_of(t) : NEG_INF;
+            }
+            if (__ballot(m >= least_x)) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float m4 = fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w));
+                    if (!__ballot(!(m4 < least_x))) continue;
+                    int at = p0 + ((j >> 2) * W + w) * 1024 + (j & 3) * 256 + lane * 4 - a0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        uint64_t r = (uint64_t)logit_key(v[j][e]) << 32 | (0xffffffffu - (uint32_t)(at + e));
+                        bool in = at + e >= 0 && at + e < (int)a.n && r > least;
+                        uint64_t mask = __ballot(in);
+                        if (!mask) continue;
+                        if (in) list[w][cnt + lanes_below(mask)] = r;
+                        cnt += __popcll(mask);
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                        if (cnt > 64) cut();
+                    }
+                }
+            }
+        }
+    }
+
+    // the row's sums: the wave's, then the waves' in order
+    float m = wave_max(s.m);
+    s.raise(m);
+    s.c = wave_sum(s.c);
+    s.S = wave_sum(s.S);
+    s.E = wave_sum(s.E);
+    if (lane == 0) {
+        sums[w][0] = m;
+        sums[w][1] = s.c;
+        sums[w][2] = s.S;
+        sums[w][3] = s.E;
+        cnts[w] = cnt;
+    }
+    __syncthreads();
+    m = sums[0][0];
+    int total = cnts[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) {
+        m = fmaxf(m, sums[i][0]);
+        total += cnts[i];
+    }
+    float c = 0.0f, S = 0.0f, E = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        RowSum q{sums[i][0], sums[i][1], sums[i][2], sums[i][3]};
+        q.raise(m);
+        c += q.c;
+        S += q.S;
+        E += q.E;
+    }
+    const bool none = m == NEG_INF && S == 0.0f;  // no logit above -inf (and no NaN)
+    const float logl = logf(c) + log1pf(S / c);
+    if (tid == 0) {
+        a.lp[row] = none ? NEG_INF : (given - m) - logl;
+        if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - E / (c + S);
+    }
+    if (!top) return;
+    uint64_t e = lane < cnt ? list[w][lane] : 0;
+    if (total > 128) {
+        uint32_t t = threshold((uint32_t)(e >> 32));
+        if ((uint32_t)(e >> 32) < t) e = 0;
+    }
+    if (e) fin[atomicAdd(&nfin, 1u)] = e;
+    __syncthreads();
+    const int n = nfin;
+    if (tid >= n) return;
+    e = fin[tid];
+    int r = 0;
+    for (int i = 0; i < n; i++) r += fin[i] > e;
+    if (r < top) {
+        uint32_t key = (uint32_t)(e >> 32), id = 0xffffffffu - (uint32_t)e;
+        a.top_ids[row * top + r] = id;
+        a.top_lp[row * top + r] = none ? NEG_INF : ((key ? logit_of(key) : __builtin_nanf("")) - m) - logl;
+    }
+}
+KERNEL void __launch_bounds__(256) slm_logprobs_4(LogpArgs a) { logprobs_body<4>(a); }
+KERNEL void __launch_bounds__(1024) slm_logprobs_16(LogpArgs a) { logprobs_body<16>(a); }

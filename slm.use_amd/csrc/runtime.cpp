@@ -152,7 +152,7 @@ struct Kernels {
     hipFunction_t gemm2hk_16, gemm2hwk_16, gemm2h_48, gemm2hw_48;  // the same in fp16 mode
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages, head sizes to 64, 128, 256
-    hipFunction_t pstore[2], pattn[2][3], pjoin, pselect, pmove[2], logprobs;
+    hipFunction_t pstore[2], pattn[2][3], pjoin, pselect, pmove[2], logprobs[2];
 };
 
 }  // namespace
@@ -908,7 +908,8 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         a.m = n[0];
         a.n = n[1];
         a.top = (int32_t)n[2];
-        out.push_back(mk_desc(k.logprobs, (uint32_t)n[0], 1024, 0, a));
+        bool wide = n[1] > 8192;  // four waves a row, or sixteen
+        out.push_back(mk_desc(k.logprobs[wide], (uint32_t)n[0], wide ? 1024 : 256, 0, a));
         out.back().abytes = 4.0 * (double)n[0] * (double)(n[1] + 3 + 2 * n[2]);
         return SLM_OK;
     }
@@ -3838,7 +3839,7 @@ int load_kernels(slm_hip* c) {
                  {&k.pattn[1][1], "slm_paged_attn16_2"}, {&k.pattn[1][2], "slm_paged_attn16_4"},
                  {&k.pjoin, "slm_paged_join"},           {&k.pselect, "slm_paged_select"},
                  {&k.pmove[0], "slm_paged_move16"},      {&k.pmove[1], "slm_paged_move8"},
-                 {&k.logprobs, "slm_logprobs"}};
+                 {&k.logprobs[0], "slm_logprobs_4"},     {&k.logprobs[1], "slm_logprobs_16"}};
     for (auto& f : batch) {
         hipError_t e = hipModuleGetFunction(f.f, c->mod_batch, f.n);
         if (e != hipSuccess) return fail(c, SLM_E_HIP, "kernel %s: %s", f.n, hipGetErrorString(e));
