@@ -15,7 +15,7 @@ struct SeqsDev {
     const uint32_t* seen;    // [n] tokens ever: the newest one's position + 1
     const uint32_t* first;   // [n + 1] rows of new tokens before each sequence's
     const uint32_t* ifirst;  // [n + 1] superblocks before each sequence's (one at least each)
-    const uint32_t* items;   // [items][2] sequence, superblock of it (SLM_NO_SEQ: none)
+    const uint32_t* items;   // [items][4] sequence (SLM_NO_SEQ: none), superblock of it, its length, 0
     const uint32_t* table;   // [n][width] pages
     int32_t n, width;
 };
@@ -27,6 +27,7 @@ struct PStoreArgs {
     uint32_t* born;          // likewise
     const float *ksrc, *vsrc;  // [rows][kh][dh]
     int32_t rows, kh, page, dh;
+    int32_t each;            // one new token in every sequence: row b is sequence b's
 };
 
 struct PAttnArgs {
@@ -37,9 +38,10 @@ struct PAttnArgs {
     const float* mass;       // with mass_out
     float* mass_out;         // or null
     const uint32_t* born;    // positions, or null: slot t holds position t
-    float* ml;               // [items][heads][2] maximum (powers of two) and sum
+    float* ml;               // [heads][items][2] maximum (powers of two) and sum
     float* po;               // [items][heads][dh] weighted values
     float* sc;               // [items][heads][SLM_PG_KEYS] scores, with mass_out
+    int32_t items;
     int32_t heads, kh, page, dh;
     int64_t gap;
     float scale;             // times log2 e

@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "batch.h"
 
 #define KERNEL extern "C" __global__
@@ -22,7 +24,7 @@ static constexpr float NEG_INF = -__builtin_inff();
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
 }
 // Sums and maxima over a row of 16 lanes (in every lane): lane pairs, quads, then the mirrored
 // lane of eight and of sixteen.
@@ -69,12 +71,6 @@ __device__ __forceinline__ float r16(float v) {
     return (float)(_Float16)v;
 }
 
-__device__ __forceinline__ f4 load4(const float* p) { return *(const f4*)p; }
-__device__ __forceinline__ f4 load4(const _Float16* p) {
-    h4 v = *(const h4*)p;
-    return f4{(float)v.x, (float)v.y, (float)v.z, (float)v.w};
-}
-
 // Row of a sequence's token t under key head h, over [pages][kh][page].
 __device__ __forceinline__ uint32_t row_of(const SeqsDev& s, int b, uint32_t t, int h, int kh, int page) {
     uint32_t pg = t / (uint32_t)page;
@@ -94,13 +90,13 @@ __device__ __forceinline__ void store_body(const PStoreArgs& a) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         uint32_t row = (uint32_t)(i / per);
         int e = (int)(i - row * per), h = e / a.dh, d = e - h * a.dh;
-        int lo = 0, hi = a.s.n;  // first[lo] <= row < first[hi]
+        int lo = a.each ? (int)row : 0, hi = a.each ? lo + 1 : a.s.n;  // first[lo] <= row < first[hi]
         while (hi - lo > 1) {
             int mid = (lo + hi) >> 1;
             if (a.s.first[mid] <= row) lo = mid;
             else hi = mid;
         }
-        uint32_t behind = a.s.first[lo + 1] - row;  // 1: the newest
+        uint32_t behind = a.each ? 1 : a.s.first[lo + 1] - row;  // 1: the newest
         uint32_t to = row_of(a.s, lo, a.s.len[lo] - behind, h, a.kh, a.page);
         ((T*)a.k)[(int64_t)to * a.dh + d] = (T)a.ksrc[i];
         ((T*)a.v)[(int64_t)to * a.dh + d] = (T)a.vsrc[i];
@@ -117,246 +113,399 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 // attend: one new token a sequence
 // ---------------------------------------------------------------------------------------
 
-// y_g = sum_t softmax_t(scale · q_g·k_t) v_t for the query heads g of one key head, over one
-// superblock of SLM_PG_KEYS slots: the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
-// x = (scale · log2 e) q·k. slm_paged_join adds the superblocks up. A superblock none of whose
-// slots is visible has m = -inf, one with a visible slot at least -FLT_MAX.
+// y_g = sum_t softmax_t(scale · q_g·k_t) v_t for the query heads g of one key head. A workgroup
+// takes one superblock of SLM_PG_KEYS slots, its waves 64 / NT keys each (NT: the head size in
+// 64s); for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
+// x = (scale · log2 e) q·k over its keys, the workgroup those of the superblock, and
+// slm_paged_join adds the superblocks up. No visible key: m = -inf; one at least: m >= -FLT_MAX.
+//
+// What bounds it is the reading of keys and values, so a wave issues all of its own (32 KB of
+// fp32) at once, straight into registers, as soon as it has its rows' addresses: 16 lanes read
+// a row, each 4 of every 64 elements. A row's dot product is then in 16 lanes, and 16 rows'
+// are brought to one lane each by adding and halving (15 additions, not 64): the softmax
+// works on a key a lane. A key's weight goes back to the 16 lanes that hold its value by a lane
+// broadcast within the row.
 extern __shared__ char lds_[];
 
-template <typename T, int NT>
-__device__ __forceinline__ void attn_body(const PAttnArgs& a) {
-    constexpr int DP = 64 * NT;
-    const int h = blockIdx.x % a.kh, item = blockIdx.x / a.kh;
-    const uint32_t b = a.s.items[2 * item], sb = a.s.items[2 * item + 1];
-    if (b == SLM_NO_SEQ) return;
-    const int G = a.heads / a.kh, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, dh = a.dh;
-    const uint32_t len = a.s.len[b], base = sb * SLM_PG_KEYS;
-    // slots to look at: all where positions are given, else those before the gap
-    const uint32_t most = a.born ? len : (int64_t)len > a.gap ? (uint32_t)(len - a.gap) : 0;
-    if (base >= most && !(a.direct && sb == 0)) return;
+template <int J>
+__device__ __forceinline__ uint32_t bcast(uint32_t x) {  // lane J of each row of 16, to the row
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x150 + J, 0xF, 0xF, true);
+}
+template <int J>
+__device__ __forceinline__ float bcast(float x) { return __uint_as_float(bcast<J>(__float_as_uint(x))); }
 
-    float* sq = (float*)lds_;                // [G][DP]
-    float* ss = sq + G * DP;                 // [G][SLM_PG_KEYS]
-    float* so = ss + G * SLM_PG_KEYS;        // [4][G][DP]
-    float* sml = so + 4 * G * DP;            // [G][2]
-    uint32_t* srow = (uint32_t*)(sml + 2 * G);  // [SLM_PG_KEYS], the top bit: not visible
-    {
-        uint32_t t = base + tid, row = 0x80000000u;
-        if (len) {
-            row = row_of(a.s, b, min(t, len - 1), h, a.kh, a.page);
-            bool sees = t < most;
-            if (sees && a.born) sees = (uint64_t)a.born[row] + (uint64_t)a.gap < a.s.seen[b];
-            if (!sees) row |= 0x80000000u;
-        }
-        srow[tid] = row;
+// J = 0 .. N - 1 as constants.
+template <int N, int J = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+    if constexpr (J < N) {
+        f(std::integral_constant<int, J>());
+        each<N, J + 1>(f);
     }
-    for (int i = tid; i < G * DP; i += 256) {
+}
+
+// Sums over rows of 16 lanes of N values a lane: value c % N to lane c.
+template <int N>
+__device__ __forceinline__ float scatter_sum(float (&s)[N], int c) {
+    auto halve = [&](auto n, auto ctrl, int bit) {
+        constexpr int H = decltype(n)::value / 2;
+#pragma unroll
+        for (int j = 0; j < H; j++) {
+            float keep = c & bit ? s[j + H] : s[j], give = c & bit ? s[j] : s[j + H];
+            s[j] = keep + dpp<decltype(ctrl)::value>(give);
+        }
+    };
+    using std::integral_constant;
+    if constexpr (N == 16) halve(integral_constant<int, 16>(), integral_constant<int, 0x128>(), 8);
+    else
+#pragma unroll
+        for (int j = 0; j < N; j++) s[j] += dpp<0x128>(s[j]);
+    // (the partners: lane 7 - i of eight, 3 - i of four, then the neighbour)
+    if constexpr (N >= 8) halve(integral_constant<int, 8>(), integral_constant<int, 0x141>(), 4);
+    else
+#pragma unroll
+        for (int j = 0; j < N; j++) s[j] += dpp<0x141>(s[j]);
+    halve(integral_constant<int, 4>(), integral_constant<int, 0x1B>(), 2);
+    halve(integral_constant<int, 2>(), integral_constant<int, 0xB1>(), 1);
+    return s[0];
+}
+
+__device__ __forceinline__ void lds_barrier() {  // (loads from memory stay in flight)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Slots of a sequence that a call looks at: all where positions are given, else those before
+// the gap.
+__device__ __forceinline__ uint32_t looks(const PAttnArgs& a, uint32_t len) {
+    return a.born ? len : (int64_t)len > a.gap ? (uint32_t)(len - a.gap) : 0;
+}
+
+// M = max m_z and L = sum l_z 2^(m_z - M) over nz superblocks for one head, by a wave: lane z % 64
+// adds z in order, the lanes as one tree.
+__device__ __forceinline__ float2 join_ml(const float2* ml, int nz) {
+    const int lane = threadIdx.x & 63;
+    float m = NEG_INF;
+    for (int z = lane; z < nz; z += 64) m = fmaxf(m, ml[z].x);
+    m = wave_max(m);
+    float l = 0.0f, ms = m == NEG_INF ? 0.0f : m;
+    for (int z = lane; z < nz; z += 64) {
+        float2 p = ml[z];
+        l = fmaf(p.y, __builtin_amdgcn_exp2f(p.x - ms), l);
+    }
+    return make_float2(m, wave_sum(l));
+}
+
+// Sums over the four rows of 16 lanes of four values a lane: value r to row r. (A swap of half
+// waves, or of the odd rows, puts two values' partners side by side: one addition for both.)
+__device__ __forceinline__ float scatter_rows(f4 v) {
+    auto add = [](auto p) { return __uint_as_float(p[0]) + __uint_as_float(p[1]); };
+    float a = add(__builtin_amdgcn_permlane32_swap(__float_as_uint(v.x), __float_as_uint(v.z), false, false));
+    float b = add(__builtin_amdgcn_permlane32_swap(__float_as_uint(v.y), __float_as_uint(v.w), false, false));
+    return add(__builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+}
+
+// GM: the query heads a key head (1 to 4: exactly, all at once), or 16: any number, four at
+// a time, the weights by way of LDS.
+template <typename T, int NT, int GM>
+__device__ __forceinline__ void attn_body(const PAttnArgs& a) {
+    constexpr int KS = 16 / NT, NW = 4 * NT, DP = 64 * NT, THREADS = 64 * NW;
+    typedef std::conditional_t<sizeof(T) == 2, h4, f4> V4;
+    using std::integral_constant;
+    const int item = blockIdx.x / a.kh, h = blockIdx.x % a.kh;
+    const uint4 it = ((const uint4*)a.s.items)[item];
+    const uint32_t b = it.x, len = it.z, base = it.y * SLM_PG_KEYS;
+    if (b == SLM_NO_SEQ) return;
+    const uint32_t most = looks(a, len);
+    // (direct: a sequence that sees nothing still gets its zeros)
+    if (base >= most && !(it.y == 0 && a.direct)) return;
+    const int G = GM <= 4 ? GM : a.heads / a.kh, dh = a.dh;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane >> 4, c = lane & 15;
+    const int GC = GM <= 4 || NT < 4 ? G : min(G, 4);  // heads whose values are added up at once
+    float* sq = (float*)lds_;                         // [G][DP]
+    float* so = sq + G * DP;                          // [NW][GC][DP]
+    float* swm = so + NW * GC * DP;                   // [NW][G][2]
+    float* sml = swm + NW * G * 2;                    // [G][2]
+    float* sw = sml + G * 2;                          // [NW][G][4 * KS], for GM 16
+    float* ss = sw + (GM <= 4 ? 0 : G * SLM_PG_KEYS);  // [G][SLM_PG_KEYS], with direct and mass_out
+
+    // this lane's key: the one whose score it will have
+    const int mine = w * (4 * KS) + 4 * (c & (KS - 1)) + r;
+    const bool some = base + w * (4 * KS) < most;     // the wave has a key to look at
+    bool sees = base + mine < most;
+    uint64_t at = 0;                                  // ... and where its row starts, in values
+    if (some) {
+        uint32_t row = row_of(a.s, b, min(base + mine, len - 1), h, a.kh, a.page);
+        if (a.born && sees) sees = (uint64_t)a.born[row] + (uint64_t)a.gap < a.s.seen[b];
+        at = (uint64_t)row * (uint32_t)dh;
+    }
+    for (int i = tid; i < G * DP; i += THREADS) {
         int g = i / DP, d = i % DP;
         sq[i] = d < dh ? a.q[((int64_t)b * a.heads + h * G + g) * dh + d] : 0.0f;
     }
-    __syncthreads();
-    const bool any_key = len > 0;
-    {  // scores: sixteen lanes a key
-        const int r = lane >> 4, c = lane & 15;
-#pragma unroll 4
-        for (int j = 0; j < 16; j++) {
-            int key = w * 64 + 4 * j + r;
-            uint32_t row = srow[key];
-            f4 kv[NT];
+    // keys and values: the lane's four of every 64 elements of its row of 16's keys (past the head
+    // size: the last four again, made zeros in the keys and of no effect in the values)
+    V4 k[KS][NT], v[KS][NT];
+    auto load = [&](const void* from, V4 (&to)[KS][NT]) {
+        each<KS>([&](auto j) {
+            uint64_t o = (uint64_t)bcast<j>((uint32_t)(at >> 32)) << 32 | bcast<j>((uint32_t)at);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                int d = 64 * t + 4 * c;
-                kv[t] = any_key && d < dh ? load4((const T*)a.k + (int64_t)(row & 0x7fffffffu) * dh + d) : f4{0, 0, 0, 0};
-            }
-            for (int g = 0; g < G; g++) {
-                float s = 0.0f;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    f4 q = *(const f4*)(sq + g * DP + 64 * t + 4 * c);
-                    s = fmaf(q.x, kv[t].x, s);
-                    s = fmaf(q.y, kv[t].y, s);
-                    s = fmaf(q.z, kv[t].z, s);
-                    s = fmaf(q.w, kv[t].w, s);
-                }
-                s = row_sum(s) * a.scale;
-                if (c == 0) ss[g * SLM_PG_KEYS + key] = (int)row < 0 ? NEG_INF : s;
-            }
-        }
+            for (int i = 0; i < NT; i++) to[j][i] = *(const V4*)((const T*)from + o + min(64 * i + 4 * c, dh - 4));
+        });
+    };
+    if (some) {
+        load(a.k, k);
+        if (NT < 4) load(a.v, v);  // (sixteen waves have room for one of the two in registers)
     }
-    __syncthreads();
-    for (int g = w; g < G; g += 4) {  // softmax: a wave a head
-        float x[4], m = NEG_INF;
-        bool sees = false;
+    const bool all = __ballot(sees) == ~0ull, any = __ballot(sees) != 0;
+    lds_barrier();
+    if (dh < DP && some)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[i] = ss[g * SLM_PG_KEYS + lane + 64 * i];
-            sees |= (int)srow[lane + 64 * i] >= 0;
-            m = fmaxf(m, x[i]);
-        }
-        m = wave_max(m);
-        if (__ballot(sees)) m = fmaxf(m, -FLT_MAX);
-        float l = 0.0f;
+        for (int i = 0; i < NT; i++)
+            if (64 * i + 4 * c >= dh)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (a.sc) a.sc[((int64_t)item * a.heads + h * G + g) * SLM_PG_KEYS + lane + 64 * i] = x[i];
-            float p = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m);
-            ss[g * SLM_PG_KEYS + lane + 64 * i] = p;
-            l += p;
-        }
-        l = wave_sum(l);
-        if (lane == 0) {
-            sml[2 * g] = m;
-            sml[2 * g + 1] = l;
-        }
-    }
-    __syncthreads();
-    {  // values: 16·NT threads a key
-        constexpr int C = 16 * NT, KG = 256 / C;
-        const int c = tid % C, kg = tid / C, d = 4 * c;
-        for (int g0 = 0; g0 < G; g0 += 4) {
-            f4 acc[4] = {};
-#pragma unroll 8
-            for (int key = kg; key < SLM_PG_KEYS; key += KG) {
-                uint32_t row = srow[key];
-                f4 v = f4{0, 0, 0, 0};
-                if ((int)row >= 0 && d < dh) v = load4((const T*)a.v + (int64_t)row * dh + d);
+                for (int j = 0; j < KS; j++) k[j][i] = V4{};
+
+    float p[GM <= 4 ? GM : 1];
+    float* sp = sw + w * G * (4 * KS) + r * KS + (c & (KS - 1));
+    auto scores = [&](auto gx, int g0, float* out) {  // gx heads from g0: their weights
+        constexpr int GX = decltype(gx)::value;
+        float x[GX], m[GX], l[GX];
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    if (g0 + g >= G) break;
-                    float p = ss[(g0 + g) * SLM_PG_KEYS + key];
-                    acc[g].x = fmaf(p, v.x, acc[g].x);
-                    acc[g].y = fmaf(p, v.y, acc[g].y);
-                    acc[g].z = fmaf(p, v.z, acc[g].z);
-                    acc[g].w = fmaf(p, v.w, acc[g].w);
+        for (int g = 0; g < GX; g++) {
+            x[g] = NEG_INF;
+            if (!some) continue;
+            float s[KS];
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                f4 q = *(const f4*)(sq + (g0 + g) * DP + 64 * i + 4 * c);
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    s[j] = i ? fmaf(q.x, (float)k[j][i].x, s[j]) : q.x * (float)k[j][i].x;
+                    s[j] = fmaf(q.y, (float)k[j][i].y, s[j]);
+                    s[j] = fmaf(q.z, (float)k[j][i].z, s[j]);
+                    s[j] = fmaf(q.w, (float)k[j][i].w, s[j]);
                 }
             }
+            x[g] = scatter_sum<KS>(s, c) * a.scale;
+            if (!sees) x[g] = NEG_INF;
+        }
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                if (g0 + g >= G) break;
+        for (int g = 0; g < GX; g++) {
+            m[g] = wave_max(x[g]);
+            if (any) m[g] = fmaxf(m[g], -FLT_MAX);
+            out[g] = m[g] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[g] - m[g]);
+        }
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float o = acc[g][e];
-                    if (NT == 1) o = sum16(o);
-                    if (NT <= 2) o = sum32(o);
-                    if (lane < C) so[(w * G + g0 + g) * DP + (tid % C) * 4 + e] = o;
-                }
+        for (int g = 0; g < GX; g++) l[g] = wave_sum(c < KS ? out[g] : 0.0f);
+#pragma unroll
+        for (int g = 0; g < GX; g++) {
+            if (lane == 0) *(float2*)(swm + (w * G + g0 + g) * 2) = make_float2(m[g], l[g]);
+            if (a.mass_out && c < KS) {
+                if (a.direct) ss[(g0 + g) * SLM_PG_KEYS + mine] = x[g];
+                else a.sc[((int64_t)item * a.heads + h * G + g0 + g) * SLM_PG_KEYS + mine] = x[g];
             }
         }
-    }
-    __syncthreads();
-    for (int i = tid; i < G * dh; i += 256) {
-        int g = i / dh, d = i - g * dh, H = h * G + g;
-        float o = 0.0f;
-        if (NT <= 2) {
+    };
+    auto values = [&](auto gx, int slot, const float* pg) {  // gx heads: their values to LDS
+        constexpr int GX = decltype(gx)::value;
+        f4 o[GX][NT];
 #pragma unroll
-            for (int k = 0; k < 4; k++) o += so[(k * G + g) * DP + d];
+        for (int g = 0; g < GX; g++)
+#pragma unroll
+            for (int i = 0; i < NT; i++) o[g][i] = f4{0, 0, 0, 0};
+        if (some)
+            each<KS>([&](auto j) {
+#pragma unroll
+                for (int g = 0; g < GX; g++) {
+                    float w1 = bcast<j>(pg[g]);
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[g][i][e] = j ? fmaf(w1, (float)v[j][i][e], o[g][i][e]) : w1 * (float)v[j][i][e];
+                }
+            });
+#pragma unroll
+        for (int g = 0; g < GX; g++)
+#pragma unroll
+            for (int i = 0; i < NT; i++) so[(w * GC + slot + g) * DP + 64 * i + 4 * c + r] = scatter_rows(o[g][i]);
+    };
+    constexpr int GS = NT == 4 ? 1 : 4;  // (sixteen waves: a head at a time, for the registers)
+    auto some_heads = [&](int n, auto f) {  // f(heads) for n of them, up to GS
+        if constexpr (GS == 4) {
+            if (n >= 4) return f(integral_constant<int, 4>());
+            if (n == 3) return f(integral_constant<int, 3>());
+            if (n == 2) return f(integral_constant<int, 2>());
+        }
+        f(integral_constant<int, 1>());
+    };
+    if constexpr (GM <= 4) {
+        scores(integral_constant<int, GM>(), 0, p);
+    } else {
+        for (int g0 = 0; g0 < G; g0 += GS)
+            some_heads(G - g0, [&](auto gx) {
+                float e[decltype(gx)::value];
+                scores(gx, g0, e);
+#pragma unroll
+                for (int g = 0; g < decltype(gx)::value; g++) sp[(g0 + g) * (4 * KS)] = e[g];
+            });
+    }
+    if (NT == 4 && some) load(a.v, v);
+    if (some && !all) {  // what is not seen may hold anything
+        uint32_t seen = sees;
+        each<KS>([&](auto j) {
+            if (!bcast<j>(seen)) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) v[j][i] = V4{};
+            }
+        });
+    }
+    for (int c0 = 0; c0 < G; c0 += GC) {
+        const int ng = min(G - c0, GC);
+        if constexpr (GM <= 4) {
+            values(integral_constant<int, GM>(), 0, p);
         } else {
+            for (int g0 = 0; g0 < ng; g0 += GS)
+                some_heads(ng - g0, [&](auto gx) {
+                    float e[decltype(gx)::value];
 #pragma unroll
-            for (int k = 0; k < 4; k++) o += so[(k * G + g) * DP + d];
+                    for (int g = 0; g < decltype(gx)::value; g++) e[g] = sp[(c0 + g0 + g) * (4 * KS)];
+                    values(gx, g0, e);
+                });
         }
-        float m = sml[2 * g], l = sml[2 * g + 1];
-        if (a.direct) {
-            float y = m == NEG_INF ? 0.0f : o / l;
-            a.y[((int64_t)b * a.heads + H) * dh + d] = a.r16 ? r16(y) : y;
-        } else {
-            a.po[((int64_t)item * a.heads + H) * dh + d] = o;
-            if (d == 0) {
-                a.ml[2 * ((int64_t)item * a.heads + H)] = m;
-                a.ml[2 * ((int64_t)item * a.heads + H) + 1] = l;
+        lds_barrier();
+        // the superblock's, from its waves' in order
+        for (int i = tid; i < ng * DP; i += THREADS) {
+            int g = i / DP, d = i % DP, gg = c0 + g;
+            if (d >= dh) continue;
+            float m = NEG_INF, l = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int k2 = 0; k2 < NW; k2++) m = fmaxf(m, swm[(k2 * G + gg) * 2]);
+            float ms = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+            for (int k2 = 0; k2 < NW; k2++) {
+                float2 ml = *(const float2*)(swm + (k2 * G + gg) * 2);
+                float f = __builtin_amdgcn_exp2f(ml.x - ms);
+                l = fmaf(ml.y, f, l);
+                o = fmaf(so[(k2 * GC + g) * DP + d], f, o);
+            }
+            if (a.direct) {
+                float y = m == NEG_INF ? 0.0f : o / l;
+                a.y[((int64_t)b * a.heads + h * G + gg) * dh + d] = a.r16 ? r16(y) : y;
+                if (d == 0) *(float2*)(sml + 2 * gg) = make_float2(m, l);
+            } else {
+                const int head = h * G + gg;
+                a.po[((int64_t)item * a.heads + head) * dh + d] = o;
+                if (d == 0) *(float2*)(a.ml + 2 * ((int64_t)head * a.items + item)) = make_float2(m, l);
             }
         }
+        if (c0 + GC < G) lds_barrier();  // (the next heads' sums go where these lie)
     }
-    if (a.direct && a.mass_out && base + tid < len) {
-        uint32_t row = srow[tid] & 0x7fffffffu;
-        float add = 0.0f;
-        for (int g = 0; g < G; g++)
-            if (sml[2 * g] != NEG_INF) add += ss[g * SLM_PG_KEYS + tid] / sml[2 * g + 1];
-        a.mass_out[row] = a.mass[row] + add;
-    }
+    if (!a.direct || !a.mass_out) return;
+    lds_barrier();
+    if (NT > 1 && tid >= SLM_PG_KEYS) return;
+    const uint32_t t = base + tid;
+    if (t >= len) return;
+    float add = 0.0f;
+    for (int g = 0; g < G; g++)
+        if (sml[2 * g] != NEG_INF) add += __builtin_amdgcn_exp2f(ss[g * SLM_PG_KEYS + tid] - sml[2 * g]) / sml[2 * g + 1];
+    uint32_t slot = row_of(a.s, b, t, h, a.kh, a.page);
+    a.mass_out[slot] = a.mass[slot] + add;
 }
 
-#define PAGED_ATTN(name, T, NT) \
-    KERNEL void __launch_bounds__(256) name(PAttnArgs a) { attn_body<T, NT>(a); }
-PAGED_ATTN(slm_paged_attn_1, float, 1)
-PAGED_ATTN(slm_paged_attn_2, float, 2)
-PAGED_ATTN(slm_paged_attn_4, float, 4)
-PAGED_ATTN(slm_paged_attn16_1, _Float16, 1)
-PAGED_ATTN(slm_paged_attn16_2, _Float16, 2)
-PAGED_ATTN(slm_paged_attn16_4, _Float16, 4)
+#define PAGED_ATTN(name, T, NT, GM) \
+    KERNEL void __launch_bounds__(256 * NT) name(PAttnArgs a) { attn_body<T, NT, GM>(a); }
+#define PAGED_ATTNS(name, T, NT)       \
+    PAGED_ATTN(name##_1, T, NT, 1)     \
+    PAGED_ATTN(name##_2, T, NT, 2)     \
+    PAGED_ATTN(name##_3, T, NT, 3)     \
+    PAGED_ATTN(name##_4, T, NT, 4)     \
+    PAGED_ATTN(name##_16, T, NT, 16)
+PAGED_ATTNS(slm_paged_attn_1, float, 1)
+PAGED_ATTNS(slm_paged_attn_2, float, 2)
+PAGED_ATTN(slm_paged_attn_4_16, float, 4, 16)
+PAGED_ATTNS(slm_paged_attn16_1, _Float16, 1)
+PAGED_ATTNS(slm_paged_attn16_2, _Float16, 2)
+PAGED_ATTN(slm_paged_attn16_4_16, _Float16, 4, 16)
 
-// The superblocks of a sequence that a call looks at.
-__device__ __forceinline__ int superblocks(const PAttnArgs& a, int b) {
-    uint32_t len = a.s.len[b];
-    uint32_t most = a.born ? len : (int64_t)len > a.gap ? (uint32_t)(len - a.gap) : 0;
-    return (int)((most + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
-}
-
-// M = max m_z and L = sum l_z 2^(m_z - M) over a sequence's nz superblocks for one head, by a
-// workgroup of 256 (every thread gets both): threads stride over z, then one fixed tree.
-__device__ __forceinline__ float2 join_ml(const float* ml, int heads, int nz, float* red) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    float m = NEG_INF;
-    for (int z = tid; z < nz; z += 256) m = fmaxf(m, ml[2 * (int64_t)z * heads]);
-    m = wave_max(m);
-    __syncthreads();
-    if (lane == 0) red[w] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float l = 0.0f, ms = m == NEG_INF ? 0.0f : m;
-    for (int z = tid; z < nz; z += 256)
-        l = fmaf(ml[2 * (int64_t)z * heads + 1], __builtin_amdgcn_exp2f(ml[2 * (int64_t)z * heads] - ms), l);
-    l = wave_sum(l);
-    if (lane == 0) red[4 + w] = l;
-    __syncthreads();
-    return make_float2(m, (red[4] + red[5]) + (red[6] + red[7]));
-}
-
-// y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), the superblocks dealt to
-// 256 / (dh / 4) groups of threads, whose sums add in order. Behind them, with mass_out, a
-// workgroup a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g.
-KERNEL void __launch_bounds__(256) slm_paged_join(PAttnArgs a) {
-    __shared__ float red[8];
-    __shared__ float so[256 * 4];
-    const int tid = threadIdx.x, H = a.heads;
+// y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), superblock z in group z % KG of
+// dh / 4 threads, a group in order, then the groups in order. Behind them, with mass_out, four
+// waves a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g.
+KERNEL void __launch_bounds__(1024) slm_paged_join(PAttnArgs a) {
+    __shared__ f4 so[1024];
+    __shared__ float2 sml[4][16];
+    const int tid = threadIdx.x, H = a.heads, dh = a.dh;
     if ((int)blockIdx.x < a.s.n * H) {
-        const int b = blockIdx.x / H, g = blockIdx.x % H, nz = superblocks(a, b);
+        const int b = blockIdx.x / H, head = blockIdx.x % H;
+        const int nz = (int)((looks(a, a.s.len[b]) + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
         const int64_t z0 = a.s.ifirst[b];
-        float2 ML = join_ml(a.ml + 2 * (z0 * H + g), H, nz, red);
-        const int C = a.dh / 4, KG = 256 / C, c = tid % C, zg = tid / C;
-        float ms = ML.x == NEG_INF ? 0.0f : ML.x;
+        const float2* ml = (const float2*)a.ml + (int64_t)head * a.items + z0;
+        const float2 ML = join_ml(ml, nz);
+        const int cols = dh / 4, KG = 1024 / cols, c = tid % cols, zg = tid / cols;
+        const float ms = ML.x == NEG_INF ? 0.0f : ML.x;
         f4 o = {0, 0, 0, 0};
-        if (zg < KG)
+        if (zg < KG) {
+            const float* po = a.po + (z0 * H + head) * dh + 4 * c;
+#pragma unroll 4
             for (int z = zg; z < nz; z += KG) {
-                float wz = __builtin_amdgcn_exp2f(a.ml[2 * ((z0 + z) * H + g)] - ms);
-                f4 v = *(const f4*)(a.po + ((z0 + z) * H + g) * a.dh + 4 * c);
+                float wz = __builtin_amdgcn_exp2f(ml[z].x - ms);
+                f4 v = *(const f4*)(po + (int64_t)z * H * dh);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[e] = fmaf(v[e], wz, o[e]);
             }
-        *(f4*)(so + 4 * tid) = o;
+        }
+        so[tid] = o;
         __syncthreads();
-        if (tid < a.dh) {
+        if (tid < dh) {
             float s = 0.0f;
-            for (int k = 0; k < KG; k++) s += so[4 * C * k + tid];
+            const int ng = min(nz, KG);
+#pragma unroll 8
+            for (int k = 0; k < ng; k++) s += ((const float*)so)[k * dh + tid];
             float y = ML.x == NEG_INF ? 0.0f : s / ML.y;
-            a.y[((int64_t)b * H + g) * a.dh + tid] = a.r16 ? r16(y) : y;
+            a.y[((int64_t)b * H + head) * dh + tid] = a.r16 ? r16(y) : y;
         }
         return;
     }
-    const int k = blockIdx.x - a.s.n * H, item = k / a.kh, h = k % a.kh, G = H / a.kh;
-    const uint32_t b = a.s.items[2 * item], sb = a.s.items[2 * item + 1];
-    if (b == SLM_NO_SEQ) return;
-    const uint32_t t = sb * SLM_PG_KEYS + tid, len = a.s.len[b];
-    const int nz = superblocks(a, b);
+    const int pair = ((int)blockIdx.x - a.s.n * H) * 4 + (tid >> 8), item = pair / a.kh, h = pair % a.kh, G = H / a.kh;
+    const int part = tid >> 8, w = (tid >> 6) & 3, key = tid & 255;
+    uint4 it = {SLM_NO_SEQ, 0, 0, 0};
+    if (item < a.items) it = ((const uint4*)a.s.items)[item];
+    const uint32_t b = it.x, len = it.z, t = it.y * SLM_PG_KEYS + key;
+    const bool live = b != SLM_NO_SEQ;
+    const int nz = live ? (int)((looks(a, len) + SLM_PG_KEYS - 1) / SLM_PG_KEYS) : 0;
+    const bool seen = (int)it.y < nz;
+    float x[4];
+    uint32_t slot = 0;
+    float old = 0.0f;
+    if (live && t < len) {
+        slot = row_of(a.s, b, t, h, a.kh, a.page);
+        old = a.mass[slot];
+    }
+    const float* sc = a.sc + ((int64_t)item * H + h * G) * SLM_PG_KEYS + key;
+#pragma unroll
+    for (int g = 0; g < 4; g++) x[g] = seen && g < G ? sc[g * SLM_PG_KEYS] : 0.0f;
+    if (seen) {
+        const int64_t z0 = a.s.ifirst[b];
+        for (int g = w; g < G; g += 4) {
+            float2 ML = join_ml((const float2*)a.ml + (int64_t)(h * G + g) * a.items + z0, nz);
+            if ((tid & 63) == 0) sml[part][g] = ML;
+        }
+    }
+    __syncthreads();
     float add = 0.0f;
-    for (int g = 0; g < G && (int)sb < nz; g++) {
-        float2 ML = join_ml(a.ml + 2 * ((int64_t)a.s.ifirst[b] * H + h * G + g), H, nz, red);
-        if (ML.x != NEG_INF)
-            add += __builtin_amdgcn_exp2f(a.sc[((int64_t)item * H + h * G + g) * SLM_PG_KEYS + tid] - ML.x) / ML.y;
+    auto take = [&](int g, float xg) {
+        float2 ML = sml[part][g];
+        if (ML.x != NEG_INF) add += __builtin_amdgcn_exp2f(xg - ML.x) / ML.y;
+    };
+    if (seen) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            if (g < G) take(g, x[g]);
+        for (int g = 4; g < G; g++) take(g, sc[g * SLM_PG_KEYS]);
     }
-    if (t < len) {
-        uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
-        a.mass_out[row] = a.mass[row] + add;
-    }
+    if (live && t < len) a.mass_out[slot] = old + add;
 }
 
 // ---------------------------------------------------------------------------------------

