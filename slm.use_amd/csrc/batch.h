@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #define SLM_PG_KEYS 256     // keys of a superblock: one workgroup's, whatever the batch
+#define SLM_MOVES_HERE 256  // moves of a sequence and key head that need no launch of their own
 #define SLM_TOP_MAX 32      // alternatives of a row of logits
 #define SLM_NO_SEQ 0xffffffffu
 
@@ -57,11 +58,13 @@ struct PEvictArgs {
     float* mass_out;
     uint32_t* born_out;
     uint32_t* moves;         // [n·kh][2][most] slots left, slots that move there
-    uint32_t* count;         // [n·kh] moves
+    uint32_t* count;         // [n·kh] moves; null: at most SLM_MOVES_HERE, made by the launch that finds them
     int32_t kh, page, dh;
     uint32_t keep, recent, most;
     int32_t in_place;        // mass_out is mass and born_out is born
     int32_t unit;            // bytes of a value
+    uint32_t room;           // slots whose keys LDS has room for, a multiple of 64
+    int32_t vec;             // mass and born can be read four slots at a time
 };
 
 struct PMoveArgs {

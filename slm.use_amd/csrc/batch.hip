@@ -535,39 +535,80 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v, uint32_t* s, uint32_
     return before;
 }
 
-// A workgroup of 1024 a (sequence, key head): the keep-th largest key by three rounds of
-// counting its digits (11, 11 and 10 bits), ties by slot; then, over the slots in order, which
-// of the first `keep` are left and which of those behind move there.
+// Row `from` to row `to`, V at a time: lane c of sixteen.
+template <typename V>
+__device__ __forceinline__ void move_row(const PEvictArgs& a, uint32_t to, uint32_t from, int c) {
+    const int vecs = a.dh * a.unit / (int)sizeof(V);
+    for (int i = c; i < vecs; i += 16) {
+        V kv = ((const V*)a.k)[(int64_t)from * vecs + i], vv = ((const V*)a.v)[(int64_t)from * vecs + i];
+        ((V*)a.k)[(int64_t)to * vecs + i] = kv;
+        ((V*)a.v)[(int64_t)to * vecs + i] = vv;
+    }
+    if (c == 0) {
+        a.mass_out[to] = a.mass[from];
+        a.born_out[to] = a.born[from];
+    }
+}
+
+// A workgroup of 1024 a (sequence, key head). The slots' keys are read once, into LDS (up to
+// `room` of them; those of longer sequences are read again each time). The keep-th largest is
+// found by three rounds of counting digits (11, 11 and 10 bits); then, over the slots in order, a
+// wave a run of them: which of the first `keep` are left, and which of those behind move there.
+// Few moves (SLM_MOVES_HERE) are made here, more by a launch of their own.
 KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     __shared__ uint32_t hist[2048];
     __shared__ uint32_t red[16];
-    __shared__ uint32_t pick[2];
-    const int h = blockIdx.x % a.kh, b = blockIdx.x / a.kh, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ uint32_t pick[3];
+    uint32_t* keys = (uint32_t*)lds_;                         // [room]
+    uint64_t* stays = (uint64_t*)(keys + a.room);             // [room / 64]: the slots that stay, a bit each
+    const int h = blockIdx.x % a.kh, b = blockIdx.x / a.kh, tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t len = a.s.len[b], seen = a.s.seen[b];
-    if (len <= a.keep) {  // nothing goes
-        if (tid == 0) a.count[blockIdx.x] = 0;
-        if (!a.in_place)
-            for (uint32_t t = tid; t < len; t += 1024) {
-                uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
-                a.mass_out[row] = a.mass[row];
-                a.born_out[row] = a.born[row];
-            }
-        return;
-    }
-    auto key_of = [&](uint32_t t) {
-        uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
-        return mass_key(a.mass[row], a.born[row], a.recent, seen);
-    };
-    uint32_t prefix = 0, need = a.keep;  // keys that share the digits so far: `need` of them stay
-    for (int round = 0; round < 3; round++) {
-        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+    const bool over = len > a.keep, held = len <= a.room;
+    if (!over && tid == 0 && a.count) a.count[blockIdx.x] = 0;
+    if (!over && a.in_place) return;
+
+    auto key_at = [&](uint32_t row) { return mass_key(a.mass[row], a.born[row], a.recent, seen); };
+    auto key_of = [&](uint32_t t) { return held ? keys[t] : key_at(row_of(a.s, b, t, h, a.kh, a.page)); };
+    auto digit = [&](uint32_t k) { atomicAdd(&hist[k >> 21], 1u); };
+    if (over) {
         for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
         __syncthreads();
-        for (uint32_t t = tid; t < len; t += 1024) {
-            uint32_t k = key_of(t);
-            if (round == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        if (held && a.vec) {  // four slots of a page at once
+            for (uint32_t t = 4 * tid; t < len; t += 4096) {
+                uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+                f4 m = *(const f4*)(a.mass + row);
+                uint4 p = *(const uint4*)(a.born + row);
+                uint4 k = {mass_key(m.x, p.x, a.recent, seen), mass_key(m.y, p.y, a.recent, seen),
+                           mass_key(m.z, p.z, a.recent, seen), mass_key(m.w, p.w, a.recent, seen)};
+                *(uint4*)(keys + t) = k;
+                digit(k.x);
+                if (t + 1 < len) digit(k.y);
+                if (t + 2 < len) digit(k.z);
+                if (t + 3 < len) digit(k.w);
+            }
+        } else {
+            for (uint32_t t = tid; t < len; t += 1024) {
+                uint32_t k = key_at(row_of(a.s, b, t, h, a.kh, a.page));
+                if (held) keys[t] = k;
+                digit(k);
+            }
         }
         __syncthreads();
+    }
+    uint32_t prefix = 0, need = a.keep;  // keys that share the digits so far: `need` of them stay
+    bool ties = false;                   // ... and some of the last such keys go
+    for (int round = 0; round < 3 && over; round++) {
+        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+        if (round) {
+            for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
+            __syncthreads();
+            for (uint32_t t = tid; t < len; t += 1024) {
+                uint32_t k = key_of(t);
+                if ((k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+            }
+            __syncthreads();
+        }
         // the digit at which the count from above reaches `need`: each thread two bins, from above
         uint32_t h1 = hist[2047 - 2 * tid], h0 = hist[2046 - 2 * tid], mine = h1 + h0;
         uint32_t incl = mine;
@@ -580,48 +621,92 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
             bool first = before + h1 >= need;
             pick[0] = 2047 - 2 * tid - (first ? 0 : 1);
             pick[1] = need - before - (first ? 0 : h1);
+            pick[2] = (first ? h1 : h0) > pick[1];
         }
         __syncthreads();
         prefix = (prefix << bits) | pick[0];
         need = pick[1];
+        ties = pick[2] != 0;
         __syncthreads();
     }
-    // keys above `prefix` stay, and the first `need` of those equal to it. A wave takes a run of
-    // whole 64s of slots.
-    const uint32_t run = (len + 1024 - 1) / 1024 * 64, lo = min(len, w * run), hi = min(len, lo + run);
-    uint32_t ties = 0;
-    for (uint32_t t0 = lo; t0 < hi; t0 += 64)
-        ties += __popcll(__ballot(t0 + lane < hi && key_of(t0 + lane) == prefix));
-    uint32_t total, tie0 = wave_prefix(ties, red, &total);
-    auto kept_of = [&](uint32_t t0, uint32_t& tie) {
-        uint32_t k = t0 + lane < hi ? key_of(t0 + lane) : 0;
-        bool in = t0 + lane < hi, eq = in && k == prefix;
-        uint64_t em = __ballot(eq);
-        bool kept = in && (k > prefix || (eq && tie + lanes_below(em) < need));
-        tie += __popcll(em);
-        return kept;
-    };
-    uint32_t holes = 0, movers = 0, tie = tie0;
-    for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
-        bool kept = kept_of(t0, tie), in = t0 + lane < hi;
-        holes += __popcll(__ballot(in && !kept && t0 + lane < a.keep));
-        movers += __popcll(__ballot(kept && t0 + lane >= a.keep));
+    if (over) {
+        // keys above `prefix` stay, and the first `need` of those equal to it. A wave takes a
+        // run of whole 64s of slots.
+        const uint32_t run = (len + 1024 - 1) / 1024 * 64, lo = min(len, w * run), hi = min(len, lo + run);
+        uint32_t total, tie0 = 0;
+        if (ties) {
+            uint32_t n = 0;
+            for (uint32_t t0 = lo; t0 < hi; t0 += 64) n += __popcll(__ballot(t0 + lane < hi && key_of(t0 + lane) == prefix));
+            tie0 = wave_prefix(n, red, &total);
+        }
+        auto stays_of = [&](uint32_t t0, uint32_t& tie) -> uint64_t {
+            const bool in = t0 + lane < hi;
+            uint32_t k = in ? key_of(t0 + lane) : 0;
+            if (!ties) return __ballot(in && k >= prefix);
+            uint64_t em = __ballot(in && k == prefix);
+            uint64_t mask = __ballot(in && (k > prefix || (k == prefix && tie + lanes_below(em) < need)));
+            tie += __popcll(em);
+            return mask;
+        };
+        auto below = [](uint32_t t0, uint32_t end) -> uint64_t {  // bits of the slots before `end`
+            return end <= t0 ? 0 : end - t0 >= 64 ? ~0ull : (1ull << (end - t0)) - 1;
+        };
+        uint32_t holes = 0, movers = 0, tie = tie0;
+        for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
+            uint64_t m = stays_of(t0, tie), front = below(t0, a.keep);
+            if (held && lane == 0) stays[t0 / 64] = m;
+            holes += __popcll(~m & front & below(t0, len));
+            movers += __popcll(m & ~front);
+        }
+        uint32_t nm, hole0 = wave_prefix(holes, red, &nm), mover0 = wave_prefix(movers, red, &nm);
+        uint32_t* to = a.count ? a.moves + (int64_t)blockIdx.x * 2 * a.most : hist;  // (few: in LDS)
+        uint32_t* from = to + a.most;
+        if (tid == 0 && a.count) a.count[blockIdx.x] = nm;
+        tie = tie0;
+        for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
+            uint64_t m = held ? stays[t0 / 64] : stays_of(t0, tie), front = below(t0, a.keep);
+            uint64_t hm = ~m & front & below(t0, len), mm = m & ~front;
+            if (hm >> lane & 1) to[hole0 + lanes_below(hm)] = t0 + lane;
+            if (mm >> lane & 1) from[mover0 + lanes_below(mm)] = t0 + lane;
+            hole0 += __popcll(hm);
+            mover0 += __popcll(mm);
+            if (!held && !a.in_place && (m & front) >> lane & 1) {
+                uint32_t row = row_of(a.s, b, t0 + lane, h, a.kh, a.page);
+                a.mass_out[row] = a.mass[row];
+                a.born_out[row] = a.born[row];
+            }
+        }
+        __syncthreads();
+        if (!a.count)
+            for (uint32_t i = tid / 16; i < nm; i += 64) {
+                uint32_t d = row_of(a.s, b, to[i], h, a.kh, a.page), f = row_of(a.s, b, from[i], h, a.kh, a.page);
+                if (a.dh * a.unit % 16 == 0) move_row<f4>(a, d, f, tid % 16);
+                else move_row<h4>(a, d, f, tid % 16);
+            }
+        if (a.in_place || !held) return;
     }
-    uint32_t nh, nm, hole0 = wave_prefix(holes, red, &nh), mover0 = wave_prefix(movers, red, &nm);
-    uint32_t* to = a.moves + (int64_t)blockIdx.x * 2 * a.most;
-    uint32_t* from = to + a.most;
-    if (tid == 0) a.count[blockIdx.x] = nm;
-    tie = tie0;
-    for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
-        uint32_t t = t0 + lane;
-        bool kept = kept_of(t0, tie), in = t < hi;
-        bool hole = in && !kept && t < a.keep, mover = kept && t >= a.keep;
-        uint64_t hm = __ballot(hole), mm = __ballot(mover);
-        if (hole) to[hole0 + lanes_below(hm)] = t;
-        if (mover) from[mover0 + lanes_below(mm)] = t;
-        hole0 += __popcll(hm);
-        mover0 += __popcll(mm);
-        if (kept && !mover && !a.in_place) {
+    // mass and born of what stays where it is, into the buffers for them
+    const uint32_t end = min(len, a.keep);
+    if (a.vec) {
+        for (uint32_t t = 4 * tid; t < end; t += 4096) {
+            uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+            uint32_t m = over ? (uint32_t)(stays[t / 64] >> (t % 64)) & 15 : 15;
+            if (end - t < 4) m &= (1u << (end - t)) - 1;
+            f4 mass = *(const f4*)(a.mass + row);
+            uint4 born = *(const uint4*)(a.born + row);
+            if (m == 15) {
+                *(f4*)(a.mass_out + row) = mass;
+                *(uint4*)(a.born_out + row) = born;
+                continue;
+            }
+            if (m & 1) a.mass_out[row] = mass.x, a.born_out[row] = born.x;
+            if (m & 2) a.mass_out[row + 1] = mass.y, a.born_out[row + 1] = born.y;
+            if (m & 4) a.mass_out[row + 2] = mass.z, a.born_out[row + 2] = born.z;
+            if (m & 8) a.mass_out[row + 3] = mass.w, a.born_out[row + 3] = born.w;
+        }
+    } else {
+        for (uint32_t t = tid; t < end; t += 1024) {
+            if (over && !(stays[t / 64] >> (t % 64) & 1)) continue;
             uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
             a.mass_out[row] = a.mass[row];
             a.born_out[row] = a.born[row];
@@ -638,19 +723,8 @@ __device__ __forceinline__ void move_body(const PEvictArgs& a, uint32_t blocks) 
     const int h = pair % a.kh, b = pair / a.kh, tid = threadIdx.x;
     const uint32_t* to = a.moves + (int64_t)pair * 2 * a.most;
     const uint32_t* from = to + a.most;
-    const int vecs = a.dh * a.unit / (int)sizeof(V);  // a row
-    for (uint32_t r = r0 + tid / 16; r < min(n, r0 + 64); r += 16) {
-        uint32_t d = row_of(a.s, b, to[r], h, a.kh, a.page), s = row_of(a.s, b, from[r], h, a.kh, a.page);
-        for (int c = tid % 16; c < vecs; c += 16) {
-            V kv = ((const V*)a.k)[(int64_t)s * vecs + c], vv = ((const V*)a.v)[(int64_t)s * vecs + c];
-            ((V*)a.k)[(int64_t)d * vecs + c] = kv;
-            ((V*)a.v)[(int64_t)d * vecs + c] = vv;
-        }
-        if (tid % 16 == 0) {
-            a.mass_out[d] = a.mass[s];
-            a.born_out[d] = a.born[s];
-        }
-    }
+    for (uint32_t r = r0 + tid / 16; r < min(n, r0 + 64); r += 16)
+        move_row<V>(a, row_of(a.s, b, to[r], h, a.kh, a.page), row_of(a.s, b, from[r], h, a.kh, a.page), tid % 16);
 }
 KERNEL void __launch_bounds__(256) slm_paged_move16(PMoveArgs a) { move_body<f4>(a.e, a.blocks); }
 KERNEL void __launch_bounds__(256) slm_paged_move8(PMoveArgs a) { move_body<h4>(a.e, a.blocks); }

@@ -60,6 +60,7 @@ constexpr int ATTN_LDS_MAX = LDS_MAX;
 constexpr int ATTN_DEC_LDS = SLM_SB_SEGS * (2 * 64 * 64 + 1024) * 4;  // one-token attention: 256 keys and values, queries
 constexpr int GEMM_STAGES_HOST = 2;          // slices in flight in slm_gemm2 (GEMM_STAGES)
 constexpr int64_t CU_COUNT = 256;           // MI355X compute units
+constexpr int64_t EVICT_ROOM = 36352;       // slots whose keys (and a bit each) an eviction's workgroup holds in LDS
 
 enum OpKind : uint32_t {
     OP_GATHER = 1, OP_COPY, OP_SHIFT, OP_COLUMNS, OP_LINEAR, OP_ADD, OP_ADD_ROW, OP_SCALE_ROWS,
@@ -966,7 +967,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         return SLM_OK;
     }
     // p0 k, p1 v, p2 mass out, p3 born out, p4 mass, p5 born; n0 n, n1 keep, n2 kh, n3 page, n4 dh, n5 pages,
-    // n6 fp16, n7 recent, n8 most moves
+    // n6 fp16, n7 recent, n8 most moves; f0 slots in LDS
     PEvictArgs a{};
     a.s = s;
     a.k = (void*)p[0];
@@ -983,13 +984,17 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     a.most = (uint32_t)n[8];
     a.in_place = p[2] == p[4] && p[3] == p[5];
     a.unit = half ? 2 : 4;
-    a.count = (uint32_t*)c->pws;
-    a.moves = a.count + n[0] * n[2];
-    out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, 0, a));
-    if (a.most) {
+    const bool here = a.most <= SLM_MOVES_HERE;
+    if (!here) {
+        a.count = (uint32_t*)c->pws;
+        a.moves = a.count + n[0] * n[2];
+    }
+    a.room = (uint32_t)o.f[0];
+    a.vec = a.page % 4 == 0 && aligned16(a.mass) && aligned16(a.born) && aligned16(a.mass_out) && aligned16(a.born_out);
+    out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, a.room * 4 + a.room / 8, a));
+    if (!here) {
         uint32_t blocks = (a.most + 63) / 64;
-        Rec r = mk_desc(k.pmove[half], (uint32_t)(n[0] * n[2]) * blocks, 256, 0, PMoveArgs{a, blocks});
-        out.push_back(r);
+        out.push_back(mk_desc(k.pmove[a.dh * a.unit % 16 != 0], (uint32_t)(n[0] * n[2]) * blocks, 256, 0, PMoveArgs{a, blocks}));
     }
     return SLM_OK;
 }
@@ -5290,7 +5295,7 @@ int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass
     size_t pairs = s->n * g->key_heads;
     if (pairs >= (size_t)1 << 24 || pairs * ((most + 63) / 64) >= (size_t)1 << 31)
         return fail(c, SLM_E_UNSUPPORTED, "paged_evict: %zu sequences of %zu key heads", s->n, g->key_heads);
-    TRY(need_pws(c, pairs * 4 + pairs * 2 * most * 4));
+    if (most > SLM_MOVES_HERE) TRY(need_pws(c, pairs * 4 + pairs * 2 * most * 4));
     Op o = op(OP_PEVICT);
     o.p[0] = g->k;
     o.p[1] = g->v;
@@ -5309,6 +5314,8 @@ int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass
     o.n[7] = (int64_t)recent;
     o.n[8] = (int64_t)most;
     o.n[9] = (int64_t)s->width;
+    // the longest sequence's keys in LDS, as far as they go (and in steps, as the moves)
+    o.f[0] = (float)std::min<int64_t>(((int64_t)s->max_len + 1023) / 1024 * 1024, EVICT_ROOM);
     return submit(c, o);
 }
 
