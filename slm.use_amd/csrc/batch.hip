@@ -520,19 +520,28 @@ __device__ __forceinline__ uint32_t mass_key(float m, uint32_t born, uint32_t re
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Exclusive prefix of one value a wave over the workgroup's 16 waves, and the total.
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t v, uint32_t* s, uint32_t* total) {
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or0(uint32_t x) {  // 0 where the lane has no such neighbour
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true);
+}
+// Inclusive prefix sums over a wave: within rows of 16, then the rows' last lanes to those behind.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += dpp_or0<0x111, 0xF>(x);
+    x += dpp_or0<0x112, 0xF>(x);
+    x += dpp_or0<0x114, 0xF>(x);
+    x += dpp_or0<0x118, 0xF>(x);
+    x += dpp_or0<0x142, 0xA>(x);
+    x += dpp_or0<0x143, 0xC>(x);
+    return x;
+}
+// Exclusive prefix sum over a workgroup of sixteen waves. s: 16 words of LDS of this call's own.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t incl = wave_scan(x);
+    if (lane == 63) s[w] = incl;
     __syncthreads();
-    if (lane == 0) s[w] = v;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int i = 0; i < 16; i++) {
-        if (i < w) before += s[i];
-        all += s[i];
-    }
-    *total = all;
-    return before;
+    uint32_t before = wave_scan(lane < 16 ? s[lane] : 0);
+    return (w ? __builtin_amdgcn_readlane(before, w - 1) : 0) + incl - x;
 }
 
 // Row `from` to row `to`, V at a time: lane c of sixteen.
@@ -552,15 +561,17 @@ __device__ __forceinline__ void move_row(const PEvictArgs& a, uint32_t to, uint3
 
 // A workgroup of 1024 a (sequence, key head). The slots' keys are read once, into LDS (up to
 // `room` of them; those of longer sequences are read again each time). The keep-th largest is
-// found by three rounds of counting digits (11, 11 and 10 bits); then, over the slots in order, a
-// wave a run of them: which of the first `keep` are left, and which of those behind move there.
-// Few moves (SLM_MOVES_HERE) are made here, more by a launch of their own.
+// found by rounds of counting digits (11, 11 and 10 bits), fewer where a round's digit leaves no
+// key to be told from another. Then the slots that stay, a bit each, 64 a wave at a time; from
+// the words' counts, added up, which of the first `keep` are left and which of those behind move
+// there. Few moves (SLM_MOVES_HERE) are made here, more by a launch of their own.
 KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     __shared__ uint32_t hist[2048];
-    __shared__ uint32_t red[16];
-    __shared__ uint32_t pick[3];
+    __shared__ uint32_t red[6][16];
+    __shared__ uint32_t pick[3][3];
     uint32_t* keys = (uint32_t*)lds_;                         // [room]
     uint64_t* stays = (uint64_t*)(keys + a.room);             // [room / 64]: the slots that stay, a bit each
+    uint32_t* counts = (uint32_t*)(stays + a.room / 64);      // [room / 64]: what comes before a word's
     const int h = blockIdx.x % a.kh, b = blockIdx.x / a.kh, tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t len = a.s.len[b], seen = a.s.seen[b];
@@ -568,148 +579,217 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     if (!over && tid == 0 && a.count) a.count[blockIdx.x] = 0;
     if (!over && a.in_place) return;
 
-    auto key_at = [&](uint32_t row) { return mass_key(a.mass[row], a.born[row], a.recent, seen); };
-    auto key_of = [&](uint32_t t) { return held ? keys[t] : key_at(row_of(a.s, b, t, h, a.kh, a.page)); };
-    auto digit = [&](uint32_t k) { atomicAdd(&hist[k >> 21], 1u); };
+    auto row = [&](uint32_t t) { return row_of(a.s, b, t, h, a.kh, a.page); };
+    auto key_at = [&](uint32_t r) { return mass_key(a.mass[r], a.born[r], a.recent, seen); };
+    auto key_of = [&](uint32_t t) { return held ? keys[t] : key_at(row(t)); };
+    auto front = [&](uint32_t t0) -> uint64_t {  // the slots of t0's 64 that are among the first `keep`
+        return a.keep <= t0 ? 0 : a.keep - t0 >= 64 ? ~0ull : (1ull << (a.keep - t0)) - 1;
+    };
+    auto there = [&](uint32_t t0) -> uint64_t {  // ... that hold a token
+        return len <= t0 ? 0 : len - t0 >= 64 ? ~0ull : (1ull << (len - t0)) - 1;
+    };
     if (over) {
-        for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
+        auto count = [&](uint32_t k) { atomicAdd(&hist[k >> 21], 1u); };
+        hist[2 * tid] = hist[2 * tid + 1] = 0;
         __syncthreads();
-        if (held && a.vec) {  // four slots of a page at once
-            for (uint32_t t = 4 * tid; t < len; t += 4096) {
-                uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
-                f4 m = *(const f4*)(a.mass + row);
-                uint4 p = *(const uint4*)(a.born + row);
-                uint4 k = {mass_key(m.x, p.x, a.recent, seen), mass_key(m.y, p.y, a.recent, seen),
-                           mass_key(m.z, p.z, a.recent, seen), mass_key(m.w, p.w, a.recent, seen)};
-                *(uint4*)(keys + t) = k;
-                digit(k.x);
-                if (t + 1 < len) digit(k.y);
-                if (t + 2 < len) digit(k.z);
-                if (t + 3 < len) digit(k.w);
+        if (held && a.vec) {  // four slots of a page at once, four times over
+            for (uint32_t t0 = 4 * tid; t0 < len; t0 += 16384) {
+                f4 m[4];
+                uint4 p[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    uint32_t r = row(min(t0 + 4096 * u, (len - 1) & ~3u));
+                    m[u] = *(const f4*)(a.mass + r);
+                    p[u] = *(const uint4*)(a.born + r);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    uint32_t t = t0 + 4096 * u;
+                    if (t >= len) break;
+                    uint4 k = {mass_key(m[u].x, p[u].x, a.recent, seen), mass_key(m[u].y, p[u].y, a.recent, seen),
+                               mass_key(m[u].z, p[u].z, a.recent, seen), mass_key(m[u].w, p[u].w, a.recent, seen)};
+                    *(uint4*)(keys + t) = k;
+                    count(k.x);
+                    if (t + 1 < len) count(k.y);
+                    if (t + 2 < len) count(k.z);
+                    if (t + 3 < len) count(k.w);
+                }
             }
         } else {
             for (uint32_t t = tid; t < len; t += 1024) {
-                uint32_t k = key_at(row_of(a.s, b, t, h, a.kh, a.page));
+                uint32_t k = key_at(row(t));
                 if (held) keys[t] = k;
-                digit(k);
+                count(k);
             }
         }
         __syncthreads();
     }
-    uint32_t prefix = 0, need = a.keep;  // keys that share the digits so far: `need` of them stay
-    bool ties = false;                   // ... and some of the last such keys go
-    for (int round = 0; round < 3 && over; round++) {
-        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+    // the first `need` of the keys that are `prefix` from bit `shift` up stay, and all above
+    uint32_t prefix = 0, need = a.keep;
+    int shift = 32;
+    bool ties = over;  // ... and some such keys go
+    for (int round = 0; round < 3 && ties; round++) {
+        const int bits = round == 2 ? 10 : 11;
         if (round) {
-            for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
-            __syncthreads();
             for (uint32_t t = tid; t < len; t += 1024) {
                 uint32_t k = key_of(t);
-                if ((k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+                if (k >> shift == prefix) atomicAdd(&hist[(k >> (shift - bits)) & ((1u << bits) - 1)], 1u);
             }
             __syncthreads();
         }
+        shift -= bits;
         // the digit at which the count from above reaches `need`: each thread two bins, from above
-        uint32_t h1 = hist[2047 - 2 * tid], h0 = hist[2046 - 2 * tid], mine = h1 + h0;
-        uint32_t incl = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-            uint32_t v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
-        uint32_t total, before = wave_prefix(__shfl(incl, 63), red, &total) + incl - mine;
-        if (before < need && before + mine >= need) {
+        uint32_t h1 = hist[2047 - 2 * tid], h0 = hist[2046 - 2 * tid];
+        hist[2047 - 2 * tid] = hist[2046 - 2 * tid] = 0;
+        uint32_t before = block_scan(h1 + h0, red[round]);
+        if (before < need && before + h1 + h0 >= need) {
             bool first = before + h1 >= need;
-            pick[0] = 2047 - 2 * tid - (first ? 0 : 1);
-            pick[1] = need - before - (first ? 0 : h1);
-            pick[2] = (first ? h1 : h0) > pick[1];
+            pick[round][0] = 2047 - 2 * tid - (first ? 0 : 1);
+            pick[round][1] = need - before - (first ? 0 : h1);
+            pick[round][2] = (first ? h1 : h0) > pick[round][1];
         }
         __syncthreads();
-        prefix = (prefix << bits) | pick[0];
-        need = pick[1];
-        ties = pick[2] != 0;
-        __syncthreads();
+        prefix = (prefix << bits) | pick[round][0];
+        need = pick[round][1];
+        ties = pick[round][2] != 0;
     }
-    if (over) {
-        // keys above `prefix` stay, and the first `need` of those equal to it. A wave takes a
-        // run of whole 64s of slots.
+    uint32_t* to = a.count ? a.moves + (int64_t)blockIdx.x * 2 * a.most : hist;  // (few: in LDS)
+    uint32_t* from = to + a.most;
+    uint32_t moves = 0;
+    if (over && held) {
+        const uint32_t words = (len + 63) / 64;
+        if (ties) {  // equal keys: the lower slots stay
+            for (uint32_t q = w; q < words; q += 16) {
+                uint64_t em = __ballot(64 * q + lane < len && keys[64 * q + lane] == prefix);
+                if (lane == 0) counts[q] = __popcll(em);
+            }
+            __syncthreads();
+            uint32_t before = block_scan(tid < words ? counts[tid] : 0, red[3]);
+            if (tid < words) counts[tid] = before;
+            __syncthreads();
+        }
+#pragma unroll 4
+        for (uint32_t q = w; q < words; q += 16) {
+            const bool in = 64 * q + lane < len;
+            uint32_t k = keys[min(64 * q + lane, len - 1)] >> shift;
+            uint64_t m = __ballot(in && k >= prefix);
+            if (ties) {
+                uint64_t em = __ballot(in && k == prefix);
+                m = __ballot(in && (k > prefix || (k == prefix && counts[q] + lanes_below(em) < need)));
+            }
+            if (lane == 0) stays[q] = m;
+        }
+        __syncthreads();
+        // holes below, movers above: both counts in one word (neither passes 2^16)
+        uint32_t both = 0;
+        if (tid < words) {
+            uint64_t m = stays[tid], f = front(64 * tid);
+            both = __popcll(~m & f & there(64 * tid)) | __popcll(m & ~f) << 16;
+        }
+        uint32_t before = block_scan(both, red[4]);
+        if (tid < words) counts[tid] = before;
+        if (tid == words - 1) pick[0][0] = (before + both) >> 16;
+        __syncthreads();
+        moves = pick[0][0];
+#pragma unroll 4
+        for (uint32_t q = w; q < words; q += 16) {
+            uint64_t m = stays[q], f = front(64 * q), hm = ~m & f & there(64 * q), mm = m & ~f;
+            uint32_t n = counts[q];
+            if (hm >> lane & 1) to[(n & 0xffff) + lanes_below(hm)] = 64 * q + lane;
+            if (mm >> lane & 1) from[(n >> 16) + lanes_below(mm)] = 64 * q + lane;
+        }
+    } else if (over) {
+        // too many for LDS: a wave a run of whole 64s of slots, their keys read again each time
         const uint32_t run = (len + 1024 - 1) / 1024 * 64, lo = min(len, w * run), hi = min(len, lo + run);
-        uint32_t total, tie0 = 0;
+        uint32_t tie0 = 0;
+        auto stay = [&](uint32_t t0, uint32_t& tie) -> uint64_t {
+            const bool in = t0 + lane < hi;
+            uint32_t k = in ? key_of(t0 + lane) >> shift : 0;
+            uint64_t em = __ballot(in && k == prefix);
+            uint64_t m = __ballot(in && (k > prefix || (k == prefix && (!ties || tie + lanes_below(em) < need))));
+            tie += __popcll(em);
+            return m;
+        };
+        auto sum_before = [&](uint32_t n, uint32_t* s, uint32_t* all) {  // over the waves before this one
+            uint32_t v = block_scan(lane == 0 ? n : 0, s);
+            __syncthreads();
+            *all = 0;
+            for (int i = 0; i < 16; i++) *all += s[i];
+            return (uint32_t)__builtin_amdgcn_readfirstlane(v);
+        };
+        uint32_t all;
         if (ties) {
             uint32_t n = 0;
-            for (uint32_t t0 = lo; t0 < hi; t0 += 64) n += __popcll(__ballot(t0 + lane < hi && key_of(t0 + lane) == prefix));
-            tie0 = wave_prefix(n, red, &total);
+            for (uint32_t t0 = lo; t0 < hi; t0 += 64) n += __popcll(__ballot(t0 + lane < hi && key_of(t0 + lane) >> shift == prefix));
+            tie0 = sum_before(n, red[3], &all);
         }
-        auto stays_of = [&](uint32_t t0, uint32_t& tie) -> uint64_t {
-            const bool in = t0 + lane < hi;
-            uint32_t k = in ? key_of(t0 + lane) : 0;
-            if (!ties) return __ballot(in && k >= prefix);
-            uint64_t em = __ballot(in && k == prefix);
-            uint64_t mask = __ballot(in && (k > prefix || (k == prefix && tie + lanes_below(em) < need)));
-            tie += __popcll(em);
-            return mask;
-        };
-        auto below = [](uint32_t t0, uint32_t end) -> uint64_t {  // bits of the slots before `end`
-            return end <= t0 ? 0 : end - t0 >= 64 ? ~0ull : (1ull << (end - t0)) - 1;
-        };
         uint32_t holes = 0, movers = 0, tie = tie0;
         for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
-            uint64_t m = stays_of(t0, tie), front = below(t0, a.keep);
-            if (held && lane == 0) stays[t0 / 64] = m;
-            holes += __popcll(~m & front & below(t0, len));
-            movers += __popcll(m & ~front);
+            uint64_t m = stay(t0, tie);
+            holes += __popcll(~m & front(t0) & there(t0));
+            movers += __popcll(m & ~front(t0));
         }
-        uint32_t nm, hole0 = wave_prefix(holes, red, &nm), mover0 = wave_prefix(movers, red, &nm);
-        uint32_t* to = a.count ? a.moves + (int64_t)blockIdx.x * 2 * a.most : hist;  // (few: in LDS)
-        uint32_t* from = to + a.most;
-        if (tid == 0 && a.count) a.count[blockIdx.x] = nm;
+        uint32_t hole0 = sum_before(holes, red[4], &all), mover0 = sum_before(movers, red[5], &moves);
         tie = tie0;
         for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
-            uint64_t m = held ? stays[t0 / 64] : stays_of(t0, tie), front = below(t0, a.keep);
-            uint64_t hm = ~m & front & below(t0, len), mm = m & ~front;
+            uint64_t m = stay(t0, tie), f = front(t0), hm = ~m & f & there(t0), mm = m & ~f;
             if (hm >> lane & 1) to[hole0 + lanes_below(hm)] = t0 + lane;
             if (mm >> lane & 1) from[mover0 + lanes_below(mm)] = t0 + lane;
             hole0 += __popcll(hm);
             mover0 += __popcll(mm);
-            if (!held && !a.in_place && (m & front) >> lane & 1) {
-                uint32_t row = row_of(a.s, b, t0 + lane, h, a.kh, a.page);
-                a.mass_out[row] = a.mass[row];
-                a.born_out[row] = a.born[row];
+            if (!a.in_place && (m & f) >> lane & 1) {
+                uint32_t r = row(t0 + lane);
+                a.mass_out[r] = a.mass[r];
+                a.born_out[r] = a.born[r];
             }
         }
-        __syncthreads();
-        if (!a.count)
-            for (uint32_t i = tid / 16; i < nm; i += 64) {
-                uint32_t d = row_of(a.s, b, to[i], h, a.kh, a.page), f = row_of(a.s, b, from[i], h, a.kh, a.page);
-                if (a.dh * a.unit % 16 == 0) move_row<f4>(a, d, f, tid % 16);
-                else move_row<h4>(a, d, f, tid % 16);
+    }
+    if (over) {
+        if (a.count) {
+            if (tid == 0) a.count[blockIdx.x] = moves;
+        } else {
+            // rows of all the moves first, then four of them a group of sixteen lanes at a time
+            __syncthreads();
+            for (uint32_t i = tid; i < 2 * moves; i += 1024) {
+                uint32_t at = i < moves ? i : a.most + i - moves;
+                to[at] = row(to[at]);
             }
+            __syncthreads();
+            if (a.dh * a.unit % 16 == 0) {
+#pragma unroll 4
+                for (uint32_t i = tid / 16; i < moves; i += 64) move_row<f4>(a, to[i], from[i], tid % 16);
+            } else {
+                for (uint32_t i = tid / 16; i < moves; i += 64) move_row<h4>(a, to[i], from[i], tid % 16);
+            }
+        }
         if (a.in_place || !held) return;
     }
     // mass and born of what stays where it is, into the buffers for them
     const uint32_t end = min(len, a.keep);
     if (a.vec) {
+#pragma unroll 2
         for (uint32_t t = 4 * tid; t < end; t += 4096) {
-            uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
+            uint32_t r = row(t);
             uint32_t m = over ? (uint32_t)(stays[t / 64] >> (t % 64)) & 15 : 15;
             if (end - t < 4) m &= (1u << (end - t)) - 1;
-            f4 mass = *(const f4*)(a.mass + row);
-            uint4 born = *(const uint4*)(a.born + row);
+            f4 mass = *(const f4*)(a.mass + r);
+            uint4 born = *(const uint4*)(a.born + r);
             if (m == 15) {
-                *(f4*)(a.mass_out + row) = mass;
-                *(uint4*)(a.born_out + row) = born;
+                *(f4*)(a.mass_out + r) = mass;
+                *(uint4*)(a.born_out + r) = born;
                 continue;
             }
-            if (m & 1) a.mass_out[row] = mass.x, a.born_out[row] = born.x;
-            if (m & 2) a.mass_out[row + 1] = mass.y, a.born_out[row + 1] = born.y;
-            if (m & 4) a.mass_out[row + 2] = mass.z, a.born_out[row + 2] = born.z;
-            if (m & 8) a.mass_out[row + 3] = mass.w, a.born_out[row + 3] = born.w;
+            if (m & 1) a.mass_out[r] = mass.x, a.born_out[r] = born.x;
+            if (m & 2) a.mass_out[r + 1] = mass.y, a.born_out[r + 1] = born.y;
+            if (m & 4) a.mass_out[r + 2] = mass.z, a.born_out[r + 2] = born.z;
+            if (m & 8) a.mass_out[r + 3] = mass.w, a.born_out[r + 3] = born.w;
         }
     } else {
         for (uint32_t t = tid; t < end; t += 1024) {
             if (over && !(stays[t / 64] >> (t % 64) & 1)) continue;
-            uint32_t row = row_of(a.s, b, t, h, a.kh, a.page);
-            a.mass_out[row] = a.mass[row];
-            a.born_out[row] = a.born[row];
+            uint32_t r = row(t);
+            a.mass_out[r] = a.mass[r];
+            a.born_out[r] = a.born[r];
         }
     }
 }

@@ -60,7 +60,7 @@ constexpr int ATTN_LDS_MAX = LDS_MAX;
 constexpr int ATTN_DEC_LDS = SLM_SB_SEGS * (2 * 64 * 64 + 1024) * 4;  // one-token attention: 256 keys and values, queries
 constexpr int GEMM_STAGES_HOST = 2;          // slices in flight in slm_gemm2 (GEMM_STAGES)
 constexpr int64_t CU_COUNT = 256;           // MI355X compute units
-constexpr int64_t EVICT_ROOM = 36352;       // slots whose keys (and a bit each) an eviction's workgroup holds in LDS
+constexpr int64_t EVICT_ROOM = 36352;       // slots whose keys an eviction's workgroup holds in LDS (4 3/16 bytes each)
 
 enum OpKind : uint32_t {
     OP_GATHER = 1, OP_COPY, OP_SHIFT, OP_COLUMNS, OP_LINEAR, OP_ADD, OP_ADD_ROW, OP_SCALE_ROWS,
@@ -991,7 +991,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     }
     a.room = (uint32_t)o.f[0];
     a.vec = a.page % 4 == 0 && aligned16(a.mass) && aligned16(a.born) && aligned16(a.mass_out) && aligned16(a.born_out);
-    out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, a.room * 4 + a.room / 8, a));
+    out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, a.room * 4 + a.room / 64 * 12, a));
     if (!here) {
         uint32_t blocks = (a.most + 63) / 64;
         out.push_back(mk_desc(k.pmove[a.dh * a.unit % 16 != 0], (uint32_t)(n[0] * n[2]) * blocks, 256, 0, PMoveArgs{a, blocks}));
