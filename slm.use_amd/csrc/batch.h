@@ -7,6 +7,7 @@
 
 #define SLM_PG_KEYS 256     // keys of a superblock: one workgroup's, whatever the batch
 #define SLM_MOVES_HERE 256  // moves of a sequence and key head that need no launch of their own
+#define SLM_MOVES_WG 64     // moves of a workgroup of such a launch
 #define SLM_TOP_MAX 32      // alternatives of a row of logits
 #define SLM_NO_SEQ 0xffffffffu
 

@@ -22,6 +22,11 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 static constexpr float NEG_INF = -__builtin_inff();
 
+// Memory that the compiler is to know as global, or as LDS (where it cannot tell, a store holds
+// up both kinds of loads).
+#define GLOBAL_MEM __attribute__((address_space(1)))
+#define LDS_MEM __attribute__((address_space(3)))
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
@@ -520,6 +525,11 @@ __device__ __forceinline__ uint32_t mass_key(float m, uint32_t born, uint32_t re
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {  // the same in every lane: to a scalar
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_or0(uint32_t x) {  // 0 where the lane has no such neighbour
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true);
@@ -544,18 +554,31 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s) {
     return (w ? __builtin_amdgcn_readlane(before, w - 1) : 0) + incl - x;
 }
 
-// Row `from` to row `to`, V at a time: lane c of sixteen.
+// Keys and values of rows from[] to rows to[], V at a time, by the workgroup: a power of two of
+// lanes a row, and `step` rows at once, four times over.
 template <typename V>
-__device__ __forceinline__ void move_row(const PEvictArgs& a, uint32_t to, uint32_t from, int c) {
-    const int vecs = a.dh * a.unit / (int)sizeof(V);
-    for (int i = c; i < vecs; i += 16) {
-        V kv = ((const V*)a.k)[(int64_t)from * vecs + i], vv = ((const V*)a.v)[(int64_t)from * vecs + i];
-        ((V*)a.k)[(int64_t)to * vecs + i] = kv;
-        ((V*)a.v)[(int64_t)to * vecs + i] = vv;
-    }
-    if (c == 0) {
-        a.mass_out[to] = a.mass[from];
-        a.born_out[to] = a.born[from];
+__device__ __forceinline__ void move_rows(const PEvictArgs& a, const uint32_t* to, const uint32_t* from, uint32_t n) {
+    const uint32_t vecs = (uint32_t)(a.dh * a.unit) / sizeof(V);
+    const int lg = vecs <= 1 ? 0 : 32 - __clz(vecs - 1);
+    const uint32_t c = threadIdx.x & ((1u << lg) - 1), r0 = threadIdx.x >> lg, step = blockDim.x >> lg;
+    if (c >= vecs) return;
+    V* k = (V*)a.k + c;
+    V* v = (V*)a.v + c;
+    for (uint32_t r = r0; r < n; r += 4 * step) {
+        V kv[4], vv[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            int64_t f = (int64_t)from[min(r + u * step, n - 1)] * vecs;
+            kv[u] = k[f];
+            vv[u] = v[f];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (r + u * step >= n) break;
+            int64_t t = (int64_t)to[r + u * step] * vecs;
+            k[t] = kv[u];
+            v[t] = vv[u];
+        }
     }
 }
 
@@ -653,8 +676,9 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
         need = pick[round][1];
         ties = pick[round][2] != 0;
     }
-    uint32_t* to = a.count ? a.moves + (int64_t)blockIdx.x * 2 * a.most : hist;  // (few: in LDS)
-    uint32_t* from = to + a.most;
+    // the lists of slots left and of slots that move there: in memory, or few of them in LDS
+    uint32_t* list = a.moves + (int64_t)blockIdx.x * 2 * a.most;
+    uint32_t *to = hist, *from = hist + SLM_MOVES_HERE;
     uint32_t moves = 0;
     if (over && held) {
         const uint32_t words = (len + 63) / 64;
@@ -691,13 +715,17 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
         if (tid == words - 1) pick[0][0] = (before + both) >> 16;
         __syncthreads();
         moves = pick[0][0];
+        auto write = [&](auto* to, auto* from) {
 #pragma unroll 4
-        for (uint32_t q = w; q < words; q += 16) {
-            uint64_t m = stays[q], f = front(64 * q), hm = ~m & f & there(64 * q), mm = m & ~f;
-            uint32_t n = counts[q];
-            if (hm >> lane & 1) to[(n & 0xffff) + lanes_below(hm)] = 64 * q + lane;
-            if (mm >> lane & 1) from[(n >> 16) + lanes_below(mm)] = 64 * q + lane;
-        }
+            for (uint32_t q = w; q < words; q += 16) {
+                uint64_t m = uniform(stays[q]), f = front(64 * q), hm = ~m & f & there(64 * q), mm = m & ~f;
+                uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane(counts[q]);
+                if (__builtin_amdgcn_inverse_ballot_w64(hm)) to[(n & 0xffff) + lanes_below(hm)] = 64 * q + lane;
+                if (__builtin_amdgcn_inverse_ballot_w64(mm)) from[(n >> 16) + lanes_below(mm)] = 64 * q + lane;
+            }
+        };
+        if (a.count) write((GLOBAL_MEM uint32_t*)list, (GLOBAL_MEM uint32_t*)(list + a.most));
+        else write((LDS_MEM uint32_t*)to, (LDS_MEM uint32_t*)from);
     } else if (over) {
         // too many for LDS: a wave a run of whole 64s of slots, their keys read again each time
         const uint32_t run = (len + 1024 - 1) / 1024 * 64, lo = min(len, w * run), hi = min(len, lo + run);
@@ -733,8 +761,14 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
         tie = tie0;
         for (uint32_t t0 = lo; t0 < hi; t0 += 64) {
             uint64_t m = stay(t0, tie), f = front(t0), hm = ~m & f & there(t0), mm = m & ~f;
-            if (hm >> lane & 1) to[hole0 + lanes_below(hm)] = t0 + lane;
-            if (mm >> lane & 1) from[mover0 + lanes_below(mm)] = t0 + lane;
+            if (__builtin_amdgcn_inverse_ballot_w64(hm)) {
+                if (a.count) ((GLOBAL_MEM uint32_t*)list)[hole0 + lanes_below(hm)] = t0 + lane;
+                else ((LDS_MEM uint32_t*)to)[hole0 + lanes_below(hm)] = t0 + lane;
+            }
+            if (__builtin_amdgcn_inverse_ballot_w64(mm)) {
+                if (a.count) ((GLOBAL_MEM uint32_t*)list)[a.most + mover0 + lanes_below(mm)] = t0 + lane;
+                else ((LDS_MEM uint32_t*)from)[mover0 + lanes_below(mm)] = t0 + lane;
+            }
             hole0 += __popcll(hm);
             mover0 += __popcll(mm);
             if (!a.in_place && (m & f) >> lane & 1) {
@@ -748,19 +782,19 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
         if (a.count) {
             if (tid == 0) a.count[blockIdx.x] = moves;
         } else {
-            // rows of all the moves first, then four of them a group of sixteen lanes at a time
+            // rows of all the moves first, then their keys and values, four loads of each in flight
             __syncthreads();
             for (uint32_t i = tid; i < 2 * moves; i += 1024) {
-                uint32_t at = i < moves ? i : a.most + i - moves;
-                to[at] = row(to[at]);
+                uint32_t at = i < moves ? i : SLM_MOVES_HERE + i - moves;
+                hist[at] = row(hist[at]);
             }
             __syncthreads();
-            if (a.dh * a.unit % 16 == 0) {
-#pragma unroll 4
-                for (uint32_t i = tid / 16; i < moves; i += 64) move_row<f4>(a, to[i], from[i], tid % 16);
-            } else {
-                for (uint32_t i = tid / 16; i < moves; i += 64) move_row<h4>(a, to[i], from[i], tid % 16);
+            for (uint32_t i = tid; i < moves; i += 1024) {
+                a.mass_out[to[i]] = a.mass[from[i]];
+                a.born_out[to[i]] = a.born[from[i]];
             }
+            if (a.dh * a.unit % 16 == 0) move_rows<f4>(a, to, from, moves);
+            else move_rows<h4>(a, to, from, moves);
         }
         if (a.in_place || !held) return;
     }
@@ -794,17 +828,24 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     }
 }
 
-// The moves of a (sequence, key head), 64 of them a workgroup: sixteen lanes a row.
+// The moves of a (sequence, key head), SLM_MOVES_WG of them a workgroup.
 template <typename V>
 __device__ __forceinline__ void move_body(const PEvictArgs& a, uint32_t blocks) {
-    const uint32_t pair = blockIdx.x / blocks, r0 = blockIdx.x % blocks * 64;
-    const uint32_t n = a.count[pair];
-    if (r0 >= n) return;
-    const int h = pair % a.kh, b = pair / a.kh, tid = threadIdx.x;
-    const uint32_t* to = a.moves + (int64_t)pair * 2 * a.most;
-    const uint32_t* from = to + a.most;
-    for (uint32_t r = r0 + tid / 16; r < min(n, r0 + 64); r += 16)
-        move_row<V>(a, row_of(a.s, b, to[r], h, a.kh, a.page), row_of(a.s, b, from[r], h, a.kh, a.page), tid % 16);
+    __shared__ uint32_t to[SLM_MOVES_WG], from[SLM_MOVES_WG];
+    const uint32_t pair = blockIdx.x / blocks, r0 = blockIdx.x % blocks * SLM_MOVES_WG, total = a.count[pair];
+    if (r0 >= total) return;
+    const int h = pair % a.kh, b = pair / a.kh;
+    const uint32_t n = min(total - r0, (uint32_t)SLM_MOVES_WG), i = threadIdx.x;
+    const uint32_t* list = a.moves + (int64_t)pair * 2 * a.most + r0;
+    if (i < n) {
+        uint32_t t = row_of(a.s, b, list[i], h, a.kh, a.page), f = row_of(a.s, b, list[a.most + i], h, a.kh, a.page);
+        to[i] = t;
+        from[i] = f;
+        a.mass_out[t] = a.mass[f];
+        a.born_out[t] = a.born[f];
+    }
+    __syncthreads();
+    move_rows<V>(a, to, from, n);
 }
 KERNEL void __launch_bounds__(256) slm_paged_move16(PMoveArgs a) { move_body<f4>(a.e, a.blocks); }
 KERNEL void __launch_bounds__(256) slm_paged_move8(PMoveArgs a) { move_body<h4>(a.e, a.blocks); }

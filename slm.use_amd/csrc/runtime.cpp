@@ -993,7 +993,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     a.vec = a.page % 4 == 0 && aligned16(a.mass) && aligned16(a.born) && aligned16(a.mass_out) && aligned16(a.born_out);
     out.push_back(mk_desc(k.pselect, (uint32_t)(n[0] * n[2]), 1024, a.room * 4 + a.room / 64 * 12, a));
     if (!here) {
-        uint32_t blocks = (a.most + 63) / 64;
+        uint32_t blocks = (a.most + SLM_MOVES_WG - 1) / SLM_MOVES_WG;
         out.push_back(mk_desc(k.pmove[a.dh * a.unit % 16 != 0], (uint32_t)(n[0] * n[2]) * blocks, 256, 0, PMoveArgs{a, blocks}));
     }
     return SLM_OK;
@@ -5293,7 +5293,7 @@ int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass
     while (step * 8 <= most) step *= 2;
     most = (most + step - 1) / step * step;
     size_t pairs = s->n * g->key_heads;
-    if (pairs >= (size_t)1 << 24 || pairs * ((most + 63) / 64) >= (size_t)1 << 31)
+    if (pairs >= (size_t)1 << 24 || pairs * ((most + SLM_MOVES_WG - 1) / SLM_MOVES_WG) >= (size_t)1 << 24)
         return fail(c, SLM_E_UNSUPPORTED, "paged_evict: %zu sequences of %zu key heads", s->n, g->key_heads);
     if (most > SLM_MOVES_HERE) TRY(need_pws(c, pairs * 4 + pairs * 2 * most * 4));
     Op o = op(OP_PEVICT);
