@@ -9,6 +9,7 @@
 #define SLM_MOVES_HERE 256  // moves of a sequence and key head that need no launch of their own
 #define SLM_MOVES_WG 64     // moves of a workgroup of such a launch
 #define SLM_TOP_MAX 32      // alternatives of a row of logits
+#define SLM_FEW_IDS 256     // tokens that go to the kernel with its arguments
 #define SLM_NO_SEQ 0xffffffffu
 
 // A batch of sequences on the device (slm_seqs).
@@ -75,12 +76,13 @@ struct PMoveArgs {
 
 struct LogpArgs {
     const float* x;          // [m][n]
-    const uint32_t* ids;     // [m]
+    const uint32_t* ids;     // [m], or null: in `few`
     float *lp, *ent;         // [m]; ent may be null
     uint32_t* top_ids;       // [m][top]
     float* top_lp;
     int64_t m, n;
     int32_t top;
+    uint32_t few[SLM_FEW_IDS];  // up to this many rows' tokens, outside a recorded step
 };
 
 #endif

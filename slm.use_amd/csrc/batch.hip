@@ -888,11 +888,11 @@ struct RowSum {
     }
 };
 
-// The largest t (to 20 bits) such that at least `want` of the wave's 64 keys are >= t: by its
-// bits from above, a ballot each; two wants at once.
+// The largest t (to 16 bits: a bound is all it is for) such that at least `want` of the wave's 64
+// keys are >= t: by its bits from above, a ballot each; two wants at once.
 __device__ __forceinline__ void wave_nth(uint32_t key, int want0, int want1, uint32_t& t0, uint32_t& t1) {
     t0 = t1 = 0;
-    for (int bit = 31; bit >= 12; bit--) {
+    for (int bit = 31; bit >= 16; bit--) {
         uint32_t c0 = t0 | (1u << bit), c1 = t1 | (1u << bit);
         if (__popcll(__ballot(key >= c0)) >= want0) t0 = c0;
         if (__popcll(__ballot(key >= c1)) >= want1) t1 = c1;
@@ -912,7 +912,7 @@ template <int W>
 __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     __shared__ uint64_t list[W][128], fin[W * 64];
     __shared__ uint32_t cnts[W], bound[W][2], nfin;
-    __shared__ float sums[W][4];
+    __shared__ __attribute__((aligned(16))) float sums[W][4];
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.top;
     const float* x = a.x + row * a.n;
@@ -920,7 +920,7 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     const int a0 = (int)(((uintptr_t)x >> 2) & 3), end = (int)a.n + a0;
     const float* xa = x - a0;
     const int fair = (top + W - 1) / W;
-    const float given = x[a.ids[row]];
+    const float given = x[a.ids ? a.ids[row] : a.few[row]];
     if (tid == 0) nfin = 0;
 
     auto threshold = [&](uint32_t key) -> uint32_t {
@@ -1025,41 +1025,39 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
         }
     }
 
-    // the row's sums: the wave's, then the waves' in order
+    // the row's sums: the wave's, then the waves' (a lane of each row of 16 for each)
     float m = wave_max(s.m);
     s.raise(m);
     s.c = wave_sum(s.c);
     s.S = wave_sum(s.S);
     s.E = wave_sum(s.E);
     if (lane == 0) {
-        sums[w][0] = m;
-        sums[w][1] = s.c;
-        sums[w][2] = s.S;
-        sums[w][3] = s.E;
+        *(f4*)sums[w] = f4{m, s.c, s.S, s.E};
         cnts[w] = cnt;
     }
     __syncthreads();
-    m = sums[0][0];
-    int total = cnts[0];
-#pragma unroll
-    for (int i = 1; i < W; i++) {
-        m = fmaxf(m, sums[i][0]);
-        total += cnts[i];
+    s = RowSum{NEG_INF, 0.0f, 0.0f, 0.0f};
+    int total = 0;
+    if ((lane & 15) < W) {
+        f4 q = *(const f4*)sums[lane & 15];
+        s = RowSum{q.x, q.y, q.z, q.w};
+        total = cnts[lane & 15];
     }
-    float c = 0.0f, S = 0.0f, E = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; i++) {
-        RowSum q{sums[i][0], sums[i][1], sums[i][2], sums[i][3]};
-        q.raise(m);
-        c += q.c;
-        S += q.S;
-        E += q.E;
-    }
-    const bool none = m == NEG_INF && S == 0.0f;  // no logit above -inf (and no NaN)
-    const float logl = logf(c) + log1pf(S / c);
-    if (tid == 0) {
-        a.lp[row] = none ? NEG_INF : (given - m) - logl;
-        if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - E / (c + S);
+    m = row_max(s.m);
+    s.raise(m);
+    s.c = row_sum(s.c);
+    s.S = row_sum(s.S);
+    s.E = row_sum(s.E);
+    total = (int)row_sum((float)total);
+    // no logit above -inf (and no NaN): no token is possible
+    const bool none = m == NEG_INF && s.S == 0.0f;
+    auto logp = [&](float x) { return none ? NEG_INF : (x - m) - (logf(s.c) + log1pf(s.S / s.c)); };
+    if (w == 0) {
+        float l = logp(given);
+        if (lane == 0) {
+            a.lp[row] = l;
+            if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + (logf(s.c) + log1pf(s.S / s.c)) - s.E / (s.c + s.S);
+        }
     }
     if (!top) return;
     uint64_t e = lane < cnt ? list[w][lane] : 0;
@@ -1067,17 +1065,24 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
         uint32_t t = threshold((uint32_t)(e >> 32));
         if ((uint32_t)(e >> 32) < t) e = 0;
     }
-    if (e) fin[atomicAdd(&nfin, 1u)] = e;
+    {  // a wave's share of the places at once
+        uint64_t mask = __ballot(e != 0);
+        uint32_t at = 0;
+        if (lane == 0 && mask) at = atomicAdd(&nfin, (uint32_t)__popcll(mask));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane(at) + lanes_below(mask);
+        if (e) fin[at] = e;
+    }
     __syncthreads();
     const int n = nfin;
-    if (tid >= n) return;
-    e = fin[tid];
+    if (64 * w >= n) return;
+    e = tid < n ? fin[tid] : 0;
     int r = 0;
+#pragma unroll 8
     for (int i = 0; i < n; i++) r += fin[i] > e;
-    if (r < top) {
+    if (tid < n && r < top) {
         uint32_t key = (uint32_t)(e >> 32), id = 0xffffffffu - (uint32_t)e;
         a.top_ids[row * top + r] = id;
-        a.top_lp[row * top + r] = none ? NEG_INF : ((key ? logit_of(key) : __builtin_nanf("")) - m) - logl;
+        a.top_lp[row * top + r] = logp(key ? logit_of(key) : __builtin_nanf(""));
     }
 }
 KERNEL void __launch_bounds__(256) slm_logprobs_4(LogpArgs a) { logprobs_body<4>(a); }

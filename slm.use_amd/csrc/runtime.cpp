@@ -900,10 +900,11 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const Kernels& k = c->k;
     const float* const* p = o.p;
     const int64_t* n = o.n;
-    if (o.kind == OP_LOGPROBS) {  // p0 lp, p1 entropy, p2 top ids, p3 top lp, p4 x; n0 m, n1 n, n2 top; dyn ids
+    if (o.kind == OP_LOGPROBS) {  // p0 lp, p1 entropy, p2 top ids, p3 top lp, p4 x; n0 m, n1 n, n2 top, n3 ids on the host; dyn ids
         LogpArgs a{};
         a.x = p[4];
-        a.ids = (const uint32_t*)o.dyn;
+        if (n[3]) std::memcpy(a.few, (const uint32_t*)o.dyn, (size_t)n[0] * 4);  // (host memory, of this call)
+        else a.ids = (const uint32_t*)o.dyn;
         a.lp = (float*)p[0];
         a.ent = (float*)p[1];
         a.top_ids = (uint32_t*)p[2];
@@ -5354,7 +5355,14 @@ int slm_hip_logprobs(slm_hip* c, float* lp, float* entropy, uint32_t* top_ids, f
     o.n[0] = (int64_t)m;
     o.n[1] = (int64_t)n;
     o.n[2] = (int64_t)top;
-    TRY(stage(c, ids, m * 4, &o.dyn));
+    // a few tokens go with the launch (a copy of four bytes ahead of it takes longer than it
+    // does); in a recorded step they are the step's values
+    if (m <= SLM_FEW_IDS && !recording(c)) {
+        o.n[3] = 1;
+        o.dyn = ids;
+    } else {
+        TRY(stage(c, ids, m * 4, &o.dyn));
+    }
     return submit(c, o);
 }
 
