@@ -122,7 +122,7 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 // takes one superblock of SLM_PG_KEYS slots, its waves 64 / NT keys each (NT: the head size in
 // 64s); for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
 // x = (scale · log2 e) q·k over its keys, the workgroup those of the superblock, and
-// slm_paged_join adds the superblocks up. No visible key: m = -inf; one at least: m >= -FLT_MAX.
+// slm_paged_join_* adds the superblocks up. No visible key: m = -inf; one at least: m >= -FLT_MAX.
 //
 // What bounds it is the reading of keys and values, so a wave issues all of its own (32 KB of
 // fp32) at once, straight into registers, as soon as it has its rows' addresses: 16 lanes read
@@ -187,14 +187,28 @@ __device__ __forceinline__ uint32_t looks(const PAttnArgs& a, uint32_t len) {
 }
 
 // M = max m_z and L = sum l_z 2^(m_z - M) over nz superblocks for one head, by a wave: lane z % 64
-// adds z in order, the lanes as one tree.
+// adds z in order, the lanes as one tree. (Up to 512 superblocks are read once, all at once.)
 __device__ __forceinline__ float2 join_ml(const float2* ml, int nz) {
     const int lane = threadIdx.x & 63;
-    float m = NEG_INF;
-    for (int z = lane; z < nz; z += 64) m = fmaxf(m, ml[z].x);
+    float2 v = make_float2(NEG_INF, 0.0f);
+    if (lane < nz) v = ml[lane];
+    if (nz <= 64) {
+        float m = wave_max(v.x);
+        return make_float2(m, wave_sum(v.y * __builtin_amdgcn_exp2f(v.x - (m == NEG_INF ? 0.0f : m))));
+    }
+    float2 q[7];
+#pragma unroll
+    for (int i = 0; i < 7; i++) q[i] = lane + 64 * i + 64 < nz ? ml[lane + 64 * i + 64] : make_float2(NEG_INF, 0.0f);
+    float m = v.x;
+#pragma unroll
+    for (int i = 0; i < 7; i++) m = fmaxf(m, q[i].x);
+    for (int z = lane + 512; z < nz; z += 64) m = fmaxf(m, ml[z].x);
     m = wave_max(m);
-    float l = 0.0f, ms = m == NEG_INF ? 0.0f : m;
-    for (int z = lane; z < nz; z += 64) {
+    const float ms = m == NEG_INF ? 0.0f : m;
+    float l = v.y * __builtin_amdgcn_exp2f(v.x - ms);
+#pragma unroll
+    for (int i = 0; i < 7; i++) l = fmaf(q[i].y, __builtin_amdgcn_exp2f(q[i].x - ms), l);
+    for (int z = lane + 512; z < nz; z += 64) {
         float2 p = ml[z];
         l = fmaf(p.y, __builtin_amdgcn_exp2f(p.x - ms), l);
     }
@@ -437,26 +451,38 @@ PAGED_ATTN(slm_paged_attn16_4_16, _Float16, 4, 16)
 
 // y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), superblock z in group z % KG of
 // dh / 4 threads, a group in order, then the groups in order. Behind them, with mass_out, four
-// waves a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g.
-KERNEL void __launch_bounds__(1024) slm_paged_join(PAttnArgs a) {
-    __shared__ f4 so[1024];
-    __shared__ float2 sml[4][16];
+// waves a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g. Sixteen waves a
+// workgroup, or four where that still leaves every superblock a group of its own (the same sums).
+template <int THREADS>
+__device__ __forceinline__ void join_body(const PAttnArgs& a) {
+    __shared__ f4 so[THREADS];
+    __shared__ float2 sml[THREADS / 256][16];
     const int tid = threadIdx.x, H = a.heads, dh = a.dh;
     if ((int)blockIdx.x < a.s.n * H) {
         const int b = blockIdx.x / H, head = blockIdx.x % H;
         const int nz = (int)((looks(a, a.s.len[b]) + SLM_PG_KEYS - 1) / SLM_PG_KEYS);
         const int64_t z0 = a.s.ifirst[b];
         const float2* ml = (const float2*)a.ml + (int64_t)head * a.items + z0;
+        const int cols = dh / 4, KG = THREADS / cols, c = tid % cols, zg = tid / cols;
+        const float* po = a.po + (z0 * H + head) * dh + 4 * c;
+        const bool mine = zg < KG && zg < nz;
+        f4 v = {0, 0, 0, 0};
+        float mz = NEG_INF;
+        if (mine) {  // (the first of its superblocks, on its way while the sums are made)
+            v = *(const f4*)(po + (int64_t)zg * H * dh);
+            mz = ml[zg].x;
+        }
         const float2 ML = join_ml(ml, nz);
-        const int cols = dh / 4, KG = 1024 / cols, c = tid % cols, zg = tid / cols;
         const float ms = ML.x == NEG_INF ? 0.0f : ML.x;
         f4 o = {0, 0, 0, 0};
-        if (zg < KG) {
-            const float* po = a.po + (z0 * H + head) * dh + 4 * c;
+        if (mine) {
+            float wz = __builtin_amdgcn_exp2f(mz - ms);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = v[e] * wz;
 #pragma unroll 4
-            for (int z = zg; z < nz; z += KG) {
-                float wz = __builtin_amdgcn_exp2f(ml[z].x - ms);
-                f4 v = *(const f4*)(po + (int64_t)z * H * dh);
+            for (int z = zg + KG; z < nz; z += KG) {
+                wz = __builtin_amdgcn_exp2f(ml[z].x - ms);
+                v = *(const f4*)(po + (int64_t)z * H * dh);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[e] = fmaf(v[e], wz, o[e]);
             }
@@ -473,7 +499,8 @@ KERNEL void __launch_bounds__(1024) slm_paged_join(PAttnArgs a) {
         }
         return;
     }
-    const int pair = ((int)blockIdx.x - a.s.n * H) * 4 + (tid >> 8), item = pair / a.kh, h = pair % a.kh, G = H / a.kh;
+    const int pair = ((int)blockIdx.x - a.s.n * H) * (THREADS / 256) + (tid >> 8);
+    const int item = pair / a.kh, h = pair % a.kh, G = H / a.kh;
     const int part = tid >> 8, w = (tid >> 6) & 3, key = tid & 255;
     uint4 it = {SLM_NO_SEQ, 0, 0, 0};
     if (item < a.items) it = ((const uint4*)a.s.items)[item];
@@ -512,6 +539,8 @@ KERNEL void __launch_bounds__(1024) slm_paged_join(PAttnArgs a) {
     }
     if (live && t < len) a.mass_out[slot] = old + add;
 }
+KERNEL void __launch_bounds__(256) slm_paged_join_4(PAttnArgs a) { join_body<256>(a); }
+KERNEL void __launch_bounds__(1024) slm_paged_join_16(PAttnArgs a) { join_body<1024>(a); }
 
 // ---------------------------------------------------------------------------------------
 // evict: which slots stay, then the moves

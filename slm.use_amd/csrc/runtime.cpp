@@ -154,7 +154,7 @@ struct Kernels {
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
-    hipFunction_t pstore[2], pattn[2][3][5], pjoin, pselect, pmove[2], logprobs[2];
+    hipFunction_t pstore[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2];
 };
 
 }  // namespace
@@ -891,6 +891,10 @@ SeqsDev seqs_dev(const slm_seqs* s, int64_t n, int64_t width) {
     return d;
 }
 
+// A paged attention's join (Op::f[1]): none, as no sequence has more than one superblock; four
+// waves a head, each superblock of the longest in a group of dh / 4 threads of its own; sixteen.
+constexpr float PATTEND_DIRECT = 0.0f, PATTEND_SHORT = 1.0f, PATTEND_LONG = 2.0f;
+
 // Bytes of the workspace that a paged attention of `items` superblocks uses.
 size_t pattend_bytes(size_t items, size_t heads, size_t dh, bool mass) {
     return items * heads * (2 + dh + (mass ? SLM_PG_KEYS : 0)) * 4;
@@ -948,7 +952,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         a.dh = (int32_t)n[4];
         a.gap = n[8];
         a.scale = o.f[0];
-        a.direct = o.f[1] != 0.0f;
+        a.direct = o.f[1] == PATTEND_DIRECT;
         a.items = (int32_t)n[7];
         a.r16 = c->fp16 ? 1 : 0;
         const int64_t items = n[7], H = n[1], kh = n[2], G = H / kh;
@@ -963,8 +967,11 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         int64_t lds = G * dp + std::max(4 * nt * gc * dp, 16 * dp) + 4 * nt * G * 2 + G * 2 + (many ? G * SLM_PG_KEYS : 0) +
                       (a.direct && a.mass_out ? G * SLM_PG_KEYS : 4);
         out.push_back(mk_desc(k.pattn[half][nti][many ? 4 : G - 1], (uint32_t)(items * kh), (uint32_t)(256 * nt), (uint32_t)(4 * lds), a));
-        if (!a.direct)
-            out.push_back(mk_desc(k.pjoin, (uint32_t)(n[0] * H + (a.mass_out ? (items * kh + 3) / 4 : 0)), 1024, 0, a));
+        if (!a.direct) {
+            int wide = o.f[1] == PATTEND_LONG, pairs = wide ? 4 : 1;
+            out.push_back(mk_desc(k.pjoin[wide], (uint32_t)(n[0] * H + (a.mass_out ? (items * kh + pairs - 1) / pairs : 0)),
+                                  wide ? 1024 : 256, 0, a));
+        }
         return SLM_OK;
     }
     // p0 k, p1 v, p2 mass out, p3 born out, p4 mass, p5 born; n0 n, n1 keep, n2 kh, n3 page, n4 dh, n5 pages,
@@ -3846,7 +3853,8 @@ int load_kernels(slm_hip* c) {
         hipFunction_t* f;
         const char* n;
     } batch[] = {{&k.pstore[0], "slm_paged_store"},  {&k.pstore[1], "slm_paged_store16"},
-                 {&k.pjoin, "slm_paged_join"},       {&k.pselect, "slm_paged_select"},
+                 {&k.pjoin[0], "slm_paged_join_4"},  {&k.pjoin[1], "slm_paged_join_16"},
+                 {&k.pselect, "slm_paged_select"},
                  {&k.pmove[0], "slm_paged_move16"},  {&k.pmove[1], "slm_paged_move8"},
                  {&k.logprobs[0], "slm_logprobs_4"}, {&k.logprobs[1], "slm_logprobs_16"}};
     auto get_batch = [&](hipFunction_t* f, std::string name) {
@@ -5261,7 +5269,8 @@ int slm_hip_paged_attend(slm_hip* c, slm_seqs* s, const slm_pages* g, float* y, 
     o.n[9] = (int64_t)s->width;
     // scores in powers of two (fp16 mode: the dtype's scalar first, as slm_hip_attend)
     o.f[0] = (float)((double)(c->fp16 ? round16(scale) : scale) * 1.4426950408889634);
-    o.f[1] = direct ? 1.0f : 0.0f;
+    size_t nz = ((size_t)s->max_len + SLM_PG_KEYS - 1) / SLM_PG_KEYS;
+    o.f[1] = direct ? PATTEND_DIRECT : nz <= 256 / (g->dh / 4) ? PATTEND_SHORT : PATTEND_LONG;
     return submit(c, o);
 }
 
