@@ -19,6 +19,8 @@
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8_4 __attribute__((ext_vector_type(8), aligned(8)));  // at a multiple of four
 
 static constexpr float NEG_INF = -__builtin_inff();
 
@@ -226,10 +228,17 @@ __device__ __forceinline__ float scatter_rows(f4 v) {
 
 // GM: the query heads a key head (1 to 4: exactly, all at once), or 16: any number, four at
 // a time, the weights by way of LDS.
+//
+// fp16 keys go through the matrix unit instead (16x16x32): its products are exact and its sums
+// fp32, so fp32 queries are cut into three fp16 parts (q = q0 + 2^-11 q1 + 2^-22 q2, 33 bits),
+// which are rows of one product: 4·part + head. A score's parts are then in three rows of 16 lanes, and
+// one exchange adds them and hands every lane its key's.
 template <typename T, int NT, int GM>
 __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
-    constexpr int KS = 16 / NT, NW = 4 * NT, DP = 64 * NT, THREADS = 64 * NW;
-    typedef std::conditional_t<sizeof(T) == 2, h4, f4> V4;
+    constexpr int QP = 64 * NT + 8;  // halves from one row of a query part to the next
+    constexpr bool HALF = sizeof(T) == 2;
+    constexpr int KS = HALF ? 16 : 16 / NT, NW = 64 / KS, DP = 64 * NT, THREADS = 64 * NW;
+    typedef std::conditional_t<HALF, h4, f4> V4;
     using std::integral_constant;
     const int item = blockIdx.x / a.kh, h = blockIdx.x % a.kh;
     const uint4 it = ((const uint4*)a.s.items)[item];
@@ -242,49 +251,123 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane >> 4, c = lane & 15;
     const int GC = GM <= 4 || NT < 4 ? G : min(G, 4);  // heads whose values are added up at once
-    float* sq = (float*)lds_;                         // [G][DP]
-    float* so = sq + G * DP;                          // [NW][GC][DP]
+    float* sq = (float*)lds_;                         // [G][DP], or the three parts: [G in fours][12][QP] halves
+    float* so = sq + (HALF ? (G + 3) / 4 * 6 * QP : G * DP);  // [NW][GC][DP]
     float* swm = so + NW * GC * DP;                   // [NW][G][2]
     float* sml = swm + NW * G * 2;                    // [G][2]
     float* sw = sml + G * 2;                          // [NW][G][4 * KS], for GM 16
     float* ss = sw + (GM <= 4 ? 0 : G * SLM_PG_KEYS);  // [G][SLM_PG_KEYS], with direct and mass_out
 
     // this lane's key: the one whose score it will have
-    const int mine = w * (4 * KS) + 4 * (c & (KS - 1)) + r;
+    const int mine = w * (4 * KS) + (HALF ? 16 * r + c : 4 * (c & (KS - 1)) + r);
     const bool some = base + w * (4 * KS) < most;     // the wave has a key to look at
     bool sees = base + mine < most;
-    uint64_t at = 0;                                  // ... and where its row starts, in values
+    uint32_t row = 0;
     if (some) {
-        uint32_t row = row_of(a.s, b, min(base + mine, len - 1), h, a.kh, a.page);
+        row = row_of(a.s, b, min(base + mine, len - 1), h, a.kh, a.page);
         if (a.born && sees) sees = (uint64_t)a.born[row] + (uint64_t)a.gap < a.s.seen[b];
-        at = (uint64_t)row * (uint32_t)dh;
     }
-    for (int i = tid; i < G * DP; i += THREADS) {
-        int g = i / DP, d = i % DP;
-        sq[i] = d < dh ? a.q[((int64_t)b * a.heads + h * G + g) * dh + d] : 0.0f;
+    const uint64_t at = (uint64_t)row * (uint32_t)dh;  // where its row starts, in values
+    // the queries, on their way to LDS
+    constexpr int QN = (DP * (GM <= 4 ? GM : 16) + THREADS - 1) / THREADS;
+    float q[QN];
+#pragma unroll
+    for (int u = 0; u < QN; u++) {
+        int i = tid + u * THREADS, g = i / DP, d = i % DP;
+        q[u] = g < G && d < dh ? a.q[((int64_t)b * a.heads + h * G + g) * dh + d] : 0.0f;
     }
-    // keys and values: the lane's four of every 64 elements of its row of 16's keys (past the head
-    // size: the last four again, made zeros in the keys and of no effect in the values)
-    V4 k[KS][NT], v[KS][NT];
-    auto load = [&](const void* from, V4 (&to)[KS][NT]) {
+    // values: the lane's four of every 64 elements of its row of 16's keys (past the head size: the
+    // last four again, of no effect)
+    V4 v[KS][NT];
+    auto load_rows = [&](const void* from, V4 (&to)[KS][NT]) {
         each<KS>([&](auto j) {
             uint64_t o = (uint64_t)bcast<j>((uint32_t)(at >> 32)) << 32 | bcast<j>((uint32_t)at);
 #pragma unroll
             for (int i = 0; i < NT; i++) to[j][i] = *(const V4*)((const T*)from + o + min(64 * i + 4 * c, dh - 4));
         });
     };
+    // keys: fp32 like the values; fp16 as the matrix unit takes them, 16 keys a tile, a lane eight of
+    // every 32 elements of key c
+    constexpr int NK = HALF ? 2 * NT : NT;
+    std::conditional_t<HALF, h8, f4> k[HALF ? 4 : KS][NK];
+    auto k_start = [&](int i) { return max(0, min(32 * i + 8 * r, dh - 8)); };
     if (some) {
-        load(a.k, k);
-        if (NT < 4) load(a.v, v);  // (sixteen waves have room for one of the two in registers)
+        if constexpr (HALF) {
+            // the four tiles' rows, from the lanes that have them
+            auto p = __builtin_amdgcn_permlane16_swap(row, row, false, false);
+            auto even = __builtin_amdgcn_permlane32_swap(p[0], p[0], false, false);
+            auto odd = __builtin_amdgcn_permlane32_swap(p[1], p[1], false, false);
+            const uint32_t rows[4] = {even[0], odd[0], even[1], odd[1]};
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const T* from = (const T*)a.k + (uint64_t)rows[t] * (uint32_t)dh;
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+                    if (dh >= 8) {
+                        k[t][i] = *(const h8_4*)(from + k_start(i));
+                    } else {
+                        h4 x = *(const h4*)from;
+                        k[t][i] = h8{x.x, x.y, x.z, x.w, 0, 0, 0, 0};
+                    }
+                }
+            }
+        } else {
+            load_rows(a.k, k);
+        }
+        if (NT < 4) load_rows(a.v, v);  // (the largest heads have room for one of the two in registers)
+    }
+    float q_shift = 1.0f;
+    if constexpr (HALF) {
+        __shared__ uint32_t q_max;
+        if (tid == 0) q_max = 0;
+        lds_barrier();
+        float m = 0.0f;
+#pragma unroll
+        for (int u = 0; u < QN; u++) m = fmaxf(m, fabsf(q[u]));
+        m = wave_max(m);
+        if (lane == 0) atomicMax(&q_max, __float_as_uint(m));
+        lds_barrier();
+        // (queries past 2^14 come down to it, by a power of two that the scores get back)
+        const int e = max(0, (int)(q_max >> 23) - 127 - 13);
+        const float down = ldexpf(1.0f, -e);
+        q_shift = ldexpf(1.0f, e);
+#pragma unroll
+        for (int u = 0; u < QN; u++) {
+            int i = tid + u * THREADS, g = i / DP, d = i % DP;
+            if (g >= G) continue;
+            _Float16* to = (_Float16*)sq + ((g >> 2) * 12 + (g & 3)) * QP + d;
+            float x = q[u] * down;
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                _Float16 part = (_Float16)x;
+                to[4 * k * QP] = part;
+                x = (x - (float)part) * 2048.0f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < QN; u++)
+            if (tid + u * THREADS < G * DP) sq[tid + u * THREADS] = q[u];
     }
     const bool all = __ballot(sees) == ~0ull, any = __ballot(sees) != 0;
     lds_barrier();
-    if (dh < DP && some)
+    // what lies past the head size becomes zeros (of fp16 keys, what another lane has already)
+    if (dh < DP && some) {
 #pragma unroll
-        for (int i = 0; i < NT; i++)
-            if (64 * i + 4 * c >= dh)
+        for (int i = 0; i < NK; i++) {
+            if constexpr (HALF) {
+                const int twice = 32 * i + 8 * r - k_start(i);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (twice >= 8 || e < twice) k[t][i][e] = 0;
+            } else if (64 * i + 4 * c >= dh) {
 #pragma unroll
                 for (int j = 0; j < KS; j++) k[j][i] = V4{};
+            }
+        }
+    }
 
     float p[GM <= 4 ? GM : 1];
     float* sp = sw + w * G * (4 * KS) + r * KS + (c & (KS - 1));
@@ -292,23 +375,56 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
         constexpr int GX = decltype(gx)::value;
         float x[GX], m[GX], l[GX];
 #pragma unroll
-        for (int g = 0; g < GX; g++) {
-            x[g] = NEG_INF;
-            if (!some) continue;
-            float s[KS];
+        for (int g = 0; g < GX; g++) x[g] = NEG_INF;
+        if (some) {
+            if constexpr (HALF) {
+                const _Float16* rows = (const _Float16*)sq + ((g0 >> 2) * 12 + (c < 12 ? c : c - 12)) * QP;
+                f4 acc[4] = {};
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                f4 q = *(const f4*)(sq + (g0 + g) * DP + 64 * i + 4 * c);
+                for (int i = 0; i < NK; i++) {
+                    h8 q = *(const h8_4*)(rows + k_start(i));
 #pragma unroll
-                for (int j = 0; j < KS; j++) {
-                    s[j] = i ? fmaf(q.x, (float)k[j][i].x, s[j]) : q.x * (float)k[j][i].x;
-                    s[j] = fmaf(q.y, (float)k[j][i].y, s[j]);
-                    s[j] = fmaf(q.z, (float)k[j][i].z, s[j]);
-                    s[j] = fmaf(q.w, (float)k[j][i].w, s[j]);
+                    for (int t = 0; t < 4; t++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q, k[t][i], acc[t], 0, 0, 0);
+                }
+                // row r has the queries' part r: part 1 is in 2^-11ths, part 2 in 2^-22ths, there is no part 3
+                const float unit = r == 0 ? 1.0f : r == 1 ? 0x1p-11f : r == 2 ? 0x1p-22f : 0.0f;
+#pragma unroll
+                for (int g = 0; g < GX; g++) {
+                    x[g] = scatter_rows(f4{acc[0][g] * unit, acc[1][g] * unit, acc[2][g] * unit, acc[3][g] * unit});
+                    if (__ballot(!(fabsf(x[g]) <= FLT_MAX))) {
+                        // an infinite or NaN key: part 0 alone says what it does (the others' zeros
+                        // would make NaNs of infinities)
+                        f4 z;
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            float y = acc[t][g] * unit;
+                            z[t] = r == 0 || fabsf(y) <= FLT_MAX ? y : 0.0f;
+                        }
+                        x[g] = scatter_rows(z);
+                    }
+                    x[g] = x[g] * q_shift * a.scale;
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < GX; g++) {
+                    float s[KS];
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        f4 q = *(const f4*)(sq + (g0 + g) * DP + 64 * i + 4 * c);
+#pragma unroll
+                        for (int j = 0; j < KS; j++) {
+                            s[j] = i ? fmaf(q.x, k[j][i].x, s[j]) : q.x * k[j][i].x;
+                            s[j] = fmaf(q.y, k[j][i].y, s[j]);
+                            s[j] = fmaf(q.z, k[j][i].z, s[j]);
+                            s[j] = fmaf(q.w, k[j][i].w, s[j]);
+                        }
+                    }
+                    x[g] = scatter_sum<KS>(s, c) * a.scale;
                 }
             }
-            x[g] = scatter_sum<KS>(s, c) * a.scale;
-            if (!sees) x[g] = NEG_INF;
+#pragma unroll
+            for (int g = 0; g < GX; g++)
+                if (!sees) x[g] = NEG_INF;
         }
 #pragma unroll
         for (int g = 0; g < GX; g++) {
@@ -351,7 +467,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 #pragma unroll
             for (int i = 0; i < NT; i++) so[(w * GC + slot + g) * DP + 64 * i + 4 * c + r] = scatter_rows(o[g][i]);
     };
-    constexpr int GS = NT == 4 ? 1 : 4;  // (sixteen waves: a head at a time, for the registers)
+    constexpr int GS = NT == 4 && !HALF ? 1 : 4;  // (sixteen waves: a head at a time, for the registers)
     auto some_heads = [&](int n, auto f) {  // f(heads) for n of them, up to GS
         if constexpr (GS == 4) {
             if (n >= 4) return f(integral_constant<int, 4>());
@@ -371,7 +487,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                 for (int g = 0; g < decltype(gx)::value; g++) sp[(g0 + g) * (4 * KS)] = e[g];
             });
     }
-    if (NT == 4 && some) load(a.v, v);
+    if (NT == 4 && some) load_rows(a.v, v);
     if (some && !all) {  // what is not seen may hold anything
         uint32_t seen = sees;
         each<KS>([&](auto j) {
@@ -435,7 +551,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 }
 
 #define PAGED_ATTN(name, T, NT, GM) \
-    KERNEL void __launch_bounds__(256 * NT) name(PAttnArgs a) { attn_body<T, NT, GM>(a); }
+    KERNEL void __launch_bounds__(sizeof(T) == 2 ? 256 : 256 * NT) name(PAttnArgs a) { attn_body<T, NT, GM>(a); }
 #define PAGED_ATTNS(name, T, NT)       \
     PAGED_ATTN(name##_1, T, NT, 1)     \
     PAGED_ATTN(name##_2, T, NT, 2)     \

@@ -962,11 +962,13 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
             if (a.mass_out) a.sc = a.po + items * H * n[4];
         }
         int nti = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
-        bool many = G > 4 || nti == 2;  // (sixteen waves have no registers for the weights)
-        int64_t nt = 1 << nti, dp = 64 * nt, gc = nt == 4 ? std::min<int64_t>(G, 4) : G;
-        int64_t lds = G * dp + std::max(4 * nt * gc * dp, 16 * dp) + 4 * nt * G * 2 + G * 2 + (many ? G * SLM_PG_KEYS : 0) +
-                      (a.direct && a.mass_out ? G * SLM_PG_KEYS : 4);
-        out.push_back(mk_desc(k.pattn[half][nti][many ? 4 : G - 1], (uint32_t)(items * kh), (uint32_t)(256 * nt), (uint32_t)(4 * lds), a));
+        bool many = G > 4 || nti == 2;
+        // (LDS: the queries or their parts; the waves' values, maxima and sums; all of theirs; the
+        // weights where they are not in registers; the scores where they go no further)
+        int64_t nt = 1 << nti, dp = 64 * nt, gc = nt == 4 ? std::min<int64_t>(G, 4) : G, nw = half ? 4 : 4 * nt;
+        int64_t lds = (half ? (G + 3) / 4 * 6 * (dp + 8) : G * dp) + nw * gc * dp + nw * G * 2 + G * 2 +
+                      (many ? G * SLM_PG_KEYS : 0) + (a.direct && a.mass_out ? G * SLM_PG_KEYS : 0);
+        out.push_back(mk_desc(k.pattn[half][nti][many ? 4 : G - 1], (uint32_t)(items * kh), (uint32_t)(64 * nw), (uint32_t)(4 * lds), a));
         if (!a.direct) {
             int wide = o.f[1] == PATTEND_LONG, pairs = wide ? 4 : 1;
             out.push_back(mk_desc(k.pjoin[wide], (uint32_t)(n[0] * H + (a.mass_out ? (items * kh + pairs - 1) / pairs : 0)),

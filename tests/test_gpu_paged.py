@@ -21,8 +21,9 @@ def rng_of(*key):
 
 
 def check(got, want, bound, what=""):
-    err = np.abs(got.astype(np.float64) - want)
-    bad = ~(err <= bound)
+    with np.errstate(invalid="ignore"):
+        err = np.abs(got.astype(np.float64) - want)
+    bad = np.where(np.isfinite(want), ~(err <= bound), ~((got == want) | (np.isnan(got) & np.isnan(want))))
     assert not bad.any(), (what, np.argwhere(bad)[:4], err[bad][:4], np.broadcast_to(bound, err.shape)[bad][:4])
 
 
@@ -119,12 +120,14 @@ def test_same_bits_in_any_batch(hip, pkg, half):
         assert np.array_equal(m1[p1, :, s1], mass[p0, :, s0])
 
 
-def test_infinities_and_nan_in_visible_keys(hip, pkg):
+@pytest.mark.parametrize("half", [False, True])
+def test_infinities_and_nan_in_visible_keys(hip, pkg, half):
     """Where the formula takes them: a NaN key, infinite scores of both signs (all of them, one
     superblock's, one key's), infinite values under weight and under none."""
     lens = [600] * 7
-    c = Cache(rng_of(4), lens, 1, 16, 16)
+    c = Cache(rng_of(4), lens, 1, 16, 16, half)
     q = np.abs(rng_of(5).standard_normal((7, 2, 16))).astype(np.float32) + 0.1
+    q[2] = q[2].astype(np.float16)  # (fp16 mode's queries: what is past fp16 in them is zero)
     at = [c.where(b) for b in range(7)]
     c.k[at[0][0][400], 0, at[0][1][400]] = np.nan
     c.k[at[1][0], 0, at[1][1]] = -np.inf                          # every score -inf
@@ -141,6 +144,21 @@ def test_infinities_and_nan_in_visible_keys(hip, pkg):
     assert np.all(np.isnan(y[0])) and np.all(np.isnan(y[1])) and np.all(np.isfinite(y[2]))
     check(y[[2, 6]], want[[2, 6]], bound[[2, 6]])
     assert fine[4].sum() == 2 * 15
+
+
+@pytest.mark.parametrize("qs,ks,scale", [(1e-6, 1.0, 3e5), (3e6, 1.0, 1e-6), (1e30, 1.0, 1e-30), (1.0, 2e-7, 1e6),
+                                         (1.0, 2e4, 2e-5), (1.0, 1e4, 4e-5), (1e-9, 1e-6, 1e15), (0.0, 1.0, 1.0)])
+def test_fp16_keys_and_queries_of_any_size(hip, pkg, qs, ks, scale):
+    """fp32 queries over fp16 keys: small ones, past fp16's range, keys below its normal numbers and at
+    its largest (some of them infinite once rounded)."""
+    c = Cache(rng_of(17), [300, 90], 2, 64, 16, True, scale=1.0)
+    c.k = c.values(c.k * ks)
+    q = (rng_of(18).standard_normal((2, 12, 64)) * qs).astype(np.float32)
+    q[..., ::7] *= np.float32(1e-4)
+    y, mass = attend(hip, pkg, c, q, scale=scale)
+    want, wmass, bound, mbound = c.attend(q, np.float64(np.float32(scale)), born=False)
+    check(y, want, bound)
+    check(mass[c.used()], wmass[c.used()], mbound[c.used()])
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
