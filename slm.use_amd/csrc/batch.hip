@@ -388,12 +388,17 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                 }
                 // row r has the queries' part r: part 1 is in 2^-11ths, part 2 in 2^-22ths, there is no part 3
                 const float unit = r == 0 ? 1.0f : r == 1 ? 0x1p-11f : r == 2 ? 0x1p-22f : 0.0f;
+                bool fine = true;
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
                     x[g] = scatter_rows(f4{acc[0][g] * unit, acc[1][g] * unit, acc[2][g] * unit, acc[3][g] * unit});
-                    if (__ballot(!(fabsf(x[g]) <= FLT_MAX))) {
-                        // an infinite or NaN key: part 0 alone says what it does (the others' zeros
-                        // would make NaNs of infinities)
+                    fine = fine && fabsf(x[g]) <= FLT_MAX;
+                }
+                if (__ballot(!fine)) {
+                    // an infinite or NaN key: part 0 alone says what it does (the others' zeros would
+                    // make NaNs of infinities)
+#pragma unroll
+                    for (int g = 0; g < GX; g++) {
                         f4 z;
 #pragma unroll
                         for (int t = 0; t < 4; t++) {
@@ -402,8 +407,9 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                         }
                         x[g] = scatter_rows(z);
                     }
-                    x[g] = x[g] * q_shift * a.scale;
                 }
+#pragma unroll
+                for (int g = 0; g < GX; g++) x[g] = x[g] * q_shift * a.scale;
             } else {
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
@@ -511,28 +517,37 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                 });
         }
         lds_barrier();
-        // the superblock's, from its waves' in order
-        for (int i = tid; i < ng * DP; i += THREADS) {
-            int g = i / DP, d = i % DP, gg = c0 + g;
+        // the superblock's, from its waves' in order: four elements a thread
+        for (int i = tid; i < ng * (DP / 4); i += THREADS) {
+            int g = i / (DP / 4), d = i % (DP / 4) * 4, gg = c0 + g;
             if (d >= dh) continue;
-            float m = NEG_INF, l = 0.0f, o = 0.0f;
+            float m = NEG_INF, l = 0.0f;
+            float2 ml[NW];
+            f4 o = {0, 0, 0, 0};
 #pragma unroll
-            for (int k2 = 0; k2 < NW; k2++) m = fmaxf(m, swm[(k2 * G + gg) * 2]);
-            float ms = m == NEG_INF ? 0.0f : m;
+            for (int k2 = 0; k2 < NW; k2++) ml[k2] = *(const float2*)(swm + (k2 * G + gg) * 2);
+#pragma unroll
+            for (int k2 = 0; k2 < NW; k2++) m = fmaxf(m, ml[k2].x);
+            const float ms = m == NEG_INF ? 0.0f : m;
 #pragma unroll
             for (int k2 = 0; k2 < NW; k2++) {
-                float2 ml = *(const float2*)(swm + (k2 * G + gg) * 2);
-                float f = __builtin_amdgcn_exp2f(ml.x - ms);
-                l = fmaf(ml.y, f, l);
-                o = fmaf(so[(k2 * GC + g) * DP + d], f, o);
+                float f = __builtin_amdgcn_exp2f(ml[k2].x - ms);
+                f4 z = *(const f4*)(so + (k2 * GC + g) * DP + d);
+                l = fmaf(ml[k2].y, f, l);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], f, o[e]);
             }
+            const int head = h * G + gg;
             if (a.direct) {
-                float y = m == NEG_INF ? 0.0f : o / l;
-                a.y[((int64_t)b * a.heads + h * G + gg) * dh + d] = a.r16 ? r16(y) : y;
+                float* y = a.y + ((int64_t)b * a.heads + head) * dh + d;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float z = m == NEG_INF ? 0.0f : o[e] / l;
+                    y[e] = a.r16 ? r16(z) : z;
+                }
                 if (d == 0) *(float2*)(sml + 2 * gg) = make_float2(m, l);
             } else {
-                const int head = h * G + gg;
-                a.po[((int64_t)item * a.heads + head) * dh + d] = o;
+                *(f4*)(a.po + ((int64_t)item * a.heads + head) * dh + d) = o;
                 if (d == 0) *(float2*)(a.ml + 2 * ((int64_t)head * a.items + item)) = make_float2(m, l);
             }
         }

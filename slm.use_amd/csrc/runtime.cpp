@@ -896,8 +896,9 @@ SeqsDev seqs_dev(const slm_seqs* s, int64_t n, int64_t width) {
 constexpr float PATTEND_DIRECT = 0.0f, PATTEND_SHORT = 1.0f, PATTEND_LONG = 2.0f;
 
 // Bytes of the workspace that a paged attention of `items` superblocks uses.
+size_t pattend_ml(size_t items, size_t heads) { return (2 * items * heads + 3) & ~(size_t)3; }  // (whole 16 bytes)
 size_t pattend_bytes(size_t items, size_t heads, size_t dh, bool mass) {
-    return items * heads * (2 + dh + (mass ? SLM_PG_KEYS : 0)) * 4;
+    return (pattend_ml(items, heads) + items * heads * (dh + (mass ? SLM_PG_KEYS : 0))) * 4;
 }
 
 int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
@@ -958,7 +959,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         const int64_t items = n[7], H = n[1], kh = n[2], G = H / kh;
         if (!a.direct) {
             a.ml = c->pws;
-            a.po = a.ml + 2 * items * H;
+            a.po = a.ml + pattend_ml(items, H);
             if (a.mass_out) a.sc = a.po + items * H * n[4];
         }
         int nti = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
