@@ -685,11 +685,6 @@ __device__ __forceinline__ uint32_t mass_key(float m, uint32_t born, uint32_t re
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {  // the same in every lane: to a scalar
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
-           (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
-}
-
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_or0(uint32_t x) {  // 0 where the lane has no such neighbour
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true);
@@ -852,36 +847,40 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
             if (tid < words) counts[tid] = before;
             __syncthreads();
         }
-#pragma unroll 4
+        // (the compute unit's sixteen waves share one scalar unit: what can be a lane's work is)
+#pragma unroll 2
         for (uint32_t q = w; q < words; q += 16) {
-            const bool in = 64 * q + lane < len;
-            uint32_t k = keys[min(64 * q + lane, len - 1)] >> shift;
-            uint64_t m = __ballot(in && k >= prefix);
+            const uint32_t t = 64 * q + lane, k = keys[min(t, len - 1)] >> shift;
+            uint64_t m = __ballot(k >= prefix);
             if (ties) {
-                uint64_t em = __ballot(in && k == prefix);
-                m = __ballot(in && (k > prefix || (k == prefix && counts[q] + lanes_below(em) < need)));
+                uint64_t em = __ballot(k == prefix && t < len);
+                m = __ballot(k > prefix || (k == prefix && counts[q] + lanes_below(em) < need));
             }
             if (lane == 0) stays[q] = m;
         }
         __syncthreads();
-        // holes below, movers above: both counts in one word (neither passes 2^16)
-        uint32_t both = 0;
+        // a thread a word: holes below, movers above, both counts in one word (neither passes 2^16)
+        ulonglong2* both = (ulonglong2*)keys;  // (the keys have done their work)
+        uint32_t n = 0;
         if (tid < words) {
-            uint64_t m = stays[tid], f = front(64 * tid);
-            both = __popcll(~m & f & there(64 * tid)) | __popcll(m & ~f) << 16;
+            uint64_t in = there(64 * tid), m = stays[tid] & in, f = front(64 * tid);
+            both[tid] = make_ulonglong2(~m & f & in, m & ~f);
+            n = __popcll(~m & f & in) | __popcll(m & ~f) << 16;
         }
-        uint32_t before = block_scan(both, red[4]);
+        uint32_t before = block_scan(n, red[4]);
         if (tid < words) counts[tid] = before;
-        if (tid == words - 1) pick[0][0] = (before + both) >> 16;
+        if (tid == words - 1) pick[0][0] = (before + n) >> 16;
         __syncthreads();
         moves = pick[0][0];
         auto write = [&](auto* to, auto* from) {
-#pragma unroll 4
+#pragma unroll 2
             for (uint32_t q = w; q < words; q += 16) {
-                uint64_t m = uniform(stays[q]), f = front(64 * q), hm = ~m & f & there(64 * q), mm = m & ~f;
-                uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane(counts[q]);
-                if (__builtin_amdgcn_inverse_ballot_w64(hm)) to[(n & 0xffff) + lanes_below(hm)] = 64 * q + lane;
-                if (__builtin_amdgcn_inverse_ballot_w64(mm)) from[(n >> 16) + lanes_below(mm)] = 64 * q + lane;
+                const ulonglong2 m = both[q];
+                const uint32_t c = counts[q];
+                const uint32_t hole = (uint32_t)(lane < 32 ? m.x : m.x >> 32) >> (lane & 31) & 1;
+                const uint32_t mover = (uint32_t)(lane < 32 ? m.y : m.y >> 32) >> (lane & 31) & 1;
+                if (hole) to[(c & 0xffff) + lanes_below(m.x)] = 64 * q + lane;
+                if (mover) from[(c >> 16) + lanes_below(m.y)] = 64 * q + lane;
             }
         };
         if (a.count) write((GLOBAL_MEM uint32_t*)list, (GLOBAL_MEM uint32_t*)(list + a.most));
