@@ -82,6 +82,9 @@ struct LogpArgs {
     float* top_lp;
     int64_t m, n;
     int32_t top;
+    int32_t parts, span;     // workgroups of a row, and the logits of each
+    float* part_sums;        // [m][parts][4]
+    uint64_t* part_top;      // [m][parts][top], best first
     uint32_t few[SLM_FEW_IDS];  // up to this many rows' tokens, outside a recorded step
 };
 

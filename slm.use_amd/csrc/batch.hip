@@ -1027,25 +1027,31 @@ __device__ __forceinline__ float logit_of(uint32_t key) {  // (a number, not a N
 // Part of a row's sums: its maximum m, the count c of logits equal to it, and over the others
 // S = sum e^(x-m) and E = sum e^(x-m) (x-m); so log L = log c + log1p(S / c) keeps its digits
 // where one token has nearly all the probability. A NaN is in S.
-struct RowSum {
-    float m, c, S, E;
+template <typename C>
+struct Sums {
+    float m;
+    C c;
+    float S, E;
     __device__ __forceinline__ void raise(float to) {  // the same sum about a maximum `to` >= m
         if (!(to > m)) return;
         if (m > NEG_INF) {
-            float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f), all = c + S;
+            float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f), all = (float)c + S;
             E = f * fmaf(fmaxf(d, -1e4f), all, E);
             S = f * all;
         }
-        c = 0.0f;
+        c = 0;
         m = to;
     }
     __device__ __forceinline__ void add(float x) {  // x <= m, or a NaN; m > -inf
         float d = x - m, e = __builtin_amdgcn_exp2f(d * 1.44269504f);
-        S += x == m ? 0.0f : e;
-        c += x == m ? 1.0f : 0.0f;
+        const bool top = x == m;
+        S += top ? 0.0f : e;
+        c += top;
         E = fmaf(e, fmaxf(d, -1e4f), E);  // (e^-1e4 is 0: an impossible token adds nothing)
     }
 };
+typedef Sums<uint32_t> LaneSum;
+typedef Sums<float> RowSum;
 
 // The largest t (to 16 bits: a bound is all it is for) such that at least `want` of the wave's 64
 // keys are >= t: by its bits from above, a ballot each; two wants at once.
@@ -1067,19 +1073,24 @@ __device__ __forceinline__ void wave_nth(uint32_t key, int want0, int want1, uin
 // wave's list, which is cut to its `top` best when more than 64 are in it (T rises with it);
 // about 5·top of a row of 32000 reach T. Of what the lists hold at the end, those that reach a
 // second bound of the same kind are ranked by counting the better ones.
-template <int W>
+//
+// With SPLIT a row goes to `parts` workgroups, which leave their sums and alternatives to
+// slm_logprobs_join.
+template <int W, bool SPLIT>
 __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     __shared__ uint64_t list[W][128], fin[W * 64];
     __shared__ uint32_t cnts[W], bound[W][2], nfin;
     __shared__ __attribute__((aligned(16))) float sums[W][4];
-    const int64_t row = blockIdx.x;
+    const int part = SPLIT ? blockIdx.x % a.parts : 0;
+    const int64_t row = SPLIT ? blockIdx.x / a.parts : blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.top;
     const float* x = a.x + row * a.n;
     // whole 16 bytes from the last such address at or before the row's first logit
     const int a0 = (int)(((uintptr_t)x >> 2) & 3), end = (int)a.n + a0;
     const float* xa = x - a0;
     const int fair = (top + W - 1) / W;
-    const float given = x[a.ids ? a.ids[row] : a.few[row]];
+    const float given = SPLIT ? 0.0f : x[a.ids ? a.ids[row] : a.few[row]];
+    const int begin = SPLIT ? part * a.span : 0, stop = SPLIT ? min(end, begin + a.span) : end;
     if (tid == 0) nfin = 0;
 
     auto threshold = [&](uint32_t key) -> uint32_t {
@@ -1100,7 +1111,7 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
         return max(most, least);
     };
 
-    RowSum s{NEG_INF, 0.0f, 0.0f, 0.0f};
+    LaneSum mine{NEG_INF, 0, 0.0f, 0.0f};
     uint64_t least = 0;  // what a logit's rank must pass to be listed
     float least_x = NEG_INF;
     int cnt = 0;
@@ -1127,7 +1138,7 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
         }
     };
 
-    for (int p0 = 0; p0 < end; p0 += W * 2048) {
+    for (int p0 = begin; p0 < stop; p0 += W * 2048) {
         f4 v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -1141,21 +1152,26 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
         }
         float m = NEG_INF;
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(fmaxf(m, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
-        s.raise(m);
-        if (s.m > NEG_INF) {
+        for (int j0 = 0; j0 < 8; j0 += 4) {  // (the first half while the second is on its way)
+            float m4 = NEG_INF;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+            for (int j = j0; j < j0 + 4; j++) m4 = fmaxf(fmaxf(m4, fmaxf(v[j].x, v[j].y)), fmaxf(v[j].z, v[j].w));
+            m = fmaxf(m, m4);
+            mine.raise(m4);
+            if (mine.m > NEG_INF) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) s.add(v[j][e]);
-        } else {
+                for (int j = j0; j < j0 + 4; j++)
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+                    for (int e = 0; e < 4; e++) mine.add(v[j][e]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) s.S += v[j][e] == NEG_INF ? 0.0f : v[j][e];  // (a NaN)
+                for (int j = j0; j < j0 + 4; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mine.S += v[j][e] == NEG_INF ? 0.0f : v[j][e];  // (a NaN)
+            }
         }
         if (top) {
-            if (p0 == 0) {
+            if (p0 == begin) {
                 // (a lane of nothing but NaNs and -infinities bounds nothing)
                 uint32_t t = threshold(m > NEG_INF ? logit_key(m) : 0);
                 least = t ? ((uint64_t)t << 32) - 1 : 0;
@@ -1169,6 +1185,7 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
                     int at = p0 + ((j >> 2) * W + w) * 1024 + (j & 3) * 256 + lane * 4 - a0;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
+                        if (!__ballot(!(v[j][e] < least_x))) continue;
                         uint64_t r = (uint64_t)logit_key(v[j][e]) << 32 | (0xffffffffu - (uint32_t)(at + e));
                         bool in = at + e >= 0 && at + e < (int)a.n && r > least;
                         uint64_t mask = __ballot(in);
@@ -1185,6 +1202,7 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     }
 
     // the row's sums: the wave's, then the waves' (a lane of each row of 16 for each)
+    RowSum s{mine.m, (float)mine.c, mine.S, mine.E};
     float m = wave_max(s.m);
     s.raise(m);
     s.c = wave_sum(s.c);
@@ -1210,12 +1228,14 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     total = (int)row_sum((float)total);
     // no logit above -inf (and no NaN): no token is possible
     const bool none = m == NEG_INF && s.S == 0.0f;
-    auto logp = [&](float x) { return none ? NEG_INF : (x - m) - (logf(s.c) + log1pf(s.S / s.c)); };
-    if (w == 0) {
-        float l = logp(given);
+    auto log_sum = [&] { return logf(s.c) + log1pf(s.S / s.c); };
+    if (SPLIT) {
+        if (tid == 0) *(f4*)(a.part_sums + 4 * (row * a.parts + part)) = f4{m, s.c, s.S, s.E};
+    } else if (w == 0) {
+        const float logl = log_sum();
         if (lane == 0) {
-            a.lp[row] = l;
-            if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + (logf(s.c) + log1pf(s.S / s.c)) - s.E / (s.c + s.S);
+            a.lp[row] = none ? NEG_INF : (given - m) - logl;
+            if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - s.E / (s.c + s.S);
         }
     }
     if (!top) return;
@@ -1233,16 +1253,85 @@ __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     }
     __syncthreads();
     const int n = nfin;
+    uint64_t* listed = SPLIT ? a.part_top + (row * a.parts + part) * top : nullptr;
+    if (SPLIT && tid >= n && tid < top) listed[tid] = 0;  // (a part of fewer logits)
     if (64 * w >= n) return;
     e = tid < n ? fin[tid] : 0;
     int r = 0;
 #pragma unroll 8
     for (int i = 0; i < n; i++) r += fin[i] > e;
-    if (tid < n && r < top) {
+    if (SPLIT) {
+        if (tid < n && r < top) listed[r] = e;
+    } else if (tid < n && r < top) {
         uint32_t key = (uint32_t)(e >> 32), id = 0xffffffffu - (uint32_t)e;
         a.top_ids[row * top + r] = id;
-        a.top_lp[row * top + r] = logp(key ? logit_of(key) : __builtin_nanf(""));
+        a.top_lp[row * top + r] = none ? NEG_INF : ((key ? logit_of(key) : __builtin_nanf("")) - m) - log_sum();
     }
 }
-KERNEL void __launch_bounds__(256) slm_logprobs_4(LogpArgs a) { logprobs_body<4>(a); }
-KERNEL void __launch_bounds__(1024) slm_logprobs_16(LogpArgs a) { logprobs_body<16>(a); }
+KERNEL void __launch_bounds__(256) slm_logprobs_4(LogpArgs a) { logprobs_body<4, false>(a); }
+KERNEL void __launch_bounds__(1024) slm_logprobs_16(LogpArgs a) { logprobs_body<16, false>(a); }
+KERNEL void __launch_bounds__(256) slm_logprobs_split(LogpArgs a) { logprobs_body<4, true>(a); }
+
+// A row's parts (at most 64) together: a workgroup a row. Of the parts' alternatives only those
+// that reach the best part's last one can be among the row's.
+KERNEL void __launch_bounds__(256) slm_logprobs_join(LogpArgs a) {
+    __shared__ uint64_t fin[64 * SLM_TOP_MAX];
+    __shared__ uint32_t nfin;
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, top = a.top, parts = a.parts;
+    const float* x = a.x + row * a.n;
+    const float given = x[a.ids ? a.ids[row] : a.few[row]];
+    if (tid == 0) nfin = 0;
+    RowSum s{NEG_INF, 0.0f, 0.0f, 0.0f};
+    if (lane < parts) {
+        f4 q = *(const f4*)(a.part_sums + 4 * (row * parts + lane));
+        s = RowSum{q.x, q.y, q.z, q.w};
+    }
+    const uint64_t* listed = a.part_top + row * parts * top;
+    uint64_t e[64 * SLM_TOP_MAX / 256], last = 0;
+    if (top) {
+        if (lane < parts) last = listed[lane * top + top - 1];
+#pragma unroll
+        for (int u = 0; u < 64 * SLM_TOP_MAX / 256; u++) e[u] = tid + 256 * u < parts * top ? listed[tid + 256 * u] : 0;
+    }
+    const float m = wave_max(s.m);
+    s.raise(m);
+    s.c = wave_sum(s.c);
+    s.S = wave_sum(s.S);
+    s.E = wave_sum(s.E);
+    const bool none = m == NEG_INF && s.S == 0.0f;
+    const float logl = logf(s.c) + log1pf(s.S / s.c);
+    if (tid == 0) {
+        a.lp[row] = none ? NEG_INF : (given - m) - logl;
+        if (a.ent) a.ent[row] = none ? 0.0f : (m - m) + logl - s.E / (s.c + s.S);
+    }
+    if (!top) return;
+    for (int o = 32; o; o >>= 1) {
+        uint64_t v = (uint64_t)__shfl_xor((unsigned long long)last, o);
+        if (v > last) last = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 64 * SLM_TOP_MAX / 256; u++) {
+        if (256 * u >= parts * top) break;
+        const bool in = e[u] != 0 && e[u] >= last;
+        uint64_t mask = __ballot(in);
+        uint32_t at = 0;
+        if (lane == 0 && mask) at = atomicAdd(&nfin, (uint32_t)__popcll(mask));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane(at) + lanes_below(mask);
+        if (in) fin[at] = e[u];
+    }
+    __syncthreads();
+    const int n = nfin;
+    for (int i = tid; i < n; i += 256) {
+        const uint64_t mine = fin[i];
+        int r = 0;
+#pragma unroll 8
+        for (int k = 0; k < n; k++) r += fin[k] > mine;
+        if (r < top) {
+            uint32_t key = (uint32_t)(mine >> 32), id = 0xffffffffu - (uint32_t)mine;
+            a.top_ids[row * top + r] = id;
+            a.top_lp[row * top + r] = none ? NEG_INF : ((key ? logit_of(key) : __builtin_nanf("")) - m) - logl;
+        }
+    }
+}

@@ -154,7 +154,7 @@ struct Kernels {
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
-    hipFunction_t pstore[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2];
+    hipFunction_t pstore[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
 };
 
 }  // namespace
@@ -901,6 +901,23 @@ size_t pattend_bytes(size_t items, size_t heads, size_t dh, bool mass) {
     return (pattend_ml(items, heads) + items * heads * (dh + (mass ? SLM_PG_KEYS : 0))) * 4;
 }
 
+// Workgroups that a row of n logits is split over while the rows are few: four-wave ones, a panel
+// of 8192 logits each, up to 64 (of whole panels); else one of sixteen waves (four for up to
+// 8192 logits). Measured, split against not, 20 alternatives: one row of 32000 11.1 against 11.7 us,
+// 65 rows of 32000 about 13.1 against 14.2, of 65536 16.1 against 18.1; 100 rows of 32000 14.4 against
+// 14.2, of 131072 28.2 against 27.7; 160 rows of 32000 16.0 against 15.6, of 131072 32.5 against 28.9.
+constexpr int64_t LOGP_SHORT = 8192, LOGP_PARTS = 64, LOGP_FEW_ROWS = 64;
+int64_t logp_parts(int64_t m, int64_t n) {
+    if (m > LOGP_FEW_ROWS || n <= LOGP_SHORT) return 1;
+    int64_t panels = (n + 3 + LOGP_SHORT - 1) / LOGP_SHORT;  // (a row may start 3 logits into 16 bytes)
+    int64_t each = (panels + LOGP_PARTS - 1) / LOGP_PARTS;
+    return (panels + each - 1) / each;
+}
+int64_t logp_span(int64_t n, int64_t parts) {
+    int64_t panels = (n + 3 + LOGP_SHORT - 1) / LOGP_SHORT;
+    return (panels + parts - 1) / parts * LOGP_SHORT;
+}
+
 int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const Kernels& k = c->k;
     const float* const* p = o.p;
@@ -917,9 +934,21 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         a.m = n[0];
         a.n = n[1];
         a.top = (int32_t)n[2];
-        bool wide = n[1] > 8192;  // four waves a row, or sixteen
+        double bytes = 4.0 * (double)n[0] * (double)(n[1] + 3 + 2 * n[2]);
+        int64_t parts = logp_parts(n[0], n[1]);
+        if (parts > 1) {
+            a.parts = (int32_t)parts;
+            a.span = (int32_t)logp_span(n[1], parts);
+            a.part_sums = c->pws;
+            a.part_top = (uint64_t*)(c->pws + 4 * n[0] * parts);
+            out.push_back(mk_desc(k.logprobs_split, (uint32_t)(n[0] * parts), 256, 0, a));
+            out.back().abytes = bytes;
+            out.push_back(mk_desc(k.logprobs_join, (uint32_t)n[0], 256, 0, a));
+            return SLM_OK;
+        }
+        bool wide = n[1] > LOGP_SHORT;  // sixteen waves a row, or four
         out.push_back(mk_desc(k.logprobs[wide], (uint32_t)n[0], wide ? 1024 : 256, 0, a));
-        out.back().abytes = 4.0 * (double)n[0] * (double)(n[1] + 3 + 2 * n[2]);
+        out.back().abytes = bytes;
         return SLM_OK;
     }
     if (o.kind != OP_PSTORE && o.kind != OP_PATTEND && o.kind != OP_PEVICT)
@@ -3859,7 +3888,8 @@ int load_kernels(slm_hip* c) {
                  {&k.pjoin[0], "slm_paged_join_4"},  {&k.pjoin[1], "slm_paged_join_16"},
                  {&k.pselect, "slm_paged_select"},
                  {&k.pmove[0], "slm_paged_move16"},  {&k.pmove[1], "slm_paged_move8"},
-                 {&k.logprobs[0], "slm_logprobs_4"}, {&k.logprobs[1], "slm_logprobs_16"}};
+                 {&k.logprobs[0], "slm_logprobs_4"}, {&k.logprobs[1], "slm_logprobs_16"},
+                 {&k.logprobs_split, "slm_logprobs_split"}, {&k.logprobs_join, "slm_logprobs_join"}};
     auto get_batch = [&](hipFunction_t* f, std::string name) {
         hipError_t e = hipModuleGetFunction(f, c->mod_batch, name.c_str());
         if (e != hipSuccess) return fail(c, SLM_E_HIP, "kernel %s: %s", name.c_str(), hipGetErrorString(e));
@@ -5048,8 +5078,8 @@ int slm_hip_seqs_new(slm_hip* c, size_t page, size_t max_n, size_t max_pages, sl
     if (!page || !max_n || !max_pages) return fail(c, SLM_E_INVALID, "seqs_new: a size of 0");
     size_t slots = 0, cells = 0;
     if (max_n > 65536 || __builtin_mul_overflow(page, max_pages, &slots) || slots >= (size_t)1 << 31 ||
-        __builtin_mul_overflow(max_n, max_pages, &cells) || cells > (size_t)1 << 26 ||
-        max_n * ((slots + SLM_PG_KEYS - 1) / SLM_PG_KEYS) > (size_t)1 << 26)
+        __builtin_mul_overflow(max_n, max_pages, &cells) || cells > (size_t)1 << 24 ||
+        max_n * ((slots + SLM_PG_KEYS - 1) / SLM_PG_KEYS) > (size_t)1 << 22)
         return fail(c, SLM_E_UNSUPPORTED, "seqs_new: %zu sequences of %zu pages of %zu slots", max_n, max_pages, page);
     TRY(refuse_capture(c, "seqs_new"));
     slm_seqs* s = new slm_seqs();
@@ -5248,7 +5278,8 @@ int slm_hip_paged_attend(slm_hip* c, slm_seqs* s, const slm_pages* g, float* y, 
         if (s->shared) return fail(c, SLM_E_INVALID, "paged_attend: weights for pages that are in the table twice");
     }
     bool direct = s->max_len <= SLM_PG_KEYS;
-    if (s->items * std::max(heads, (size_t)1) >= (size_t)1 << 31)
+    // (a launch's threads are a 32-bit count)
+    if (heads > 65536 || s->n * heads + s->items * g->key_heads >= (size_t)1 << 22)
         return fail(c, SLM_E_UNSUPPORTED, "paged_attend: %zu superblocks of %zu heads", s->items, heads);
     if (!direct) TRY(need_pws(c, pattend_bytes(s->items, heads, g->dh, mass_out != nullptr)));
     Op o = op(OP_PATTEND);
@@ -5306,7 +5337,7 @@ int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass
     while (step * 8 <= most) step *= 2;
     most = (most + step - 1) / step * step;
     size_t pairs = s->n * g->key_heads;
-    if (pairs >= (size_t)1 << 24 || pairs * ((most + SLM_MOVES_WG - 1) / SLM_MOVES_WG) >= (size_t)1 << 24)
+    if (pairs >= (size_t)1 << 22 || pairs * ((most + SLM_MOVES_WG - 1) / SLM_MOVES_WG) >= (size_t)1 << 24)
         return fail(c, SLM_E_UNSUPPORTED, "paged_evict: %zu sequences of %zu key heads", s->n, g->key_heads);
     if (most > SLM_MOVES_HERE) TRY(need_pws(c, pairs * 4 + pairs * 2 * most * 4));
     Op o = op(OP_PEVICT);
@@ -5367,6 +5398,8 @@ int slm_hip_logprobs(slm_hip* c, float* lp, float* entropy, uint32_t* top_ids, f
     o.n[0] = (int64_t)m;
     o.n[1] = (int64_t)n;
     o.n[2] = (int64_t)top;
+    int64_t parts = logp_parts((int64_t)m, (int64_t)n);
+    if (parts > 1) TRY(need_pws(c, m * (size_t)parts * (16 + 8 * top)));
     // a few tokens go with the launch (a copy of four bytes ahead of it takes longer than it
     // does); in a recorded step they are the step's values
     if (m <= SLM_FEW_IDS && !recording(c)) {
