@@ -18,6 +18,7 @@
 #define KERNEL extern "C" __global__
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8_4 __attribute__((ext_vector_type(8), aligned(8)));  // at a multiple of four
@@ -121,8 +122,7 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 // ---------------------------------------------------------------------------------------
 
 // y_g = sum_t softmax_t(scale · q_g·k_t) v_t for the query heads g of one key head. A workgroup
-// takes one superblock of SLM_PG_KEYS slots, its waves 64 / NT keys each (NT: the head size in
-// 64s); for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
+// takes one superblock of SLM_PG_KEYS slots, its waves 64 keys each (32 of fp32 heads above 64); for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
 // x = (scale · log2 e) q·k over its keys, the workgroup those of the superblock, and
 // slm_paged_join_* adds the superblocks up. No visible key: m = -inf; one at least: m >= -FLT_MAX.
 //
@@ -226,18 +226,21 @@ __device__ __forceinline__ float scatter_rows(f4 v) {
     return add(__builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
 }
 
-// GM: the query heads a key head (1 to 4: exactly, all at once), or 16: any number, four at
-// a time, the weights by way of LDS.
+// GM: the query heads a key head (1 to 4: exactly), or 16: any number, which go through the matrix
+// unit (16x16x4, fp32; the heads are the rows of both products, whatever their number): a score
+// tile is 16 heads by 16 keys, a lane eight or sixteen bytes of every 32 or 16 elements of key c
+// of the tile; the weights go by way of LDS to where a value product wants them, which takes the
+// values as they lie.
 //
-// fp16 keys go through the matrix unit instead (16x16x32): its products are exact and its sums
+// fp16 keys always go through the matrix unit (16x16x32): its products are exact and its sums
 // fp32, so fp32 queries are cut into three fp16 parts (q = q0 + 2^-11 q1 + 2^-22 q2, 33 bits),
 // which are rows of one product: 4·part + head. A score's parts are then in three rows of 16 lanes, and
 // one exchange adds them and hands every lane its key's.
 template <typename T, int NT, int GM>
 __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     constexpr int QP = 64 * NT + 8;  // halves from one row of a query part to the next
-    constexpr bool HALF = sizeof(T) == 2;
-    constexpr int KS = HALF ? 16 : 16 / NT, NW = 64 / KS, DP = 64 * NT, THREADS = 64 * NW;
+    constexpr bool HALF = sizeof(T) == 2, MANY = GM > 4;
+    constexpr int KS = HALF || NT == 1 ? 16 : 8, NW = 64 / KS, DP = 64 * NT, THREADS = 64 * NW;
     typedef std::conditional_t<HALF, h4, f4> V4;
     using std::integral_constant;
     const int item = blockIdx.x / a.kh, h = blockIdx.x % a.kh;
@@ -250,16 +253,17 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     const int G = GM <= 4 ? GM : a.heads / a.kh, dh = a.dh;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane >> 4, c = lane & 15;
-    const int GC = GM <= 4 || NT < 4 ? G : min(G, 4);  // heads whose values are added up at once
-    float* sq = (float*)lds_;                         // [G][DP], or the three parts: [G in fours][12][QP] halves
-    float* so = sq + (HALF ? (G + 3) / 4 * 6 * QP : G * DP);  // [NW][GC][DP]
-    float* swm = so + NW * GC * DP;                   // [NW][G][2]
+    constexpr int QS = MANY ? DP + 4 : DP;            // floats from one query to the next
+    constexpr int CH = MANY ? 64 : DP;                // elements whose values are added up at once
+    float* sq = (float*)lds_;                         // [G][QS], or the three parts: [G in fours][12][QP] halves
+    float* so = sq + (HALF ? (G + 3) / 4 * 6 * QP : G * QS);  // [NW][G][CH]
+    float* swm = so + NW * G * CH;                    // [NW][G][2]
     float* sml = swm + NW * G * 2;                    // [G][2]
-    float* sw = sml + G * 2;                          // [NW][G][4 * KS], for GM 16
-    float* ss = sw + (GM <= 4 ? 0 : G * SLM_PG_KEYS);  // [G][SLM_PG_KEYS], with direct and mass_out
+    float* sw = sml + ((G * 2 + 3) & ~3);             // [NW][G][4 * KS], for GM 16
+    float* ss = sw + (MANY ? G * SLM_PG_KEYS : 0);    // [G][SLM_PG_KEYS], with direct and mass_out
 
     // this lane's key: the one whose score it will have
-    const int mine = w * (4 * KS) + (HALF ? 16 * r + c : 4 * (c & (KS - 1)) + r);
+    const int mine = w * (4 * KS) + (HALF || MANY ? KS * r + (c & (KS - 1)) : 4 * (c & (KS - 1)) + r);
     const bool some = base + w * (4 * KS) < most;     // the wave has a key to look at
     bool sees = base + mine < most;
     uint32_t row = 0;
@@ -286,11 +290,11 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
             for (int i = 0; i < NT; i++) to[j][i] = *(const V4*)((const T*)from + o + min(64 * i + 4 * c, dh - 4));
         });
     };
-    // keys: fp32 like the values; fp16 as the matrix unit takes them, 16 keys a tile, a lane eight of
-    // every 32 elements of key c
-    constexpr int NK = HALF ? 2 * NT : NT;
-    std::conditional_t<HALF, h8, f4> k[HALF ? 4 : KS][NK];
+    // keys: like the values, or as the matrix unit takes them, 16 keys a tile
+    constexpr int TILES = KS / 4, NK = HALF ? 2 * NT : MANY ? 4 * NT : NT;
+    std::conditional_t<HALF, h8, f4> k[HALF || MANY ? TILES : KS][NK];
     auto k_start = [&](int i) { return max(0, min(32 * i + 8 * r, dh - 8)); };
+    auto tile_lane = [&](int t) { return ((16 * t + c) / KS << 4) | ((16 * t + c) & (KS - 1)); };  // of key c's row
     if (some) {
         if constexpr (HALF) {
             // the four tiles' rows, from the lanes that have them
@@ -310,6 +314,13 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                         k[t][i] = h8{x.x, x.y, x.z, x.w, 0, 0, 0, 0};
                     }
                 }
+            }
+        } else if constexpr (MANY) {
+#pragma unroll
+            for (int t = 0; t < TILES; t++) {
+                const T* from = (const T*)a.k + (uint64_t)__shfl(row, tile_lane(t)) * (uint32_t)dh;
+#pragma unroll
+                for (int i = 0; i < NK; i++) k[t][i] = *(const f4*)(from + min(16 * i + 4 * r, dh - 4));
             }
         } else {
             load_rows(a.k, k);
@@ -346,8 +357,10 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
         }
     } else {
 #pragma unroll
-        for (int u = 0; u < QN; u++)
-            if (tid + u * THREADS < G * DP) sq[tid + u * THREADS] = q[u];
+        for (int u = 0; u < QN; u++) {
+            int i = tid + u * THREADS;
+            if (i < G * DP) sq[i / DP * QS + i % DP] = q[u];
+        }
     }
     const bool all = __ballot(sees) == ~0ull, any = __ballot(sees) != 0;
     lds_barrier();
@@ -362,15 +375,14 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 #pragma unroll
                     for (int e = 0; e < 8; e++)
                         if (twice >= 8 || e < twice) k[t][i][e] = 0;
-            } else if (64 * i + 4 * c >= dh) {
+            } else if (MANY ? 16 * i + 4 * r >= dh : 64 * i + 4 * c >= dh) {
 #pragma unroll
-                for (int j = 0; j < KS; j++) k[j][i] = V4{};
+                for (int j = 0; j < (MANY ? TILES : KS); j++) k[j][i] = V4{};
             }
         }
     }
 
-    float p[GM <= 4 ? GM : 1];
-    float* sp = sw + w * G * (4 * KS) + r * KS + (c & (KS - 1));
+    float p[MANY ? 1 : GM];
     auto scores = [&](auto gx, int g0, float* out) {  // gx heads from g0: their weights
         constexpr int GX = decltype(gx)::value;
         float x[GX], m[GX], l[GX];
@@ -410,7 +422,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                 }
 #pragma unroll
                 for (int g = 0; g < GX; g++) x[g] = x[g] * q_shift * a.scale;
-            } else {
+            } else if constexpr (!MANY) {
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
                     float s[KS];
@@ -444,54 +456,82 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
         for (int g = 0; g < GX; g++) {
             if (lane == 0) *(float2*)(swm + (w * G + g0 + g) * 2) = make_float2(m[g], l[g]);
             if (a.mass_out && c < KS) {
-                if (a.direct) ss[(g0 + g) * SLM_PG_KEYS + mine] = x[g];
-                else a.sc[((int64_t)item * a.heads + h * G + g0 + g) * SLM_PG_KEYS + mine] = x[g];
+                if (a.direct) ((LDS_MEM float*)ss)[(g0 + g) * SLM_PG_KEYS + mine] = x[g];
+                else ((GLOBAL_MEM float*)a.sc)[((int64_t)item * a.heads + h * G + g0 + g) * SLM_PG_KEYS + mine] = x[g];
             }
         }
     };
-    auto values = [&](auto gx, int slot, const float* pg) {  // gx heads: their values to LDS
-        constexpr int GX = decltype(gx)::value;
-        f4 o[GX][NT];
-#pragma unroll
-        for (int g = 0; g < GX; g++)
-#pragma unroll
-            for (int i = 0; i < NT; i++) o[g][i] = f4{0, 0, 0, 0};
-        if (some)
-            each<KS>([&](auto j) {
-#pragma unroll
-                for (int g = 0; g < GX; g++) {
-                    float w1 = bcast<j>(pg[g]);
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            o[g][i][e] = j ? fmaf(w1, (float)v[j][i][e], o[g][i][e]) : w1 * (float)v[j][i][e];
-                }
-            });
-#pragma unroll
-        for (int g = 0; g < GX; g++)
-#pragma unroll
-            for (int i = 0; i < NT; i++) so[(w * GC + slot + g) * DP + 64 * i + 4 * c + r] = scatter_rows(o[g][i]);
-    };
-    constexpr int GS = NT == 4 && !HALF ? 1 : 4;  // (sixteen waves: a head at a time, for the registers)
-    auto some_heads = [&](int n, auto f) {  // f(heads) for n of them, up to GS
-        if constexpr (GS == 4) {
-            if (n >= 4) return f(integral_constant<int, 4>());
-            if (n == 3) return f(integral_constant<int, 3>());
-            if (n == 2) return f(integral_constant<int, 2>());
-        }
-        f(integral_constant<int, 1>());
-    };
-    if constexpr (GM <= 4) {
+    float wgt[MANY ? KS : 1];  // head c's weights for the row's keys
+    if constexpr (!MANY) {
         scores(integral_constant<int, GM>(), 0, p);
     } else {
-        for (int g0 = 0; g0 < G; g0 += GS)
-            some_heads(G - g0, [&](auto gx) {
+        float* sp = sw + w * G * (4 * KS);
+        if constexpr (HALF) {
+            auto four = [&](auto gx, int g0) {
                 float e[decltype(gx)::value];
                 scores(gx, g0, e);
 #pragma unroll
-                for (int g = 0; g < decltype(gx)::value; g++) sp[(g0 + g) * (4 * KS)] = e[g];
-            });
+                for (int g = 0; g < decltype(gx)::value; g++) sp[(g0 + g) * (4 * KS) + KS * r + c] = e[g];
+            };
+            for (int g0 = 0; g0 < G; g0 += 4) {
+                if (G - g0 >= 4) four(integral_constant<int, 4>(), g0);
+                else if (G - g0 == 3) four(integral_constant<int, 3>(), g0);
+                else if (G - g0 == 2) four(integral_constant<int, 2>(), g0);
+                else four(integral_constant<int, 1>(), g0);
+            }
+        } else {
+            f4 acc[TILES] = {};
+            if (some)
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+                    if (16 * i >= dh) break;
+                    const f4 q1 = *(const f4*)(sq + min(c, G - 1) * QS + 16 * i + 4 * r);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int t = 0; t < TILES; t++)
+                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(q1[e], k[t][i][e], acc[t], 0, 0, 0);
+                }
+            // row r has heads 4r .. 4r + 3, a lane the tiles' key c
+            bool seen[TILES];
+#pragma unroll
+            for (int t = 0; t < TILES; t++) seen[t] = __shfl((int)sees, tile_lane(t));
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const int g = 4 * r + n;
+                float x[TILES], m = NEG_INF, l = 0.0f;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    x[t] = seen[t] ? acc[t][n] * a.scale : NEG_INF;
+                    m = fmaxf(m, x[t]);
+                }
+                m = row_max(m);
+                if (any) m = fmaxf(m, -FLT_MAX);
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    float e = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[t] - m);
+                    l += e;
+                    if (g >= G) continue;
+                    sp[g * (4 * KS) + 16 * t + c] = e;
+                    if (a.mass_out) {
+                        const int key = w * (4 * KS) + 16 * t + c;
+                        if (a.direct) ((LDS_MEM float*)ss)[g * SLM_PG_KEYS + key] = x[t];
+                        else ((GLOBAL_MEM float*)a.sc)[((int64_t)item * a.heads + h * G + g) * SLM_PG_KEYS + key] = x[t];
+                    }
+                }
+                l = row_sum(l);
+                if (c == 0 && g < G) *(float2*)(swm + (w * G + g) * 2) = make_float2(m, l);
+            }
+        }
+        // (a wave's own writes: in order before these reads)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < KS; j += 4) {
+            f4 x = *(const f4*)(sp + min(c, G - 1) * (4 * KS) + KS * r + j);
+#pragma unroll
+            for (int e = 0; e < 4; e++) wgt[j + e] = x[e];
+        }
     }
     if (NT == 4 && some) load_rows(a.v, v);
     if (some && !all) {  // what is not seen may hold anything
@@ -503,41 +543,64 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
             }
         });
     }
-    for (int c0 = 0; c0 < G; c0 += GC) {
-        const int ng = min(G - c0, GC);
-        if constexpr (GM <= 4) {
-            values(integral_constant<int, GM>(), 0, p);
-        } else {
-            for (int g0 = 0; g0 < ng; g0 += GS)
-                some_heads(ng - g0, [&](auto gx) {
-                    float e[decltype(gx)::value];
+    each<DP / CH>([&](auto part) {  // elements CH·part on
+        if constexpr (MANY) {
+            f4 acc[4] = {};  // element 64·part + 4c + e of heads 4r .. 4r + 3
+            if (some)
+                each<KS>([&](auto j) {
 #pragma unroll
-                    for (int g = 0; g < decltype(gx)::value; g++) e[g] = sp[(c0 + g0 + g) * (4 * KS)];
-                    values(gx, g0, e);
+                    for (int e = 0; e < 4; e++)
+                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(wgt[j], (float)v[j][part][e], acc[e], 0, 0, 0);
                 });
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                if (4 * r + n < G)
+                    *(f4*)(so + (w * G + 4 * r + n) * CH + 4 * c) = f4{acc[0][n], acc[1][n], acc[2][n], acc[3][n]};
+        } else {
+            f4 o[GM][NT];
+#pragma unroll
+            for (int g = 0; g < GM; g++)
+#pragma unroll
+                for (int i = 0; i < NT; i++) o[g][i] = f4{0, 0, 0, 0};
+            if (some)
+                each<KS>([&](auto j) {
+#pragma unroll
+                    for (int g = 0; g < GM; g++) {
+                        float w1 = bcast<j>(p[g]);
+#pragma unroll
+                        for (int i = 0; i < NT; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                o[g][i][e] = j ? fmaf(w1, (float)v[j][i][e], o[g][i][e]) : w1 * (float)v[j][i][e];
+                    }
+                });
+#pragma unroll
+            for (int g = 0; g < GM; g++)
+#pragma unroll
+                for (int i = 0; i < NT; i++) so[(w * G + g) * CH + 64 * i + 4 * c + r] = scatter_rows(o[g][i]);
         }
         lds_barrier();
         // the superblock's, from its waves' in order: four elements a thread
-        for (int i = tid; i < ng * (DP / 4); i += THREADS) {
-            int g = i / (DP / 4), d = i % (DP / 4) * 4, gg = c0 + g;
+        for (int i = tid; i < G * (CH / 4); i += THREADS) {
+            const int g = i / (CH / 4), in = i % (CH / 4) * 4, d = CH * part + in;
             if (d >= dh) continue;
             float m = NEG_INF, l = 0.0f;
             float2 ml[NW];
             f4 o = {0, 0, 0, 0};
 #pragma unroll
-            for (int k2 = 0; k2 < NW; k2++) ml[k2] = *(const float2*)(swm + (k2 * G + gg) * 2);
+            for (int k2 = 0; k2 < NW; k2++) ml[k2] = *(const float2*)(swm + (k2 * G + g) * 2);
 #pragma unroll
             for (int k2 = 0; k2 < NW; k2++) m = fmaxf(m, ml[k2].x);
             const float ms = m == NEG_INF ? 0.0f : m;
 #pragma unroll
             for (int k2 = 0; k2 < NW; k2++) {
                 float f = __builtin_amdgcn_exp2f(ml[k2].x - ms);
-                f4 z = *(const f4*)(so + (k2 * GC + g) * DP + d);
+                f4 z = *(const f4*)(so + (k2 * G + g) * CH + in);
                 l = fmaf(ml[k2].y, f, l);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], f, o[e]);
             }
-            const int head = h * G + gg;
+            const int head = h * G + g;
             if (a.direct) {
                 float* y = a.y + ((int64_t)b * a.heads + head) * dh + d;
 #pragma unroll
@@ -545,14 +608,14 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                     float z = m == NEG_INF ? 0.0f : o[e] / l;
                     y[e] = a.r16 ? r16(z) : z;
                 }
-                if (d == 0) *(float2*)(sml + 2 * gg) = make_float2(m, l);
+                if (d == 0) *(LDS_MEM f2*)(sml + 2 * g) = f2{m, l};
             } else {
                 *(f4*)(a.po + ((int64_t)item * a.heads + head) * dh + d) = o;
-                if (d == 0) *(float2*)(a.ml + 2 * ((int64_t)head * a.items + item)) = make_float2(m, l);
+                if (d == 0) *(GLOBAL_MEM f2*)(a.ml + 2 * ((int64_t)head * a.items + item)) = f2{m, l};
             }
         }
-        if (c0 + GC < G) lds_barrier();  // (the next heads' sums go where these lie)
-    }
+        if (part + 1 < DP / CH) lds_barrier();  // (the next elements' sums go where these lie)
+    });
     if (!a.direct || !a.mass_out) return;
     lds_barrier();
     if (NT > 1 && tid >= SLM_PG_KEYS) return;
@@ -566,7 +629,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 }
 
 #define PAGED_ATTN(name, T, NT, GM) \
-    KERNEL void __launch_bounds__(sizeof(T) == 2 ? 256 : 256 * NT) name(PAttnArgs a) { attn_body<T, NT, GM>(a); }
+    KERNEL void __launch_bounds__(sizeof(T) == 2 || NT == 1 ? 256 : 512) name(PAttnArgs a) { attn_body<T, NT, GM>(a); }
 #define PAGED_ATTNS(name, T, NT)       \
     PAGED_ATTN(name##_1, T, NT, 1)     \
     PAGED_ATTN(name##_2, T, NT, 2)     \
@@ -575,10 +638,10 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     PAGED_ATTN(name##_16, T, NT, 16)
 PAGED_ATTNS(slm_paged_attn_1, float, 1)
 PAGED_ATTNS(slm_paged_attn_2, float, 2)
-PAGED_ATTN(slm_paged_attn_4_16, float, 4, 16)
+PAGED_ATTNS(slm_paged_attn_4, float, 4)
 PAGED_ATTNS(slm_paged_attn16_1, _Float16, 1)
 PAGED_ATTNS(slm_paged_attn16_2, _Float16, 2)
-PAGED_ATTN(slm_paged_attn16_4_16, _Float16, 4, 16)
+PAGED_ATTNS(slm_paged_attn16_4, _Float16, 4)
 
 // y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), superblock z in group z % KG of
 // dh / 4 threads, a group in order, then the groups in order. Behind them, with mass_out, four

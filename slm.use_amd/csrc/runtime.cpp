@@ -904,8 +904,8 @@ size_t pattend_bytes(size_t items, size_t heads, size_t dh, bool mass) {
 // Workgroups that a row of n logits is split over while the rows are few: four-wave ones, a panel
 // of 8192 logits each, up to 64 (of whole panels); else one of sixteen waves (four for up to
 // 8192 logits). Measured, split against not, 20 alternatives: one row of 32000 11.1 against 11.7 us,
-// 65 rows of 32000 about 13.1 against 14.2, of 65536 16.1 against 18.1; 100 rows of 32000 14.4 against
-// 14.2, of 131072 28.2 against 27.7; 160 rows of 32000 16.0 against 15.6, of 131072 32.5 against 28.9.
+// 64 rows of 32000 13.1 (65 of them, not split, 14.2), of 65536 16.1 (18.1); 100 rows of 131072 28.2
+// against 27.7; 159 rows of 32000 16.0 (161, not split, 15.6), of 131072 32.5 (28.9).
 constexpr int64_t LOGP_SHORT = 8192, LOGP_PARTS = 64, LOGP_FEW_ROWS = 64;
 int64_t logp_parts(int64_t m, int64_t n) {
     if (m > LOGP_FEW_ROWS || n <= LOGP_SHORT) return 1;
@@ -992,12 +992,13 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
             if (a.mass_out) a.sc = a.po + items * H * n[4];
         }
         int nti = n[4] <= 64 ? 0 : n[4] <= 128 ? 1 : 2;
-        bool many = G > 4 || nti == 2;
+        bool many = G > 4;
         // (LDS: the queries or their parts; the waves' values, maxima and sums; all of theirs; the
         // weights where they are not in registers; the scores where they go no further)
-        int64_t nt = 1 << nti, dp = 64 * nt, gc = nt == 4 ? std::min<int64_t>(G, 4) : G, nw = half ? 4 : 4 * nt;
-        int64_t lds = (half ? (G + 3) / 4 * 6 * (dp + 8) : G * dp) + nw * gc * dp + nw * G * 2 + G * 2 +
-                      (many ? G * SLM_PG_KEYS : 0) + (a.direct && a.mass_out ? G * SLM_PG_KEYS : 0);
+        int64_t nt = 1 << nti, dp = 64 * nt, nw = half || nti == 0 ? 4 : 8;
+        int64_t lds = (half ? (G + 3) / 4 * 6 * (dp + 8) : G * (many ? dp + 4 : dp)) + nw * G * (many ? 64 : dp) +
+                      nw * G * 2 + ((G * 2 + 3) & ~3) + (many ? G * SLM_PG_KEYS : 0) +
+                      (a.direct && a.mass_out ? G * SLM_PG_KEYS : 0);
         out.push_back(mk_desc(k.pattn[half][nti][many ? 4 : G - 1], (uint32_t)(items * kh), (uint32_t)(64 * nw), (uint32_t)(4 * lds), a));
         if (!a.direct) {
             int wide = o.f[1] == PATTEND_LONG, pairs = wide ? 4 : 1;
@@ -3899,7 +3900,7 @@ int load_kernels(slm_hip* c) {
     for (auto& f : batch) TRY(get_batch(f.f, f.n));
     for (int half = 0; half < 2; half++)
         for (int t = 0; t < 3; t++)
-            for (int m = t == 2 ? 4 : 0; m < 5; m++)
+            for (int m = 0; m < 5; m++)
                 TRY(get_batch(&k.pattn[half][t][m], std::string("slm_paged_attn") + (half ? "16_" : "_") +
                                                         std::to_string(1 << t) + "_" + std::to_string(m < 4 ? m + 1 : 16)));
     return SLM_OK;
