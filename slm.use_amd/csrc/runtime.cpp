@@ -24,6 +24,7 @@
 #include <cstdio>
 #include <cstring>
 #include <map>
+#include <new>
 #include <set>
 #include <string>
 #include <vector>
@@ -5083,7 +5084,8 @@ int slm_hip_seqs_new(slm_hip* c, size_t page, size_t max_n, size_t max_pages, sl
         max_n * ((slots + SLM_PG_KEYS - 1) / SLM_PG_KEYS) > (size_t)1 << 22)
         return fail(c, SLM_E_UNSUPPORTED, "seqs_new: %zu sequences of %zu pages of %zu slots", max_n, max_pages, page);
     TRY(refuse_capture(c, "seqs_new"));
-    slm_seqs* s = new slm_seqs();
+    slm_seqs* s = new (std::nothrow) slm_seqs();
+    if (!s) return fail(c, SLM_E_MEMORY, "seqs_new");
     s->page = page;
     s->max_n = max_n;
     s->max_pages = max_pages;
@@ -5110,6 +5112,7 @@ int slm_hip_seqs_free(slm_hip* c, slm_seqs* s) {
     if (!s) return SLM_OK;
     for (auto it = c->seqs.begin(); it != c->seqs.end(); ++it) {
         if (it->second != s) continue;
+        TRY(refuse_capture(c, "seqs_free"));
         TRY(taint(c));  // a step's calls recorded so far run first
         drop_graphs(c);
         HIPC(c, hipStreamSynchronize(mstream(c)));
@@ -5151,6 +5154,12 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     }
     if (max_page >= (uint32_t)1 << 27) return fail(c, SLM_E_UNSUPPORTED, "seqs_set: page %u (2^27 or more)", max_page);
     if (rows >= (size_t)1 << 31) return fail(c, SLM_E_UNSUPPORTED, "seqs_set: %zu new tokens", rows);
+    try {  // (a byte a page)
+        s->uses.assign(n ? max_page + 1 : 0, 0);
+        s->len.reserve(n);
+    } catch (const std::bad_alloc&) {
+        return fail(c, SLM_E_MEMORY, "seqs_set: page %u", max_page);
+    }
     TRY(taint(c));  // a step's calls recorded so far run with the batch as it was
     // Launches are sized by these, and a kept step is kept for its launches: the table's width
     // and the count of superblocks go up in steps, so that a batch that grows by a token changes
@@ -5160,7 +5169,6 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     while (step * 16 <= items) step *= 2;
     size_t all = (items + step - 1) / step * step;
 
-    s->uses.assign(n ? max_page + 1 : 0, 0);
     s->shared = s->fresh_shared = false;
     for (size_t b = 0; b < n; b++)
         for (size_t i = 0; i < pages_of(len[b]); i++) {

@@ -249,6 +249,7 @@ def test_under_a_callers_capture(host, hip):
         refused(host, -3, f)
     refused(host, -3, t.s.set, t.lens, t.table)
     refused(host, -3, hip.seqs, 16, 1, 1)
+    refused(host, -3, t.s.free)
     refused(host, -3, hip.logprobs, lp.ptr, x.ptr, [0], 100)
     host.lib.stub_set_capturing(0)
     t.attend()
