@@ -3,9 +3,9 @@
 // compiled with the same flags (expressions round as written).
 //
 // A paged cache is [pages][key heads][page][dh]: token t of a sequence lies in slot t % page of
-// page table[t / page]. Every result is computed in an order that depends on the sequence
-// alone, not on the batch around it or on how the launch is cut: the bits of a sequence's
-// attention are the same whatever it is batched with.
+// page table[t / page]. The bits of a sequence's attention and eviction depend on the sequence
+// alone, not on the batch around it or on how the launch is cut. (Log probabilities add a row up in
+// an order that goes by the rows' number and alignment.)
 
 #include <float.h>
 #include <hip/hip_runtime.h>
@@ -91,7 +91,8 @@ __device__ __forceinline__ uint32_t row_of(const SeqsDev& s, int b, uint32_t t, 
 
 // Rows of new tokens lie one sequence after another; a row's sequence is found by bisection of
 // the batch's row offsets. One thread an element: a row of 64 floats is one wave's store of 256
-// bytes. A slot's noted weight starts at zero, its position is the token's.
+// bytes. A slot's noted weight starts at zero, its position is the token's. Bound by the launch and
+// its chain of reads (offset, length, table, row): 1.5 to 5 us from one sequence to 64.
 template <typename T>
 __device__ __forceinline__ void store_body(const PStoreArgs& a) {
     const int64_t per = (int64_t)a.kh * a.dh, total = (int64_t)a.rows * per;
@@ -122,11 +123,21 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 // ---------------------------------------------------------------------------------------
 
 // y_g = sum_t softmax_t(scale · q_g·k_t) v_t for the query heads g of one key head. A workgroup
-// takes one superblock of SLM_PG_KEYS slots, its waves 64 keys each (32 of fp32 heads above 64); for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
+// takes one superblock of SLM_PG_KEYS slots, its waves 64 keys each (32 of fp32 heads above 64);
+// for each head a wave has the maximum m, l = sum 2^(x - m) and o = sum 2^(x - m) v of
 // x = (scale · log2 e) q·k over its keys, the workgroup those of the superblock, and
 // slm_paged_join_* adds the superblocks up. No visible key: m = -inf; one at least: m >= -FLT_MAX.
 //
-// What bounds it is the reading of keys and values, so a wave issues all of its own (32 KB of
+// A superblock is where a long cache is cut for the chip's 256 compute units and where bits are
+// fixed: 12000 tokens of one sequence are 47 workgroups a key head. Heads of one key head follow
+// each other in the grid: their rows are one page's (the heads slowest: 62 -> 103 us for 64 x 2500
+// tokens of 12 heads).
+//
+// What bounds it is the reading of keys and values (fp32, 64 sequences of up to 2500 tokens, 12
+// heads of 64: 346 MB in 61 us, 5.6 TB/s; two of 100003, 4 key heads: 410 MB in 81 us, 5.0; fp16,
+// 24 of up to 6000, 4 key heads: 55 MB in 15 us, 3.6, where four workgroups a compute unit are
+// all there are), and for short caches its chain: batch, table, rows, keys, scores, values, sums
+// (one sequence of 37 tokens 4.8 us). So a wave issues all of its keys and values (32 KB of
 // fp32) at once, straight into registers, as soon as it has its rows' addresses: 16 lanes read
 // a row, each 4 of every 64 elements. A row's dot product is then in 16 lanes, and 16 rows'
 // are brought to one lane each by adding and halving (15 additions, not 64): the softmax
@@ -226,8 +237,12 @@ __device__ __forceinline__ float scatter_rows(f4 v) {
     return add(__builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
 }
 
-// GM: the query heads a key head (1 to 4: exactly), or 16: any number, which go through the matrix
-// unit (16x16x4, fp32; the heads are the rows of both products, whatever their number): a score
+// GM: the query heads a key head, 1 to 4 exactly, on the vector units; or 16: any number, through the
+// matrix unit. Measured, 8 sequences of 12000 tokens, 4 heads on each of 4 key heads: exactly 47 us
+// (fp32, 64), 97 (128), 30 (fp16, 64), 56 (fp16, 128), by the matrix unit 50, 118, 35, 76; 16 heads on
+// one of 64 exactly, four at a time, 31, by the matrix unit 23. GM 16 (9 sequences of up to 7777, 8 heads
+// on each of 2 fp16 key heads of 128: 18 us, 1.8 TB/s, one workgroup a compute unit): the products
+// are 16x16x4, fp32; the heads are the rows of both, whatever their number: a score
 // tile is 16 heads by 16 keys, a lane eight or sixteen bytes of every 32 or 16 elements of key c
 // of the tile; the weights go by way of LDS to where a value product wants them, which takes the
 // values as they lie.
@@ -646,7 +661,12 @@ PAGED_ATTNS(slm_paged_attn16_4, _Float16, 4)
 // y = sum_z o_z 2^(m_z - M) / L: a workgroup a (sequence, head), superblock z in group z % KG of
 // dh / 4 threads, a group in order, then the groups in order. Behind them, with mass_out, four
 // waves a (superblock, key head): mass_out = mass + sum_g 2^(x_g - M_g) / L_g. Sixteen waves a
-// workgroup, or four where that still leaves every superblock a group of its own (the same sums).
+// workgroup, or four where that still leaves every superblock a group of its own: the same sums.
+// Bound by its chain (4.1 us for 64 x 12 heads of 10 superblocks), for long caches by the noted weights
+// (two of 100003 tokens, 12 heads: 11 us for 18 MB). Measured, the whole call: 64 sequences of
+// 1066 tokens 32 us with four waves, 34 with sixteen; one of 51200 fp16 tokens, heads of 256, 74
+// with four, 71 with sixteen. (Joined by the workgroup that is last to be done instead of a
+// launch: 6 to 12 us slower, by the fence that every workgroup then needs.)
 template <int THREADS>
 __device__ __forceinline__ void join_body(const PAttnArgs& a) {
     __shared__ f4 so[THREADS];
@@ -806,6 +826,13 @@ __device__ __forceinline__ void move_rows(const PEvictArgs& a, const uint32_t* t
 // key to be told from another. Then the slots that stay, a bit each, 64 a wave at a time; from
 // the words' counts, added up, which of the first `keep` are left and which of those behind move
 // there. Few moves (SLM_MOVES_HERE) are made here, more by a launch of their own.
+//
+// Bound by the chain of its steps, a barrier each (one sequence of 1040 tokens, 4 heads: 7 us; 32
+// of up to 4200, 4 heads, of which up to 199 move: 14; 12 of 16384, 12 heads: 27), and past `room` by one
+// compute unit's reading of the weights, five to eight times over: one sequence of 36000 tokens cut
+// to 30000 takes 60 us, of 40000 149. Measured for the moves: 32 sequences, up to 250 moves, here
+// 17.5 us against 20.3 by a launch; one sequence, 500 moves, 15.7 here, 14.1 by a launch; 900,
+// 18.9 and 14.9.
 KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     __shared__ uint32_t hist[2048];
     __shared__ uint32_t red[6][16];
@@ -1050,7 +1077,8 @@ KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     }
 }
 
-// The moves of a (sequence, key head), SLM_MOVES_WG of them a workgroup.
+// The moves of a (sequence, key head), SLM_MOVES_WG of them a workgroup. Bound by memory: 12
+// sequences of 12 heads of 64, 467 MB read and written in 101 us, 4.6 TB/s.
 template <typename V>
 __device__ __forceinline__ void move_body(const PEvictArgs& a, uint32_t blocks) {
     __shared__ uint32_t to[SLM_MOVES_WG], from[SLM_MOVES_WG];
@@ -1139,6 +1167,10 @@ __device__ __forceinline__ void wave_nth(uint32_t key, int want0, int want1, uin
 //
 // With SPLIT a row goes to `parts` workgroups, which leave their sums and alternatives to
 // slm_logprobs_join.
+//
+// Bound by reading the logits where there are many (1021 rows of 65003: 265 MB in 55 us, 4.8
+// TB/s), else by its chain: read, maxima, bound, lists, ranks (256 rows of 32000, 5 alternatives:
+// one workgroup a compute unit, 11 to 12 us; one row of 32000 with 20: 7.5 and 4 us for its join).
 template <int W, bool SPLIT>
 __device__ __forceinline__ void logprobs_body(const LogpArgs& a) {
     __shared__ uint64_t list[W][128], fin[W * 64];
