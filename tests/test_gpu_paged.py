@@ -199,6 +199,42 @@ def test_long_cache(hip, pkg):
 
 
 @pytest.mark.parametrize("half", [False, True])
+def test_cache_of_more_than_2_32_values(hip, pkg, half):
+    """Stored, attended, evicted and attended again on a cache's first and last pages."""
+    KH, dh, page, pages, n, keep = 1, 256, 64, (1 << 32) // (256 * 64) + 40, 200, 100
+    k, v = (hip.alloc_pages(pages, KH, page, dh, half=half) for _ in range(2))
+    mass, born = hip.alloc(pages * page), hip.alloc(pages * page)
+    g = pkg.Pages(pages=pages, page=page, key_heads=KH, dh=dh, k=k.ptr, v=v.ptr, mass=mass.ptr, born=born.ptr)
+    ids = np.array([pages - 1, 0, pages - 2, 7])
+    rng = rng_of(9, half)
+    ref = Cache(rng, [n], 1, dh, n, half=half, spare=0)
+    s = hip.seqs(page, 1, 4)
+    s.set([n], [ids], fresh=[n])
+    dk, dv = hip.upload(ref.k), hip.upload(ref.v)
+    hip.paged_store(s, g, dk.ptr, dv.ptr)
+    ref.mass[:] = 0
+    for lens in (n, keep):
+        q = rng.standard_normal((1, 1, dh)).astype(np.float32)
+        dq, y = hip.upload(q), hip.alloc(dh)
+        s.set([lens], [ids], seen=[n])
+        hip.paged_attend(s, g, y.ptr, dq.ptr, heads=1, scale=1 / 16, mass_out=mass.ptr)
+        ref.lens[:] = lens
+        want, wmass, bound, mbound = ref.attend(q, 1 / 16)
+        check(y.read().reshape(q.shape), want, bound)
+        got = mass.read().reshape(pages, page)[ids].ravel()[:n]
+        check(got[:lens], wmass.ravel()[:lens], mbound.ravel()[:lens])
+        if lens == n:
+            ref.mass[:] = got.reshape(ref.mass.shape)
+            hip.paged_evict(s, g, mass.ptr, born.ptr, keep=keep, recent=10)
+            ref.evict(keep, 10)
+            got = read_bits(born).reshape(pages, page)[ids].ravel()[:keep]
+            assert np.array_equal(got, ref.born.ravel()[:keep])
+    s.free()
+    for b in (k, v, mass, born):
+        b.free()
+
+
+@pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("page,dh,KH", [(1, 4, 1), (16, 64, 4), (7, 80, 3), (100, 256, 2)])
 def test_store(hip, pkg, page, dh, KH, half):
     """New tokens of several sequences, none to a whole prompt: their slots alone change."""
@@ -449,6 +485,53 @@ def test_kept_steps_follow_the_batch(hip, pkg):
         check(got, wmass, mbound)
         c.mass = got
     assert hip.graph_stats()["captured"] > before
+
+
+def test_kept_steps_share_the_workspace(pkg):
+    """Two recorded steps kept as graphs, run in turn, and between them calls of their own that need
+    more of the workspace than either: every run gives what the first gave."""
+    hip = pkg.Hip(0)
+    rng = rng_of(32)
+    H, KH, dh, vocab = 4, 2, 64, 40000
+    sets, x = [], hip.upload(rng.standard_normal((2, vocab)))
+    for lens in ([700, 90], [1500, 3, 400], [3000] * 6):
+        c = Cache(rng, lens, KH, dh, 16)
+        g, up = c.upload(hip, pkg, born=False)
+        q, n = rng.standard_normal((len(lens), H, dh)).astype(np.float32), len(lens)
+        s = c.batch(hip)
+        s.set(c.lens, c.table, fresh=np.zeros(n))
+        sets.append((c, g, s, q, hip.upload(q), hip.alloc(q.size), hip.alloc(c.mass.size), up))
+    inv, cs, sn = hip.upload(np.ones(2, np.float32)), hip.alloc(2), hip.alloc(2)
+    lp, ti, tl = hip.alloc(2), hip.alloc(64), hip.alloc(64)
+    first = {}
+
+    def run(i, recorded, step):
+        c, g, s, q, dq, y, mass, up = sets[i]
+        hip.write(y, np.zeros(q.size)), hip.write(lp, np.zeros(2)), hip.write(tl, np.zeros(64))
+        if recorded:
+            hip.rope_table(cs.ptr, sn.ptr, inv.ptr, step, 1, 2)
+        hip.paged_attend(s, g, y.ptr, dq.ptr, heads=H, scale=0.1, mass_out=mass.ptr)
+        hip.logprobs(lp.ptr, x.ptr, [5, 39999], vocab, top=32, top_ids=ti.ptr, top_lp=tl.ptr)
+        if recorded:
+            hip.flush()
+        out = [b.read() for b in (y, lp, ti, tl)] + [mass.read().reshape(c.mass.shape)[c.used()]]
+        if i not in first:
+            want, wmass, bound, mbound = c.attend(q, np.float64(np.float32(0.1)), born=False)
+            check(out[0].reshape(q.shape), want, bound)
+            check(out[4], wmass[c.used()], mbound[c.used()])
+            first[i] = out
+        for a, b in zip(out, first[i]):
+            assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+    before = hip.graph_stats()["captured"]
+    for step in range(8):
+        run(0, True, step)
+        if step >= 4:
+            run(2, False, step)
+        run(1, True, step)
+        run(0, False, step)
+    assert hip.graph_stats()["captured"] >= before + 2
+    hip.close()
 
 
 def test_refusals(hip, pkg):
