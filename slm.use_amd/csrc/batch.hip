@@ -237,6 +237,13 @@ __device__ __forceinline__ float scatter_rows(f4 v) {
     return add(__builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
 }
 
+__device__ __forceinline__ float scatter_rows_max(f4 v) {  // the same of maxima
+    auto most = [](auto p) { return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])); };
+    float a = most(__builtin_amdgcn_permlane32_swap(__float_as_uint(v.x), __float_as_uint(v.z), false, false));
+    float b = most(__builtin_amdgcn_permlane32_swap(__float_as_uint(v.y), __float_as_uint(v.w), false, false));
+    return most(__builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+}
+
 // GM: the query heads a key head, 1 to 4 exactly, on the vector units; or 16: any number, through the
 // matrix unit. Measured, 8 sequences of 12000 tokens, 4 heads on each of 4 key heads: exactly 47 us
 // (fp32, 64), 97 (128), 30 (fp16, 64), 56 (fp16, 128), by the matrix unit 50, 118, 35, 76; 16 heads on
@@ -400,7 +407,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     float p[MANY ? 1 : GM];
     auto scores = [&](auto gx, int g0, float* out) {  // gx heads from g0: their weights
         constexpr int GX = decltype(gx)::value;
-        float x[GX], m[GX], l[GX];
+        float x[GX];
 #pragma unroll
         for (int g = 0; g < GX; g++) x[g] = NEG_INF;
         if (some) {
@@ -459,17 +466,23 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
             for (int g = 0; g < GX; g++)
                 if (!sees) x[g] = NEG_INF;
         }
+        // maxima and sums of the heads in one reduction: head r's in row r
+        f4 heads = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+        for (int g = 0; g < GX; g++) heads[g] = x[g];
+        float mr = GX == 1 ? wave_max(x[0]) : row_max(scatter_rows_max(heads));
+        if (any) mr = fmaxf(mr, -FLT_MAX);
+        heads = f4{0, 0, 0, 0};
 #pragma unroll
         for (int g = 0; g < GX; g++) {
-            m[g] = wave_max(x[g]);
-            if (any) m[g] = fmaxf(m[g], -FLT_MAX);
-            out[g] = m[g] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[g] - m[g]);
+            const float m = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mr), 16 * g));
+            out[g] = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[g] - m);
+            heads[g] = c < KS ? out[g] : 0.0f;
         }
-#pragma unroll
-        for (int g = 0; g < GX; g++) l[g] = wave_sum(c < KS ? out[g] : 0.0f);
+        const float lr = GX == 1 ? wave_sum(heads[0]) : row_sum(scatter_rows(heads));
+        if (c == 0 && r < GX) *(float2*)(swm + (w * G + g0 + r) * 2) = make_float2(mr, lr);
 #pragma unroll
         for (int g = 0; g < GX; g++) {
-            if (lane == 0) *(float2*)(swm + (w * G + g0 + g) * 2) = make_float2(m[g], l[g]);
             if (a.mass_out && c < KS) {
                 if (a.direct) ((LDS_MEM float*)ss)[(g0 + g) * SLM_PG_KEYS + mine] = x[g];
                 else ((GLOBAL_MEM float*)a.sc)[((int64_t)item * a.heads + h * G + g0 + g) * SLM_PG_KEYS + mine] = x[g];
@@ -561,12 +574,24 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     each<DP / CH>([&](auto part) {  // elements CH·part on
         if constexpr (MANY) {
             f4 acc[4] = {};  // element 64·part + 4c + e of heads 4r .. 4r + 3
-            if (some)
+            if (some) {
+                auto wide = [&](int j) {
+                    f4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = (float)v[j][part][e];
+                    return x;
+                };
+                f4 x = wide(0);
                 each<KS>([&](auto j) {
+                    // (the next four are widened while these are multiplied)
+                    f4 next = wide(j + 1 < KS ? j + 1 : j);
+                    if (HALF) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(wgt[j], (float)v[j][part][e], acc[e], 0, 0, 0);
+                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(wgt[j], x[e], acc[e], 0, 0, 0);
+                    x = next;
                 });
+            }
 #pragma unroll
             for (int n = 0; n < 4; n++)
                 if (4 * r + n < G)
