@@ -247,7 +247,7 @@ __device__ __forceinline__ float scatter_rows_max(f4 v) {  // the same of maxima
 // GM: the query heads a key head, 1 to 4 exactly, on the vector units; or 16: any number, through the
 // matrix unit. Measured, 8 sequences of 12000 tokens, 4 heads on each of 4 key heads: exactly 47 us
 // (fp32, 64), 97 (128), 30 (fp16, 64), 56 (fp16, 128), by the matrix unit 50, 118, 35, 76; 16 heads on
-// one of 64 exactly, four at a time, 31, by the matrix unit 23. GM 16 (9 sequences of up to 7777, 8 heads
+// one of 64 exactly, four at a time, 31, by the matrix unit 22. GM 16 (9 sequences of up to 7777, 8 heads
 // on each of 2 fp16 key heads of 128: 18 us, 1.8 TB/s, one workgroup a compute unit): the products
 // are 16x16x4, fp32; the heads are the rows of both, whatever their number: a score
 // tile is 16 heads by 16 keys, a lane eight or sixteen bytes of every 32 or 16 elements of key c
@@ -256,8 +256,8 @@ __device__ __forceinline__ float scatter_rows_max(f4 v) {  // the same of maxima
 //
 // fp16 keys always go through the matrix unit (16x16x32): its products are exact and its sums
 // fp32, so fp32 queries are cut into three fp16 parts (q = q0 + 2^-11 q1 + 2^-22 q2, 33 bits),
-// which are rows of one product: 4·part + head. A score's parts are then in three rows of 16 lanes, and
-// one exchange adds them and hands every lane its key's.
+// which are rows of one product for four heads: 4·part + head. A score's parts are then in three
+// rows of 16 lanes, and one exchange adds them and hands every lane its key's.
 template <typename T, int NT, int GM>
 __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     constexpr int QP = 64 * NT + 8;  // halves from one row of a query part to the next
@@ -501,15 +501,55 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 #pragma unroll
                 for (int g = 0; g < decltype(gx)::value; g++) sp[(g0 + g) * (4 * KS) + KS * r + c] = e[g];
             };
-            for (int g0 = 0; g0 < G; g0 += 4) {
+            for (int g0 = 0; G <= 8 && g0 < G; g0 += 4) {
                 if (G - g0 >= 4) four(integral_constant<int, 4>(), g0);
                 else if (G - g0 == 3) four(integral_constant<int, 3>(), g0);
                 else if (G - g0 == 2) four(integral_constant<int, 2>(), g0);
                 else four(integral_constant<int, 1>(), g0);
             }
-        } else {
+        }
+        // The heads are the rows: of fp32 keys, and of fp16 keys with more than eight heads, in three products
+        // (8 x 12000 tokens, 16 heads on one of 128: 34 us, four at a time 36.5; of 256 54 and 57; but 8
+        // heads on each of two of 128 46 and 44.5, of 256 49 and 45.5).
+        if (!HALF || G > 8) {
             f4 acc[TILES] = {};
-            if (some)
+            if constexpr (HALF) {
+                // the queries' smallest part first: each one's sums are 2^-11 of the next's unit
+                auto add = [&](int part, f4 (&to)[TILES]) {
+                    const _Float16* q = (const _Float16*)sq + ((min(c, G - 1) >> 2) * 12 + 4 * part + (min(c, G - 1) & 3)) * QP;
+#pragma unroll
+                    for (int i = 0; i < NK; i++) {
+                        h8 x = *(const h8_4*)(q + k_start(i));
+#pragma unroll
+                        for (int t = 0; t < TILES; t++) to[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, k[t][i], to[t], 0, 0, 0);
+                    }
+                };
+                if (some) {
+                    bool fine = true;
+#pragma unroll
+                    for (int part = 2; part >= 0; part--) {
+                        add(part, acc);
+#pragma unroll
+                        for (int t = 0; t < TILES; t++)
+#pragma unroll
+                            for (int n = 0; n < 4; n++) {
+                                if (part) acc[t][n] *= 0x1p-11f;
+                                else fine = fine && fabsf(acc[t][n]) <= FLT_MAX;
+                            }
+                    }
+                    if (__ballot(!fine)) {  // (an infinite or NaN key: part 0 alone says what it does)
+                        f4 one[TILES] = {};
+                        add(0, one);
+#pragma unroll
+                        for (int t = 0; t < TILES; t++)
+#pragma unroll
+                            for (int n = 0; n < 4; n++)
+                                if (!(fabsf(acc[t][n]) <= FLT_MAX)) acc[t][n] = one[t][n];
+                    }
+#pragma unroll
+                    for (int t = 0; t < TILES; t++) acc[t] *= q_shift;
+                }
+            } else if (some) {
 #pragma unroll
                 for (int i = 0; i < NK; i++) {
                     if (16 * i >= dh) break;
@@ -520,35 +560,55 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                         for (int t = 0; t < TILES; t++)
                             acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(q1[e], k[t][i][e], acc[t], 0, 0, 0);
                 }
+            }
             // row r has heads 4r .. 4r + 3, a lane the tiles' key c
-            bool seen[TILES];
 #pragma unroll
-            for (int t = 0; t < TILES; t++) seen[t] = __shfl((int)sees, tile_lane(t));
+            for (int t = 0; t < TILES; t++) acc[t] *= a.scale;
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < TILES; t++)
+                    if (!__shfl((int)sees, tile_lane(t))) acc[t] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+            }
+            float m[4], l[4];
+            f4 e[TILES];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                m[n] = NEG_INF;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) m[n] = fmaxf(m[n], acc[t][n]);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                m[n] = row_max(m[n]);
+                if (any) m[n] = fmaxf(m[n], -FLT_MAX);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                l[n] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    e[t][n] = m[n] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(acc[t][n] - m[n]);
+                    l[n] += e[t][n];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++) l[n] = row_sum(l[n]);
+            const int key = w * (4 * KS) + c;  // of tile 0
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 const int g = 4 * r + n;
-                float x[TILES], m = NEG_INF, l = 0.0f;
+                if (g >= G) continue;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) sp[g * (4 * KS) + 16 * t + c] = e[t][n];
+                if (c == 0) *(float2*)(swm + (w * G + g) * 2) = make_float2(m[n], l[n]);
+                if (!a.mass_out) continue;
+                LDS_MEM float* near = (LDS_MEM float*)ss + g * SLM_PG_KEYS + key;
+                GLOBAL_MEM float* far = (GLOBAL_MEM float*)a.sc + ((int64_t)item * a.heads + h * G + g) * SLM_PG_KEYS + key;
 #pragma unroll
                 for (int t = 0; t < TILES; t++) {
-                    x[t] = seen[t] ? acc[t][n] * a.scale : NEG_INF;
-                    m = fmaxf(m, x[t]);
+                    if (a.direct) near[16 * t] = acc[t][n];
+                    else far[16 * t] = acc[t][n];
                 }
-                m = row_max(m);
-                if (any) m = fmaxf(m, -FLT_MAX);
-#pragma unroll
-                for (int t = 0; t < TILES; t++) {
-                    float e = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(x[t] - m);
-                    l += e;
-                    if (g >= G) continue;
-                    sp[g * (4 * KS) + 16 * t + c] = e;
-                    if (a.mass_out) {
-                        const int key = w * (4 * KS) + 16 * t + c;
-                        if (a.direct) ((LDS_MEM float*)ss)[g * SLM_PG_KEYS + key] = x[t];
-                        else ((GLOBAL_MEM float*)a.sc)[((int64_t)item * a.heads + h * G + g) * SLM_PG_KEYS + key] = x[t];
-                    }
-                }
-                l = row_sum(l);
-                if (c == 0 && g < G) *(float2*)(swm + (w * G + g) * 2) = make_float2(m, l);
             }
         }
         // (a wave's own writes: in order before these reads)

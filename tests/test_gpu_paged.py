@@ -146,12 +146,46 @@ def test_infinities_and_nan_in_visible_keys(hip, pkg, half):
     assert fine[4].sum() == 2 * 15
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("heads", [7, 16])
+def test_infinities_under_many_heads(hip, pkg, heads, half):
+    """The same with more query heads on the key head; queries of both signs where a key is infinite."""
+    c = Cache(rng_of(41, heads), [600] * 5, 1, 64, 16, half)
+    q = np.abs(rng_of(42, heads).standard_normal((5, heads, 64))).astype(np.float32) + 0.1
+    q[2] = q[2].astype(np.float16)
+    at = [c.where(b) for b in range(5)]
+    bound = c.attend(q, 0.125, born=False)[2]  # (of all the keys: no less than of those that weigh)
+    c.k[at[0][0][400], 0, at[0][1][400]] = np.nan
+    c.k[at[1][0], 0, at[1][1]] = -np.inf
+    c.k[at[2][0][256:512], 0, at[2][1][256:512]] = -np.inf
+    c.k[at[3][0][5], 0, at[3][1][5], 9] = -np.inf                 # no weight: its infinite score is one element's
+    c.v[at[4][0][10], 0, at[4][1][10], 3] = np.inf
+    y, _ = attend(hip, pkg, c, q, mass=False)
+    want = c.attend(q, 0.125, born=False)[0]
+    assert np.all(np.isnan(y[:2])) and np.all(want[4, :, 3] == np.inf)
+    check(y[2:], want[2:], bound[2:])
+
+
 @pytest.mark.parametrize("qs,ks,scale", [(1e-6, 1.0, 3e5), (3e6, 1.0, 1e-6), (1e30, 1.0, 1e-30), (1.0, 2e-7, 1e6),
                                          (1.0, 2e4, 2e-5), (1.0, 1e4, 4e-5), (1e-9, 1e-6, 1e15), (0.0, 1.0, 1.0)])
 def test_fp16_keys_and_queries_of_any_size(hip, pkg, qs, ks, scale):
     """fp32 queries over fp16 keys: small ones, past fp16's range, keys below its normal numbers and at
     its largest (some of them infinite once rounded)."""
     c = Cache(rng_of(17), [300, 90], 2, 64, 16, True, scale=1.0)
+    c.k = c.values(c.k * ks)
+    q = (rng_of(18).standard_normal((2, 12, 64)) * qs).astype(np.float32)
+    q[..., ::7] *= np.float32(1e-4)
+    y, mass = attend(hip, pkg, c, q, scale=scale)
+    want, wmass, bound, mbound = c.attend(q, np.float64(np.float32(scale)), born=False)
+    check(y, want, bound)
+    check(mass[c.used()], wmass[c.used()], mbound[c.used()])
+
+
+@pytest.mark.parametrize("qs,ks,scale", [(1e-6, 1.0, 3e5), (3e6, 1.0, 1e-6), (1e30, 1.0, 1e-30), (1.0, 2e-7, 1e6),
+                                         (1.0, 2e4, 2e-5), (1.0, 1e4, 4e-5), (1e-9, 1e-6, 1e15), (0.0, 1.0, 1.0)])
+def test_fp16_keys_and_twelve_heads_of_any_size(hip, pkg, qs, ks, scale):
+    """The same with twelve query heads on one key head."""
+    c = Cache(rng_of(17), [300, 90], 1, 64, 16, True, scale=1.0)
     c.k = c.values(c.k * ks)
     q = (rng_of(18).standard_normal((2, 12, 64)) * qs).astype(np.float32)
     q[..., ::7] *= np.float32(1e-4)
