@@ -349,27 +349,30 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
         }
         if (NT < 4) load_rows(a.v, v);  // (the largest heads have room for one of the two in registers)
     }
-    float q_shift = 1.0f;
+    __shared__ __attribute__((aligned(16))) float q_unit[16];  // of fp16 keys: each head's power of two
     if constexpr (HALF) {
-        __shared__ uint32_t q_max;
-        if (tid == 0) q_max = 0;
+        // A head's queries are cut with its largest number in [2^13, 2^14), by a power of two that its scores
+        // get back: what another head of the key head holds has no part in it.
+        __shared__ uint32_t q_top[16];
+        if (tid < 16) q_top[tid] = 0;
         lds_barrier();
-        float m = 0.0f;
 #pragma unroll
-        for (int u = 0; u < QN; u++) m = fmaxf(m, fabsf(q[u]));
-        m = wave_max(m);
-        if (lane == 0) atomicMax(&q_max, __float_as_uint(m));
+        for (int u = 0; u < QN; u++) {
+            const int g = (64 * w + u * THREADS) / DP;  // (a wave's 64 elements are one head's)
+            if (g >= G) continue;
+            float m = fabsf(q[u]);
+            m = wave_max(m <= FLT_MAX ? m : 0.0f);
+            if (lane == 0) atomicMax(&q_top[g], __float_as_uint(m));
+        }
         lds_barrier();
-        // (queries past 2^14 come down to it, by a power of two that the scores get back)
-        const int e = max(0, (int)(q_max >> 23) - 127 - 13);
-        const float down = ldexpf(1.0f, -e);
-        q_shift = ldexpf(1.0f, e);
+        auto exponent = [&](int g) { return max((int)(q_top[g] >> 23) - 127 - 13, -126); };
+        if (tid < 16) q_unit[tid] = __uint_as_float((uint32_t)(127 + exponent(tid)) << 23);
 #pragma unroll
         for (int u = 0; u < QN; u++) {
             int i = tid + u * THREADS, g = i / DP, d = i % DP;
             if (g >= G) continue;
             _Float16* to = (_Float16*)sq + ((g >> 2) * 12 + (g & 3)) * QP + d;
-            float x = q[u] * down;
+            float x = q[u] * __uint_as_float((uint32_t)(127 - exponent(g)) << 23);
 #pragma unroll
             for (int k = 0; k < 3; k++) {
                 _Float16 part = (_Float16)x;
@@ -443,7 +446,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                     }
                 }
 #pragma unroll
-                for (int g = 0; g < GX; g++) x[g] = x[g] * q_shift * a.scale;
+                for (int g = 0; g < GX; g++) x[g] = x[g] * q_unit[g0 + g] * a.scale;
             } else if constexpr (!MANY) {
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
@@ -546,8 +549,9 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                             for (int n = 0; n < 4; n++)
                                 if (!(fabsf(acc[t][n]) <= FLT_MAX)) acc[t][n] = one[t][n];
                     }
+                    const f4 unit = *(const f4*)(q_unit + 4 * r);
 #pragma unroll
-                    for (int t = 0; t < TILES; t++) acc[t] *= q_shift;
+                    for (int t = 0; t < TILES; t++) acc[t] *= unit;
                 }
             } else if (some) {
 #pragma unroll
