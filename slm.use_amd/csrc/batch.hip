@@ -372,13 +372,17 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
             int i = tid + u * THREADS, g = i / DP, d = i % DP;
             if (g >= G) continue;
             _Float16* to = (_Float16*)sq + ((g >> 2) * 12 + (g & 3)) * QP + d;
-            float x = q[u] * __uint_as_float((uint32_t)(127 - exponent(g)) << 23);
+            const float whole = q[u] * __uint_as_float((uint32_t)(127 - exponent(g)) << 23);
+            float x = whole;
 #pragma unroll
             for (int k = 0; k < 3; k++) {
                 _Float16 part = (_Float16)x;
                 to[4 * k * QP] = part;
                 x = (x - (float)part) * 2048.0f;
             }
+            // What the parts leave (x 2^-33) is less than fp32's rounding of the element, but where that is far
+            // below the head's largest: a NaN then has the head's scores made element by element.
+            if (fabsf(x) > 512.0f * fabsf(whole) || (whole == 0.0f && q[u] != 0.0f)) to[0] = (_Float16)__builtin_nanf("");
         }
     } else {
 #pragma unroll
@@ -407,6 +411,21 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
         }
     }
 
+    // A score over fp16 keys that the parts cannot say (an infinite or NaN key or query, a query whose
+    // elements' sizes lie far apart): head g's and this lane's key's, element by element in fp32, read again.
+    auto by_element = [&](int g) {
+        const float* from = a.q + ((int64_t)b * a.heads + h * G + g) * dh;
+        const T* key = (const T*)a.k + (uint64_t)row * (uint32_t)dh;
+        float z = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < dh; d += 4) {
+            const V4 x = *(const V4*)(key + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) z = fmaf(from[d + e], (float)x[e], z);
+        }
+        return z;
+    };
+
     float p[MANY ? 1 : GM];
     auto scores = [&](auto gx, int g0, float* out) {  // gx heads from g0: their weights
         constexpr int GX = decltype(gx)::value;
@@ -425,28 +444,24 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                 }
                 // row r has the queries' part r: part 1 is in 2^-11ths, part 2 in 2^-22ths, there is no part 3
                 const float unit = r == 0 ? 1.0f : r == 1 ? 0x1p-11f : r == 2 ? 0x1p-22f : 0.0f;
-                bool fine = true;
+                uint32_t odd = 0;
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
                     x[g] = scatter_rows(f4{acc[0][g] * unit, acc[1][g] * unit, acc[2][g] * unit, acc[3][g] * unit});
-                    fine = fine && fabsf(x[g]) <= FLT_MAX;
+                    odd |= fabsf(x[g]) <= FLT_MAX ? 0 : 1u << g;
+                    x[g] *= q_unit[g0 + g];
                 }
-                if (__ballot(!fine)) {
-                    // an infinite or NaN key: part 0 alone says what it does (the others' zeros would
-                    // make NaNs of infinities)
+                if (__ballot(odd != 0)) {
+#pragma unroll 1
+                    for (int n = 0; n < GX; n++) {
+                        const float z = by_element(g0 + n);
 #pragma unroll
-                    for (int g = 0; g < GX; g++) {
-                        f4 z;
-#pragma unroll
-                        for (int t = 0; t < 4; t++) {
-                            float y = acc[t][g] * unit;
-                            z[t] = r == 0 || fabsf(y) <= FLT_MAX ? y : 0.0f;
-                        }
-                        x[g] = scatter_rows(z);
+                        for (int g = 0; g < GX; g++)
+                            if (g == n && (odd >> g & 1)) x[g] = z;
                     }
                 }
 #pragma unroll
-                for (int g = 0; g < GX; g++) x[g] = x[g] * q_unit[g0 + g] * a.scale;
+                for (int g = 0; g < GX; g++) x[g] *= a.scale;
             } else if constexpr (!MANY) {
 #pragma unroll
                 for (int g = 0; g < GX; g++) {
@@ -528,7 +543,7 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
                     }
                 };
                 if (some) {
-                    bool fine = true;
+                    uint32_t odd = 0;
 #pragma unroll
                     for (int part = 2; part >= 0; part--) {
                         add(part, acc);
@@ -537,21 +552,25 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
 #pragma unroll
                             for (int n = 0; n < 4; n++) {
                                 if (part) acc[t][n] *= 0x1p-11f;
-                                else fine = fine && fabsf(acc[t][n]) <= FLT_MAX;
+                                else odd |= fabsf(acc[t][n]) <= FLT_MAX ? 0 : 1u << (4 * t + n);
                             }
-                    }
-                    if (__ballot(!fine)) {  // (an infinite or NaN key: part 0 alone says what it does)
-                        f4 one[TILES] = {};
-                        add(0, one);
-#pragma unroll
-                        for (int t = 0; t < TILES; t++)
-#pragma unroll
-                            for (int n = 0; n < 4; n++)
-                                if (!(fabsf(acc[t][n]) <= FLT_MAX)) acc[t][n] = one[t][n];
                     }
                     const f4 unit = *(const f4*)(q_unit + 4 * r);
 #pragma unroll
                     for (int t = 0; t < TILES; t++) acc[t] *= unit;
+                    if (__ballot(odd != 0)) {
+#pragma unroll 1
+                        for (int g = 0; g < G; g++) {
+                            const float z = by_element(g);
+#pragma unroll
+                            for (int t = 0; t < TILES; t++) {
+                                const float y = __shfl(z, tile_lane(t));
+#pragma unroll
+                                for (int n = 0; n < 4; n++)
+                                    if (4 * r + n == g && (odd >> (4 * t + n) & 1)) acc[t][n] = y;
+                            }
+                        }
+                    }
                 }
             } else if (some) {
 #pragma unroll

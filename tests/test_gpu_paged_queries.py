@@ -69,3 +69,59 @@ def test_a_head_that_is_no_number(hip, pkg, shape, what, half):
         q[0, 1, 2] = what
         y, want = hold(hip, pkg, c, q)
         assert np.isnan(want[0, 1]).all() and np.isfinite(want[0, 0]).all() and np.isfinite(want[1]).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("size", [1e10, 1e20, 1e38])
+def test_a_large_element_that_meets_zeros(hip, pkg, shape, size, half):
+    """A query element of any size against keys that are zero there: the others decide."""
+    for i, lens in enumerate(LENS):
+        c, q = case(shape, lens, half, i)
+        c.k[..., 1] = 0
+        q[:, 0, 1] = size
+        q[:, 1, 1] = -size
+        hold(hip, pkg, c, q)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_small_elements_at_infinite_keys(hip, pkg, shape, half):
+    """An infinite key element counts with the query element's sign, however small that is: a score of
+    -inf (no weight) for positive ones at -inf, +inf (a NaN) for negative ones, NaN for zeros."""
+    for i, lens in enumerate(LENS):
+        c, q = case(shape, lens, half, i)
+        q[:, :, 3] = 1e-12
+        q[0, 0, 3] = 1e-39
+        with np.errstate(all="ignore"):
+            _, _, *bounds = c.attend(q, shape[2] ** -0.5, born=False)  # (of all the keys: no less than of those that weigh)
+        pg, sl = c.where(0)
+        c.k[pg[5], :, sl[5], 3] = -np.inf
+        c.k[pg[-1], :, sl[-1], 3] = -np.inf
+        y, want = hold(hip, pkg, c, q, bounds)
+        assert np.isfinite(want).all()
+        q[0, 1, 3] = -1e-12
+        y, want = hold(hip, pkg, c, q, bounds)
+        assert np.isnan(want[0, 1]).all() and np.isfinite(want[0, 0]).all()
+        q[0, 1, 3] = 0
+        y, want = hold(hip, pkg, c, q, bounds)
+        assert np.isnan(want[0, 1]).all() and np.isfinite(want[0, 0]).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_infinite_keys_under_full_queries(hip, pkg, shape, half):
+    """A superblock (and a whole wave's part of one) of keys that are -inf throughout, under positive
+    queries with all of fp32's digits: no weight. Under queries of both signs: NaN."""
+    c, q = case(shape, [600, 90], half)
+    with np.errstate(all="ignore"):
+        q = np.abs(q) + np.float32(0.1)
+        _, _, *bounds = c.attend(q, shape[2] ** -0.5, born=False)
+    for b, part in ((0, slice(256, 512)), (1, slice(0, 64))):
+        pg, sl = c.where(b)
+        c.k[pg[part], :, sl[part]] = -np.inf
+    y, want = hold(hip, pkg, c, q, bounds)
+    assert np.isfinite(want).all()
+    q[:, 1, 1] *= -1
+    y, want = hold(hip, pkg, c, q, bounds)
+    assert np.isnan(want[:, 1]).all() and np.isfinite(want[:, 0]).all()
