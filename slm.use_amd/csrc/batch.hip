@@ -143,7 +143,7 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 // are brought to one lane each by adding and halving (15 additions, not 64): the softmax
 // works on a key a lane. A key's weight goes back to the 16 lanes that hold its value by a lane
 // broadcast within the row.
-extern __shared__ char lds_[];
+extern __shared__ __attribute__((aligned(16))) char lds_[];  // (read and written 8 and 16 bytes at once)
 
 template <int J>
 __device__ __forceinline__ uint32_t bcast(uint32_t x) {  // lane J of each row of 16, to the row
