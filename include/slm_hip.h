@@ -240,7 +240,8 @@ int slm_hip_paged_evict(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, fl
  * [m][top] (both NULL with top 0): larger logits first, of equal ones the lower token, NaNs
  * last. `ids` is host memory, as slm_hip_gather's. Logits of −infinity are impossible tokens;
  * a row of nothing else has lp −infinity and entropy 0. A NaN or +infinity in a row goes where
- * the formulas take it. The outputs are fp32 in fp16 mode too. */
+ * the formulas take it. The outputs are fp32 in fp16 mode too. Up to 2^22 - 1 rows of up to 2^28
+ * logits (SLM_E_UNSUPPORTED past that). */
 int slm_hip_logprobs(slm_hip* ctx, float* lp, float* entropy, uint32_t* top_ids, float* top_lp, size_t top,
                      const float* x, const uint32_t* ids, size_t m, size_t n);
 

@@ -5398,26 +5398,32 @@ int slm_hip_logprobs(slm_hip* c, float* lp, float* entropy, uint32_t* top_ids, f
     }
     for (size_t i = 0; i < m; i++)
         if (ids[i] >= n) return fail(c, SLM_E_BOUNDS, "logprobs: token %u of %zu logits", ids[i], n);
-    Op o = op(OP_LOGPROBS);
-    o.p[0] = lp;
-    o.p[1] = entropy;
-    o.p[2] = top ? (const float*)top_ids : nullptr;
-    o.p[3] = top ? top_lp : nullptr;
-    o.p[4] = x;
-    o.n[0] = (int64_t)m;
-    o.n[1] = (int64_t)n;
-    o.n[2] = (int64_t)top;
-    int64_t parts = logp_parts((int64_t)m, (int64_t)n);
-    if (parts > 1) TRY(need_pws(c, m * (size_t)parts * (16 + 8 * top)));
-    // a few tokens go with the launch (a copy of four bytes ahead of it takes longer than it
-    // does); in a recorded step they are the step's values
-    if (m <= SLM_FEW_IDS && !recording(c)) {
-        o.n[3] = 1;
-        o.dyn = ids;
-    } else {
-        TRY(stage(c, ids, m * 4, &o.dyn));
+    // (the tokens of so many rows go up at once: more rows are launches of their own, of even sizes)
+    const size_t pieces = (m + STAGE_CAP / 4 - 1) / (STAGE_CAP / 4), each = (m + pieces - 1) / pieces;
+    for (size_t i = 0; i < m; i += each) {
+        const size_t rows = std::min(each, m - i);
+        Op o = op(OP_LOGPROBS);
+        o.p[0] = lp + i;
+        o.p[1] = entropy ? entropy + i : nullptr;
+        o.p[2] = top ? (const float*)(top_ids + i * top) : nullptr;
+        o.p[3] = top ? top_lp + i * top : nullptr;
+        o.p[4] = x + i * n;
+        o.n[0] = (int64_t)rows;
+        o.n[1] = (int64_t)n;
+        o.n[2] = (int64_t)top;
+        int64_t parts = logp_parts((int64_t)rows, (int64_t)n);
+        if (parts > 1) TRY(need_pws(c, rows * (size_t)parts * (16 + 8 * top)));
+        // a few tokens go with the launch (a copy of four bytes ahead of it takes longer than it
+        // does); in a recorded step they are the step's values
+        if (rows <= SLM_FEW_IDS && !recording(c)) {
+            o.n[3] = 1;
+            o.dyn = ids + i;
+        } else {
+            TRY(stage(c, ids + i, rows * 4, &o.dyn));
+        }
+        TRY(submit(c, o));
     }
-    return submit(c, o);
+    return SLM_OK;
 }
 
 // ---- diagnostics ----

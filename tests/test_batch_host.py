@@ -327,3 +327,18 @@ def test_logprobs(host, hip):
     f(lp.ptr, x.ptr, [], 50)
     assert host.lib.stub_launches() == before
     assert host.lib.slm_hip_logprobs(hip.ctx, lp.ptr, None, None, None, 0, x.ptr, None, 1, 50) == -1
+
+
+def test_many_rows_of_logits(host, hip):
+    """More rows than the tokens' way to the device takes at once; the most there may be, and one more."""
+    for m in (1 << 20, (1 << 20) + 1, (1 << 22) - 1):
+        x, lp = hip.alloc(2 * m), hip.alloc(m)
+        before = host.lib.stub_launches()
+        hip.logprobs(lp.ptr, x.ptr, np.ones(m), 2)
+        assert host.lib.stub_launches() == before + -(-m // (1 << 20))
+        ids = np.zeros(m)
+        ids[-1] = 2
+        refused(host, -5, hip.logprobs, lp.ptr, x.ptr, ids, 2)
+        x.free()
+        lp.free()
+    refused(host, -3, hip.logprobs, None, None, np.zeros(1 << 22), 2)
