@@ -197,7 +197,9 @@ typedef struct slm_pages {
  * it (slm_hip_upload rounds into it, slm_hip_read widens). Freed with slm_hip_free. */
 int slm_hip_alloc_pages(slm_hip* ctx, size_t pages, size_t key_heads, size_t page, size_t dh, int half,
                         float** out);
-/* Room for a batch of up to max_n sequences of up to max_pages pages of `page` slots. */
+/* Room for a batch of up to max_n sequences of up to max_pages pages of `page` slots: up to 65536
+ * sequences, fewer than 2^31 slots in each, 2^24 places in the table and 2^22 superblocks of 256
+ * slots in all (SLM_E_UNSUPPORTED past that). */
 int slm_hip_seqs_new(slm_hip* ctx, size_t page, size_t max_n, size_t max_pages, slm_seqs** out);
 int slm_hip_seqs_free(slm_hip* ctx, slm_seqs* seqs);
 /* The batch from now on: n sequences of len[b] tokens, of which the last fresh[b] are new (fresh

@@ -135,7 +135,7 @@ KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<
 //
 // What bounds it is the reading of keys and values (fp32, 64 sequences of up to 2500 tokens, 12
 // heads of 64: 346 MB in 61 us, 5.6 TB/s; two of 100003, 4 key heads: 410 MB in 81 us, 5.0; fp16,
-// 24 of up to 6000, 4 key heads: 55 MB in 15 us, 3.6, where four workgroups a compute unit are
+// 24 of up to 6000, 4 key heads: 55 MB in 14.4 us, 3.8, where four workgroups a compute unit are
 // all there are), and for short caches its chain: batch, table, rows, keys, scores, values, sums
 // (one sequence of 37 tokens 4.8 us). So a wave issues all of its keys and values (32 KB of
 // fp32) at once, straight into registers, as soon as it has its rows' addresses: 16 lanes read
@@ -246,18 +246,19 @@ __device__ __forceinline__ float scatter_rows_max(f4 v) {  // the same of maxima
 
 // GM: the query heads a key head, 1 to 4 exactly, on the vector units; or 16: any number, through the
 // matrix unit. Measured, 8 sequences of 12000 tokens, 4 heads on each of 4 key heads: exactly 47 us
-// (fp32, 64), 97 (128), 30 (fp16, 64), 56 (fp16, 128), by the matrix unit 50, 118, 35, 76; 16 heads on
+// (fp32, 64), 94 (128), 27 (fp16, 64), 54 (fp16, 128), by the matrix unit 49, 115, 33, 72; 16 heads on
 // one of 64 exactly, four at a time, 31, by the matrix unit 22. GM 16 (9 sequences of up to 7777, 8 heads
-// on each of 2 fp16 key heads of 128: 18 us, 1.8 TB/s, one workgroup a compute unit): the products
+// on each of 2 fp16 key heads of 128: 17 us, 1.9 TB/s, one workgroup a compute unit): the products
 // are 16x16x4, fp32; the heads are the rows of both, whatever their number: a score
 // tile is 16 heads by 16 keys, a lane eight or sixteen bytes of every 32 or 16 elements of key c
 // of the tile; the weights go by way of LDS to where a value product wants them, which takes the
 // values as they lie.
 //
 // fp16 keys always go through the matrix unit (16x16x32): its products are exact and its sums
-// fp32, so fp32 queries are cut into three fp16 parts (q = q0 + 2^-11 q1 + 2^-22 q2, 33 bits),
-// which are rows of one product for four heads: 4·part + head. A score's parts are then in three
-// rows of 16 lanes, and one exchange adds them and hands every lane its key's.
+// fp32, so fp32 queries are cut into three fp16 parts (q = q0 + 2^-11 q1 + 2^-22 q2, 33 bits, about
+// each head's own power of two), which are rows of one product for four heads: 4·part + head. A
+// score's parts are then in three rows of 16 lanes, and one exchange adds them and hands every lane
+// its key's. What the parts cannot say is made from the query and the key themselves.
 template <typename T, int NT, int GM>
 __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
     constexpr int QP = 64 * NT + 8;  // halves from one row of a query part to the next
@@ -527,8 +528,9 @@ __device__ __forceinline__ void attn_body(const PAttnArgs& a) {
             }
         }
         // The heads are the rows: of fp32 keys, and of fp16 keys with more than eight heads, in three products
-        // (8 x 12000 tokens, 16 heads on one of 128: 34 us, four at a time 36.5; of 256 54 and 57; but 8
-        // heads on each of two of 128 46 and 44.5, of 256 49 and 45.5).
+        // (8 x 12000 tokens, 16 heads on one of 128: 28.9 us, four at a time 30.2; of 256 43 and 44.6. The
+        // border is from when this LDS lay off 16 bytes and 8 heads on each of two of 128 took 46 us as rows
+        // and 44.5 four at a time; they now would take 36 as rows, and take 40; of 64, 24 either way).
         if (!HALF || G > 8) {
             f4 acc[TILES] = {};
             if constexpr (HALF) {
@@ -772,8 +774,8 @@ PAGED_ATTNS(slm_paged_attn16_4, _Float16, 4)
 // workgroup, or four where that still leaves every superblock a group of its own: the same sums.
 // Bound by its chain (4.1 us for 64 x 12 heads of 10 superblocks), for long caches by the noted weights
 // (two of 100003 tokens, 12 heads: 11 us for 18 MB). Measured, the whole call: 64 sequences of
-// 1066 tokens 32 us with four waves, 34 with sixteen; one of 51200 fp16 tokens, heads of 256, 74
-// with four, 71 with sixteen. (Joined by the workgroup that is last to be done instead of a
+// 1066 tokens 32 us with four waves, 34 with sixteen; one of 51200 fp16 tokens, 12 heads of 256 on 4,
+// 70 with four, 67 with sixteen. (Joined by the workgroup that is last to be done instead of a
 // launch: 6 to 12 us slower, by the fence that every workgroup then needs.)
 template <int THREADS>
 __device__ __forceinline__ void join_body(const PAttnArgs& a) {
@@ -936,11 +938,11 @@ __device__ __forceinline__ void move_rows(const PEvictArgs& a, const uint32_t* t
 // there. Few moves (SLM_MOVES_HERE) are made here, more by a launch of their own.
 //
 // Bound by the chain of its steps, a barrier each (one sequence of 1040 tokens, 4 heads: 7 us; 32
-// of up to 4200, 4 heads, of which up to 199 move: 14; 12 of 16384, 12 heads: 27), and past `room` by one
+// of up to 4200, 4 heads, of which up to 199 move: 12.5; 12 of 16384, 12 heads: 22), and past `room` by one
 // compute unit's reading of the weights, five to eight times over: one sequence of 36000 tokens cut
-// to 30000 takes 60 us, of 40000 149. Measured for the moves: 32 sequences, up to 250 moves, here
-// 17.5 us against 20.3 by a launch; one sequence, 500 moves, 15.7 here, 14.1 by a launch; 900,
-// 18.9 and 14.9.
+// to 30000 takes 43 us, of 40000 149. Measured for the moves: 32 sequences, up to 250 moves, here
+// 15.9 us against 18.9 by a launch; one sequence, 500 moves, 14.1 here, 12.8 by a launch; 900,
+// 17.1 and 13.4; but 32 sequences, 500 moves, 21.7 and 24.2.
 KERNEL void __launch_bounds__(1024) slm_paged_select(PEvictArgs a) {
     __shared__ uint32_t hist[2048];
     __shared__ uint32_t red[6][16];
