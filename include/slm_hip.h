@@ -236,6 +236,40 @@ int slm_hip_paged_attend(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, f
  * stay as they were). SLM_E_INVALID where a page is in the table twice. */
 int slm_hip_paged_evict(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* mass_out, uint32_t* born_out,
                         size_t keep, size_t recent);
+/* The batch's new tokens as a tree, until the batch is set anew: parent[row] (rows as paged_store takes
+ * them, the sequences' new tokens one after another) is the place among its sequence's new tokens of the
+ * one that a token follows, which lies before it, or SLM_NO_PARENT for one that follows the old tokens.
+ * ids (NULL: none, and no slm_hip_verify): the tokens. Host arrays, copied. At most 256 new tokens in a
+ * sequence (SLM_E_UNSUPPORTED). A step being recorded runs what it holds first. */
+#define SLM_NO_PARENT 0xffffffffu
+int slm_hip_seqs_tree(slm_hip* ctx, slm_seqs* seqs, const uint32_t* parent, const uint32_t* ids);
+/* Softmax attention of all new tokens, which paged_store has put into the pages: q and y are
+ * [rows][heads][dh], the sequences' new tokens one after another; query head h reads key head h / (heads /
+ * key_heads). A token of position p sees those of its own sequence at p − reach + 1 to p − gap (reach
+ * SIZE_MAX: all from the first on; never one behind its own): positions of old tokens by `born` where the
+ * cache has it, else slot t holds position t; new ones follow them in order. A token that sees none gets zeros.
+ * What of a page is not seen may hold anything. Rows of y behind the last new token stay as they were. Scores,
+ * weights and sums are fp32, in fp16 mode too; y is rounded there as slm_hip_attend rounds it. The slots are
+ * cut into stretches by the whole batch's work: a sequence's last bits may differ in another batch. */
+int slm_hip_paged_prompt(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* y, const float* q, size_t heads,
+                         size_t reach, size_t gap, float scale);
+/* The same for a tree of drafted tokens (slm_hip_seqs_tree): a token sees, of the new ones, itself and those
+ * that it comes from, and its position is the old tokens' end plus its depth (0 without a parent). */
+int slm_hip_paged_tree(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* y, const float* q, size_t heads,
+                       size_t reach, size_t gap, float scale);
+/* The tree against the logits of its tokens ([rows][vocab]): greedy, by slm_hip_argmax's order. A sequence's
+ * first new token is one that was picked before; from it the path goes on to the first of a token's children
+ * that is its pick. count[b]: the tokens of the path, the first among them (0: no new tokens); path[rows]:
+ * their places among the sequence's new tokens, in order, 0xffffffff behind them; next[b]: the pick of the
+ * last (0xffffffff: no new tokens). Fewer than 2^22 rows of up to 2^28 logits (SLM_E_UNSUPPORTED past that). */
+int slm_hip_verify(slm_hip* ctx, slm_seqs* seqs, uint32_t* count, uint32_t* path, uint32_t* next, const float* logits,
+                   size_t vocab);
+/* The path's keys, values and mass (where the cache has it) into the first slots of the sequence's new tokens:
+ * slot i gets what slot path[i] holds, i < count[b] (device memory, as slm_hip_verify writes it; a path that
+ * does not rise, or leaves the new tokens, ends there). Their `born` is the slots' own already. The
+ * other slots stay as they were; the caller then sets the batch's lengths to the old tokens and count[b].
+ * SLM_E_INVALID where a page that takes new tokens is in the table twice. */
+int slm_hip_paged_keep(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, const uint32_t* count, const uint32_t* path);
 /* What rows of logits x ([m][n]) say of given tokens (beside slm_hip_argmax; sample.rs keeps no
  * probabilities): lp[i] = x[i][ids[i]] − log Σ e^x[i]; entropy[i] = −Σ p log p in nats (NULL:
  * none); and the `top` (0 to 32, at most n) likeliest tokens with their log probabilities,

@@ -129,6 +129,11 @@ _SIGS = {
     "slm_hip_paged_store": (_i, [_p, _p, C.POINTER(Pages), _p, _p]),
     "slm_hip_paged_attend": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _p, _sz, _sz, _f]),
     "slm_hip_paged_evict": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _sz, _sz]),
+    "slm_hip_seqs_tree": (_i, [_p, _p, _u32p, _u32p]),
+    "slm_hip_paged_prompt": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _sz, _sz, _sz, _f]),
+    "slm_hip_paged_tree": (_i, [_p, _p, C.POINTER(Pages), _p, _p, _sz, _sz, _sz, _f]),
+    "slm_hip_verify": (_i, [_p, _p, _p, _p, _p, _p, _sz]),
+    "slm_hip_paged_keep": (_i, [_p, _p, C.POINTER(Pages), _p, _p]),
     "slm_hip_logprobs": (_i, [_p, _p, _p, _p, _p, _sz, _p, _u32p, _sz, _sz]),
     "slm_model_load": (_i, [_p, C.c_char_p, C.POINTER(_p)]),
     "slm_model_free": (None, [_p]),
@@ -417,6 +422,23 @@ class Hip:
     def paged_evict(self, seqs: "Seqs", pages: Pages, mass_out, born_out, keep, recent):
         self.check(lib.slm_hip_paged_evict(self.ctx, seqs.h, C.byref(pages), mass_out, born_out, keep, recent))
 
+    def paged_prompt(self, seqs: "Seqs", pages: Pages, y, q, heads, scale, reach=None, gap=0):
+        """All new tokens of the batch; reach None: from the first token on."""
+        self.check(lib.slm_hip_paged_prompt(self.ctx, seqs.h, C.byref(pages), y, q, heads,
+                                            USIZE_MAX if reach is None else reach, gap, scale))
+
+    def paged_tree(self, seqs: "Seqs", pages: Pages, y, q, heads, scale, reach=None, gap=0):
+        """The same for the drafted tokens of Seqs.tree."""
+        self.check(lib.slm_hip_paged_tree(self.ctx, seqs.h, C.byref(pages), y, q, heads,
+                                          USIZE_MAX if reach is None else reach, gap, scale))
+
+    def verify(self, seqs: "Seqs", count, path, next, logits, vocab):
+        """The drafted tokens of Seqs.tree against their logits."""
+        self.check(lib.slm_hip_verify(self.ctx, seqs.h, count, path, next, logits, vocab))
+
+    def paged_keep(self, seqs: "Seqs", pages: Pages, count, path):
+        self.check(lib.slm_hip_paged_keep(self.ctx, seqs.h, C.byref(pages), count, path))
+
     def logprobs(self, lp, x, ids, n, entropy=None, top=0, top_ids=None, top_lp=None):
         """x: rows of n logits, one a token of ids."""
         ids = np.ascontiguousarray(ids, dtype=np.uint32)
@@ -453,7 +475,7 @@ class Seqs:
     """A batch of sequences over paged caches (slm_seqs)."""
 
     def __init__(self, hip: Hip, page: int, max_n: int, max_pages: int):
-        self.hip, self.page, self.h = hip, page, None
+        self.hip, self.page, self.h, self.rows = hip, page, None, 0
         h = _p()
         hip.check(lib.slm_hip_seqs_new(hip.ctx, page, max_n, max_pages, C.byref(h)))
         self.h = h.value
@@ -470,6 +492,16 @@ class Seqs:
             raise ValueError(f"seqs: arrays of {n} sequences are wanted")
         self.hip.check(lib.slm_hip_seqs_set(self.hip.ctx, self.h, n, *(None if a is None else _up(a) for a in (
             lens, fresh, seen)), _up(table), width))
+        self.rows = n - int((lens == 0).sum()) if fresh is None else int(fresh.sum())
+
+    def tree(self, parent, ids=None):
+        """The new tokens as a tree: parent [rows], the place among the sequence's new tokens of the one that
+        each follows (-1: the old tokens); ids [rows]: the tokens, for verify."""
+        parent = np.ascontiguousarray(np.asarray(parent, dtype=np.int64).astype(np.int32)).view(np.uint32)
+        ids = None if ids is None else np.ascontiguousarray(ids, dtype=np.uint32)
+        if parent.shape != (self.rows,) or (ids is not None and ids.shape != parent.shape):
+            raise ValueError(f"tree: arrays of {self.rows} new tokens are wanted")
+        self.hip.check(lib.slm_hip_seqs_tree(self.hip.ctx, self.h, _up(parent), None if ids is None else _up(ids)))
 
     def free(self):
         if self.h and self.hip.ctx:

@@ -11,6 +11,7 @@
 #define SLM_TOP_MAX 32      // alternatives of a row of logits
 #define SLM_FEW_IDS 256     // tokens that go to the kernel with its arguments
 #define SLM_NO_SEQ 0xffffffffu
+#define SLM_TREE_MAX 256    // drafted tokens of a sequence
 
 // A batch of sequences on the device (slm_seqs).
 struct SeqsDev {
@@ -86,6 +87,46 @@ struct LogpArgs {
     float* part_sums;        // [m][parts][4]
     uint64_t* part_top;      // [m][parts][top], best first
     uint32_t few[SLM_FEW_IDS];  // up to this many rows' tokens, outside a recorded step
+};
+
+// Attention of several new tokens a sequence. An item: sequence (SLM_NO_SEQ: none), first row, rows, the slots from and
+// to, the place of its part in the workspace (SLM_NO_SEQ: none, it has all of its rows' slots). A job: the items of
+// one tile of rows, joined: sequence, first row, rows, the first one's place, their number.
+struct SpanArgs {
+    SeqsDev s;
+    float* y;                // [rows][heads][dh]
+    const float* q;
+    const void *k, *v;
+    const uint32_t* born;    // positions, or null: slot t holds position t
+    const uint32_t *up, *depth;  // a tree's: [rows][words] the bits of the tokens that a row's comes from, its own among them; depths; or null
+    const uint32_t *items, *jobs;  // [..][8]
+    float* ml;               // [places][kh][most][2]
+    float* po;               // [places][kh][most][dh]
+    int32_t heads, group, kh, page, dh;
+    uint32_t gap, back;      // seen: what lies gap to back positions before the row
+    uint32_t page_mul, page_shift, g_mul, g_shift;  // divisions by page and group
+    int32_t words, most;     // most: rows of an item
+    int32_t lanes;           // of the join: threads of a row, a power of two >= dh / 4
+    float scale;             // times log2 e
+    int32_t r16;             // fp16 mode: y rounded to fp16
+};
+
+struct VerifyArgs {
+    SeqsDev s;
+    const float* x;          // [rows][vocab]
+    const uint32_t *parent, *ids;  // [rows]
+    uint32_t *count, *path, *next;  // [n], [rows], [n]
+    uint64_t* best;          // [rows][parts]
+    int64_t vocab, span;     // a part's logits
+    int32_t parts;
+};
+
+struct KeepArgs {
+    SeqsDev s;
+    void *k, *v;
+    float* mass;             // or null
+    const uint32_t *count, *path;
+    int32_t kh, page, bytes; // of a row
 };
 
 #endif

@@ -1540,3 +1540,5 @@ KERNEL void __launch_bounds__(256) slm_logprobs_join(LogpArgs a) {
         }
     }
 }
+
+#include "spans.inc"

@@ -66,7 +66,8 @@ constexpr int64_t EVICT_ROOM = 36352;       // slots whose keys an eviction's wo
 enum OpKind : uint32_t {
     OP_GATHER = 1, OP_COPY, OP_SHIFT, OP_COLUMNS, OP_LINEAR, OP_ADD, OP_ADD_ROW, OP_SCALE_ROWS,
     OP_MIX, OP_RMS, OP_SILU_MUL, OP_ROPE_TABLE, OP_ROPE, OP_L2NORM, OP_GLA, OP_STORE, OP_ATTEND,
-    OP_ARGMAX, OP_GROW, OP_PSTORE, OP_PATTEND, OP_PEVICT, OP_LOGPROBS
+    OP_ARGMAX, OP_GROW, OP_PSTORE, OP_PATTEND, OP_PEVICT, OP_LOGPROBS,
+    OP_PSPAN, OP_VERIFY, OP_PKEEP
 };
 
 // One operation, by value. p[] are device pointers (outputs first), n[] sizes, f[]
@@ -156,7 +157,31 @@ struct Kernels {
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
     hipFunction_t pstore[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
+    // several new tokens a sequence (spans.inc): fp32 and fp16 pages; head sizes to 32, 64, 128, 256; many rows and few
+    hipFunction_t span[2][4][2], span_join[2], tree_pick, tree_walk, tree_keep[2];
 };
+
+// A block of device memory that host arrays go up into, through two pinned uploads in turn.
+struct Upload {
+    unsigned char* dev = nullptr;
+    size_t bytes = 0;
+    unsigned char* pin[2] = {nullptr, nullptr};
+    hipEvent_t ev[2] = {nullptr, nullptr};
+    int flip = 0;
+};
+
+// How an attention of a batch's new tokens is cut into workgroups (SpanArgs' items and jobs), kept until the batch
+// is set anew: a model's layers of one kind share it.
+struct SpanPlan {
+    size_t group = 0, heads = 0;
+    int64_t most = 0;
+    uint32_t gap = 0, back = 0;
+    bool born = false, tree = false, valid = false;
+    Upload up;
+    size_t items = 0, jobs = 0, slots = 0, longest = 0;  // counts of the launches; a job's most items
+    uint64_t used = 0;
+};
+constexpr size_t SPAN_PLANS = 8;          // of a batch at a time
 
 }  // namespace
 
@@ -174,8 +199,15 @@ struct slm_seqs {
     bool shared = false;        // a page that two places of the table name
     bool fresh_shared = false;  // ... and new tokens go into
     bool each = false;          // one new token in every sequence
-    std::vector<uint32_t> len;
+    std::vector<uint32_t> len, fresh;
     std::vector<uint8_t> uses;  // per page, while a table is read
+    // the new tokens as a tree (slm_hip_seqs_tree): parents, tokens and depths of the rows, then each row's line as bits
+    Upload tree;
+    bool has_tree = false, has_ids = false;
+    uint32_t words = 0;               // 32-bit words of a row's line
+    std::vector<uint32_t> deepest;    // per sequence
+    std::vector<SpanPlan> plans;
+    uint64_t clock = 0;
     size_t at_seen() const { return 4 * max_n; }
     size_t at_first() const { return 8 * max_n; }
     size_t at_ifirst() const { return 12 * max_n + 4; }
@@ -919,6 +951,90 @@ int64_t logp_span(int64_t n, int64_t parts) {
     return (panels + parts - 1) / parts * LOGP_SHORT;
 }
 
+// Attention of several new tokens a sequence: rows of an item, by head size and whether the rows are few (a sequence has
+// at most SPAN_FEW under a key head); the slots of a stretch are a multiple of SPAN_STEP.
+constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128;
+int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
+int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
+// LDS: a tile's keys, values and positions; where waves share rows, their parts as they are joined.
+int64_t span_lds(int64_t dh, bool half, bool few) {
+    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = few ? (half ? 128 : 64) : dp * unit <= 256 ? 64 : 32;
+    const int64_t tile = kt * (dp + 16 / unit) * unit * 2 + kt * 4, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
+    return std::max(tile, join);
+}
+size_t span_ml(size_t slots, size_t kh, size_t most) { return slots * kh * most * 2; }  // (whole 16 bytes: most is even)
+
+// n / d for n < 2^31 as span_div makes it.
+void span_divisor(uint32_t d, uint32_t* mul, uint32_t* shift) {
+    uint32_t s = 0;
+    while (((uint64_t)1 << s) < d) s++;
+    *shift = s;
+    *mul = (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d);
+}
+
+// n0 n, n1 rows, n9 width; p6 the batch's block
+int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
+    const Kernels& k = c->k;
+    const float* const* p = o.p;
+    const int64_t* n = o.n;
+    auto it = c->seqs.find((uintptr_t)p[6]);
+    if (it == c->seqs.end()) return fail(c, SLM_E_INVALID, "paged: the batch is gone");
+    const SeqsDev s = seqs_dev(it->second, n[0], n[9]);
+    if (o.kind == OP_VERIFY) {  // p0 count, p1 path, p2 next, p3 logits, p4 parents, p5 tokens; n2 vocab, n3 parts, n4 a part's logits
+        VerifyArgs a{s, p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], (uint32_t*)p[0], (uint32_t*)p[1], (uint32_t*)p[2],
+                     (uint64_t*)c->pws, n[2], n[4], (int32_t)n[3]};
+        if (n[1]) out.push_back(mk_desc(k.tree_pick, (uint32_t)(n[1] * n[3]), 256, 0, a));
+        out.push_back(mk_desc(k.tree_walk, (uint32_t)n[0], SLM_TREE_MAX, 0, a));
+        return SLM_OK;
+    }
+    if (o.kind == OP_PKEEP) {  // p0 k, p1 v, p2 mass, p3 count, p4 path; n2 kh, n3 page, n4 dh, n5 pages, n6 fp16
+        KeepArgs a{s, (void*)p[0], (void*)p[1], (float*)p[2], (const uint32_t*)p[3], (const uint32_t*)p[4],
+                   (int32_t)n[2], (int32_t)n[3], (int32_t)(n[4] * (n[6] ? 2 : 4))};
+        out.push_back(mk_desc(k.tree_keep[a.bytes % 16 != 0], (uint32_t)(n[0] * n[2]), 256, 0, a));
+        return SLM_OK;
+    }
+    // p0 y, p1 q, p2 k, p3 v, p4 born, p5 the plan, p7 the tree; n2 heads and key heads, n3 page and head size, n4 gap and
+    // back, n5 pages, n6 fp16, few rows, wide join, a line's words; n7 items and jobs, n8 places; f0 scale
+    SpanArgs a{};
+    a.s = s;
+    a.y = (float*)p[0];
+    a.q = p[1];
+    a.k = p[2];
+    a.v = p[3];
+    a.born = (const uint32_t*)p[4];
+    a.heads = (int32_t)(n[2] & 0xffffffff);
+    a.kh = (int32_t)(n[2] >> 32);
+    a.group = a.heads / a.kh;
+    a.page = (int32_t)(n[3] & 0xffffffff);
+    a.dh = (int32_t)(n[3] >> 32);
+    a.gap = (uint32_t)(n[4] & 0xffffffff);
+    a.back = (uint32_t)((uint64_t)n[4] >> 32);
+    const bool half = n[6] & 1, few = n[6] & 2, wide = n[6] & 4;
+    a.words = (int32_t)(n[6] >> 8);
+    if (p[7]) {
+        a.depth = (const uint32_t*)p[7] + 2 * n[1];
+        a.up = a.depth + n[1];
+    }
+    const int64_t items = n[7] & 0xffffffff, jobs = n[7] >> 32;
+    a.items = (const uint32_t*)p[5];
+    a.jobs = a.items + 8 * items;
+    a.most = (int32_t)span_rows(a.dh, few);
+    a.ml = c->pws;
+    a.po = a.ml + span_ml((size_t)n[8], (size_t)a.kh, (size_t)a.most);
+    span_divisor((uint32_t)a.page, &a.page_mul, &a.page_shift);
+    span_divisor((uint32_t)a.group, &a.g_mul, &a.g_shift);
+    a.lanes = 1;
+    while (a.lanes * 4 < a.dh) a.lanes *= 2;
+    a.scale = o.f[0];
+    a.r16 = c->fp16 ? 1 : 0;
+    out.push_back(mk_desc(k.span[half][span_class(a.dh)][few], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, few), a));
+    if (jobs) {
+        const int64_t each = wide ? 1 : 256 / a.lanes;
+        out.push_back(mk_desc(k.span_join[wide], (uint32_t)(jobs * a.kh * ((a.most + each - 1) / each)), 256, 0, a));
+    }
+    return SLM_OK;
+}
+
 int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const Kernels& k = c->k;
     const float* const* p = o.p;
@@ -952,6 +1068,7 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
         out.back().abytes = bytes;
         return SLM_OK;
     }
+    if (o.kind == OP_PSPAN || o.kind == OP_VERIFY || o.kind == OP_PKEEP) return lower_spans(c, o, out);
     if (o.kind != OP_PSTORE && o.kind != OP_PATTEND && o.kind != OP_PEVICT)
         return fail(c, SLM_E_INVALID, "unknown op %u", o.kind);
     const void* dev = o.kind == OP_PSTORE ? p[6] : p[o.kind == OP_PATTEND ? 7 : 6];
@@ -1326,6 +1443,28 @@ void op_ranges(const Op& o, std::vector<Range>& rd, std::vector<Range>& wr) {
             for (int q = 0; q < 2; q++) slots(p[q], ring_floats(sl * n[4], n[6]));
             for (int q = 2; q < 4; q++) slots(p[q], sl);
             for (int q = 4; q < 6; q++) rd.push_back(rng(p[q], sl));
+            break;
+        }
+        case OP_PSPAN: {
+            const int64_t heads = n[2] & 0xffffffff, kh = n[2] >> 32, page = n[3] & 0xffffffff, dh = n[3] >> 32;
+            wr.push_back(rng(p[0], n[1] * heads * dh));
+            rd.push_back(rng(p[1], n[1] * heads * dh));
+            for (int q = 2; q < 4; q++) rd.push_back(rng(p[q], ring_floats(n[5] * kh * page * dh, n[6] & 1)));
+            if (p[4]) rd.push_back(rng(p[4], n[5] * kh * page));
+            break;
+        }
+        case OP_VERIFY:
+            wr.push_back(rng(p[0], n[0]));
+            wr.push_back(rng(p[1], n[1]));
+            wr.push_back(rng(p[2], n[0]));
+            rd.push_back(rng(p[3], n[1] * n[2]));
+            break;
+        case OP_PKEEP: {
+            int64_t sl = n[5] * n[2] * n[3];
+            for (int q = 0; q < 2; q++) slots(p[q], ring_floats(sl * n[4], n[6]));
+            slots(p[2], sl);
+            rd.push_back(rng(p[3], n[0]));
+            rd.push_back(rng(p[4], n[1]));
             break;
         }
         case OP_LOGPROBS:
@@ -3199,8 +3338,61 @@ int need_pws(slm_hip* c, size_t bytes) {
     return SLM_OK;
 }
 
+void upload_free(slm_hip* c, Upload& u) {
+    if (u.dev) dev_free(c, u.dev);
+    for (int i = 0; i < 2; i++) {
+        if (u.pin[i]) hipHostFree(u.pin[i]);
+        if (u.ev[i]) hipEventDestroy(u.ev[i]);
+    }
+    u = Upload{};
+}
+
+// Room for `bytes`, and the pinned memory to fill (nothing queued reads it any more). What the block held is gone.
+int upload_begin(slm_hip* c, Upload& u, size_t bytes, unsigned char** fill) {
+    if (bytes > u.bytes) {
+        const size_t room = std::max(bytes, u.bytes * 2);
+        unsigned char* pin[2] = {nullptr, nullptr};
+        hipError_t e = hipSuccess;
+        for (int i = 0; i < 2 && e == hipSuccess; i++) {
+            e = hipHostMalloc((void**)&pin[i], room, hipHostMallocDefault);
+            if (e == hipSuccess && !u.ev[i]) e = hipEventCreateWithFlags(&u.ev[i], hipEventDisableTiming);
+            if (e == hipSuccess) e = hipEventSynchronize(u.ev[i]);
+        }
+        int rc = SLM_OK;
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            rc = fail(c, SLM_E_MEMORY, "%zu bytes of a batch: %s", room, hipGetErrorString(e));
+        } else {
+            rc = internal_realloc(c, (void**)&u.dev, room);
+        }
+        if (rc) {
+            for (auto* q : pin)
+                if (q) hipHostFree(q);
+            return rc;
+        }
+        for (int i = 0; i < 2; i++) {
+            if (u.pin[i]) hipHostFree(u.pin[i]);
+            u.pin[i] = pin[i];
+        }
+        u.bytes = room;
+    }
+    u.flip ^= 1;
+    HIPC(c, hipEventSynchronize(u.ev[u.flip]));
+    *fill = u.pin[u.flip];
+    return SLM_OK;
+}
+
+int upload_send(slm_hip* c, Upload& u, size_t bytes) {
+    hipStream_t st = mstream(c);
+    HIPC(c, hipMemcpyAsync(u.dev, u.pin[u.flip], bytes, hipMemcpyHostToDevice, st));
+    HIPC(c, hipEventRecord(u.ev[u.flip], st));
+    return SLM_OK;
+}
+
 // A batch's memory (nothing queued may still use it).
 void free_seqs(slm_hip* c, slm_seqs* s) {
+    upload_free(c, s->tree);
+    for (auto& p : s->plans) upload_free(c, p.up);
     if (s->dev && c->pooled.count((uintptr_t)s->dev)) dev_free(c, s->dev);
     else if (s->dev) hipFree(s->dev);
     for (int i = 0; i < 2; i++) {
@@ -3899,6 +4091,17 @@ int load_kernels(slm_hip* c) {
         return (int)SLM_OK;
     };
     for (auto& f : batch) TRY(get_batch(f.f, f.n));
+    TRY(get_batch(&k.span_join[0], "slm_span_join"));
+    TRY(get_batch(&k.span_join[1], "slm_span_join_wide"));
+    TRY(get_batch(&k.tree_pick, "slm_tree_pick"));
+    TRY(get_batch(&k.tree_walk, "slm_tree_walk"));
+    TRY(get_batch(&k.tree_keep[0], "slm_tree_keep16"));
+    TRY(get_batch(&k.tree_keep[1], "slm_tree_keep8"));
+    for (int half = 0; half < 2; half++)
+        for (int t = 0; t < 4; t++)
+            for (int few = 0; few < 2; few++)
+                TRY(get_batch(&k.span[half][t][few], std::string("slm_span") + (half ? "16_" : "_") + std::to_string(32 << t) +
+                                                         (few ? "_1" : "_4")));
     for (int half = 0; half < 2; half++)
         for (int t = 0; t < 3; t++)
             for (int m = 0; m < 5; m++)
@@ -5157,6 +5360,7 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     try {  // (a byte a page)
         s->uses.assign(n ? max_page + 1 : 0, 0);
         s->len.reserve(n);
+        s->fresh.reserve(n);
     } catch (const std::bad_alloc&) {
         return fail(c, SLM_E_MEMORY, "seqs_set: page %u", max_page);
     }
@@ -5214,6 +5418,8 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     for (size_t i = items; i < all; i++) ht[4 * i] = SLM_NO_SEQ;
     hipStream_t st = mstream(c);
     s->n = 0;  // (nothing until both copies are queued)
+    s->has_tree = false;
+    for (auto& p : s->plans) p.valid = false;
     HIPC(c, hipMemcpyAsync(s->dev, h, s->at_items() + 16 * all, hipMemcpyHostToDevice, st));
     if (n) HIPC(c, hipMemcpyAsync(s->dev + s->at_table(), hp, 4 * n * w, hipMemcpyHostToDevice, st));
     HIPC(c, hipEventRecord(s->ev[k], st));
@@ -5225,6 +5431,8 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     s->max_len = max_len;
     s->max_page = max_page;
     s->len.assign(len, len + n);
+    s->fresh.resize(n);
+    for (size_t b = 0; b < n; b++) s->fresh[b] = fresh_of(b);
     return SLM_OK;
 }
 
@@ -5372,6 +5580,325 @@ int slm_hip_paged_evict(slm_hip* c, slm_seqs* s, const slm_pages* g, float* mass
     return submit(c, o);
 }
 
+int slm_hip_seqs_tree(slm_hip* c, slm_seqs* s, const uint32_t* parent, const uint32_t* ids) {
+    if (!c || !s) return SLM_E_INVALID;
+    bool live = false;
+    for (auto& q : c->seqs) live = live || q.second == s;
+    if (!live) return fail(c, SLM_E_INVALID, "seqs_tree: not a batch of this context");
+    TRY(refuse_capture(c, "seqs_tree"));
+    if (s->rows && !parent) return SLM_E_INVALID;
+    uint32_t most = 0;
+    for (uint32_t f : s->fresh) most = std::max(most, f);
+    if (most > SLM_TREE_MAX)
+        return fail(c, SLM_E_UNSUPPORTED, "seqs_tree: %u drafted tokens in a sequence (at most %d)", most, SLM_TREE_MAX);
+    const uint32_t* at = parent;
+    for (size_t b = 0; b < s->n; at += s->fresh[b++])
+        for (uint32_t i = 0; i < s->fresh[b]; i++)
+            if (at[i] != SLM_NO_PARENT && at[i] >= i)
+                return fail(c, SLM_E_INVALID, "seqs_tree: token %u of sequence %zu follows token %u", i, b, at[i]);
+    TRY(taint(c));  // a step's calls recorded so far run with the tree as it was
+    const size_t rows = s->rows, words = std::max<size_t>(1, (most + 31) / 32), bytes = std::max<size_t>(1, rows) * (3 + words) * 4;
+    std::vector<uint32_t> deepest;
+    try {
+        deepest.assign(s->n, 0);
+    } catch (const std::bad_alloc&) {
+        return fail(c, SLM_E_MEMORY, "seqs_tree: %zu sequences", s->n);
+    }
+    unsigned char* fill = nullptr;
+    s->has_tree = false;
+    for (auto& p : s->plans) p.valid = p.valid && !p.tree;
+    TRY(upload_begin(c, s->tree, bytes, &fill));
+    uint32_t *hp = (uint32_t*)fill, *hi = hp + rows, *hd = hi + rows, *hu = hd + rows;
+    if (rows) {
+        std::memcpy(hp, parent, rows * 4);
+        if (ids) std::memcpy(hi, ids, rows * 4);
+        else std::memset(hi, 0, rows * 4);
+    }
+    std::memset(hu, 0, rows * words * 4);
+    size_t row = 0;
+    for (size_t b = 0; b < s->n; row += s->fresh[b++])
+        for (uint32_t i = 0; i < s->fresh[b]; i++) {
+            const uint32_t from = parent[row + i];
+            uint32_t* line = hu + (row + i) * words;
+            hd[row + i] = 0;
+            if (from != SLM_NO_PARENT) {
+                hd[row + i] = hd[row + from] + 1;
+                std::memcpy(line, hu + (row + from) * words, words * 4);
+            }
+            line[i / 32] |= 1u << (i % 32);
+            deepest[b] = std::max(deepest[b], hd[row + i]);
+        }
+    TRY(upload_send(c, s->tree, bytes));
+    s->words = (uint32_t)words;
+    s->has_ids = ids != nullptr;
+    s->deepest.swap(deepest);
+    s->has_tree = true;
+    return SLM_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Cuts the new tokens' rows and the slots that they see into items: rows in tiles of `most` at most, of about one size;
+// slots in stretches of one length for the whole batch, such that there are about SPAN_ITEMS workgroups, each of SPAN_STEP
+// slots at least. The longest go first.
+constexpr uint64_t SPAN_ITEMS = 1024;
+int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan** out) {
+    SpanPlan* p = nullptr;
+    for (auto& q : s->plans)
+        if (q.valid && q.group == want.group && q.heads == want.heads && q.most == want.most && q.gap == want.gap &&
+            q.back == want.back && q.born == want.born && q.tree == want.tree)
+            p = &q;
+    if (p) {
+        p->used = ++s->clock;
+        *out = p;
+        return SLM_OK;
+    }
+    struct Tile {
+        uint32_t b, row, rows, lo, hi;
+    };
+    struct Item {
+        uint32_t v[8];
+    };
+    std::vector<Item> items, jobs;
+    size_t slots = 0, longest = 0;
+    try {
+        std::vector<Tile> tiles;
+        uint64_t work = 0;
+        for (size_t b = 0; b < s->n; b++) {
+            const uint64_t f = s->fresh[b], old = s->len[b] - f, rows = f * want.group;
+            if (!rows) continue;
+            const uint64_t count = (rows + want.most - 1) / want.most;
+            const uint64_t each = ((rows + count - 1) / count + SPAN_FEW - 1) / SPAN_FEW * SPAN_FEW;
+            for (uint64_t at = 0; at < rows; at += each) {
+                const uint64_t n = std::min(each, rows - at), i0 = at / want.group, i1 = (at + n - 1) / want.group;
+                // the newest slot and the oldest that one of the rows sees
+                uint64_t hi = old + i1 + 1, lo = 0;
+                if (!want.born) {
+                    const uint64_t far = want.tree ? old + s->deepest[b] : old + i1, near = want.tree ? old : old + i0;
+                    if (!want.tree || want.gap > s->deepest[b]) hi = far + 1 > want.gap ? far + 1 - want.gap : 0;
+                    lo = near > want.back ? near - want.back : 0;
+                }
+                if (hi < lo) hi = lo;
+                tiles.push_back({(uint32_t)b, (uint32_t)at, (uint32_t)n, (uint32_t)lo, (uint32_t)hi});
+                work += hi - lo;
+            }
+        }
+        uint64_t stretch = std::max<uint64_t>(1, work * kh / SPAN_ITEMS);
+        stretch = (stretch + SPAN_STEP - 1) / SPAN_STEP * SPAN_STEP;
+        for (const Tile& t : tiles) {
+            const uint64_t n = t.hi - t.lo, parts = std::max<uint64_t>(1, (n + stretch - 1) / stretch);
+            const uint64_t each = ((n + parts - 1) / parts + SPAN_STEP - 1) / SPAN_STEP * SPAN_STEP;
+            const uint64_t used = std::max<uint64_t>(1, each ? (n + each - 1) / each : 1);
+            if (used > 1) jobs.push_back({{t.b, t.row, t.rows, (uint32_t)slots, (uint32_t)used, 0, 0, 0}});
+            longest = std::max<size_t>(longest, used > 1 ? used : 0);
+            for (uint64_t z = 0; z < used; z++)
+                items.push_back({{t.b, t.row, t.rows, (uint32_t)(t.lo + z * each), (uint32_t)std::min<uint64_t>(t.hi, t.lo + (z + 1) * each),
+                                  used > 1 ? (uint32_t)slots++ : SLM_NO_SEQ, 0, 0}});
+        }
+        std::stable_sort(items.begin(), items.end(), [](const Item& x, const Item& y) { return x.v[4] - x.v[3] > y.v[4] - y.v[3]; });
+        // (launches are sized by these counts, and a kept step is kept for its launches: they go up in steps)
+        const Item none = {{SLM_NO_SEQ, 0, 0, 0, 0, 0, 0, 0}};
+        auto pad = [&](std::vector<Item>& v) {
+            size_t step = 1;
+            while (step * 16 <= v.size()) step *= 2;
+            while (v.size() % step) v.push_back(none);
+        };
+        pad(items);
+        pad(jobs);
+        size_t step = 1;
+        while (step * 16 <= slots) step *= 2;
+        slots = (slots + step - 1) / step * step;
+        if (s->plans.size() < SPAN_PLANS) s->plans.reserve(SPAN_PLANS);
+    } catch (const std::bad_alloc&) {
+        return fail(c, SLM_E_MEMORY, "a batch's attention: %zu new tokens", s->rows);
+    }
+    if (items.size() * kh >= (size_t)1 << 22 || jobs.size() * kh * want.most >= (size_t)1 << 22)
+        return fail(c, SLM_E_UNSUPPORTED, "a batch's attention: %zu pieces of %zu key heads", items.size(), kh);
+    for (auto& q : s->plans)
+        if (!q.valid) p = &q;
+    if (!p && s->plans.size() < SPAN_PLANS) {
+        s->plans.emplace_back();
+        p = &s->plans.back();
+    }
+    if (!p) {
+        for (auto& q : s->plans)
+            if (!p || q.used < p->used) p = &q;
+        TRY(taint(c));  // a step's calls recorded so far run with this plan
+    }
+    unsigned char* fill = nullptr;
+    const size_t bytes = (items.size() + jobs.size()) * sizeof(Item);
+    p->valid = false;
+    TRY(upload_begin(c, p->up, bytes, &fill));
+    std::memcpy(fill, items.data(), items.size() * sizeof(Item));
+    if (jobs.size()) std::memcpy(fill + items.size() * sizeof(Item), jobs.data(), jobs.size() * sizeof(Item));
+    TRY(upload_send(c, p->up, bytes));
+    p->group = want.group;
+    p->heads = want.heads;
+    p->most = want.most;
+    p->gap = want.gap;
+    p->back = want.back;
+    p->born = want.born;
+    p->tree = want.tree;
+    p->items = items.size();
+    p->jobs = jobs.size();
+    p->slots = slots;
+    p->longest = longest;
+    p->used = ++s->clock;
+    p->valid = true;
+    *out = p;
+    return SLM_OK;
+}
+
+int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_pages* g, float* y, const float* q, size_t heads,
+               size_t reach, size_t gap, float scale) {
+    bool half = false;
+    size_t slots = 0;
+    TRY(check_pages(c, name, s, g, &half, &slots));
+    if (!heads || heads % g->key_heads)
+        return fail(c, SLM_E_INVALID, "%s: %zu heads over %zu key heads", name, heads, g->key_heads);
+    if (!reach) return fail(c, SLM_E_INVALID, "%s: a reach of 0", name);
+    if (tree && !s->has_tree) return fail(c, SLM_E_INVALID, "%s: the batch's new tokens are no tree (slm_hip_seqs_tree)", name);
+    if (!s->n || !s->rows) return SLM_OK;
+    uint64_t most = 0;
+    for (uint32_t f : s->fresh) most = std::max<uint64_t>(most, f);
+    const size_t group = heads / g->key_heads;
+    if (heads > 65536 || most * group >= (uint64_t)1 << 31)
+        return fail(c, SLM_E_UNSUPPORTED, "%s: %zu heads of %llu new tokens", name, heads, (unsigned long long)most);
+    const size_t n = s->rows * heads * g->dh;
+    NEED(c, name, y, n);
+    NEED(c, name, q, n);
+    if (!aligned16(q)) return fail(c, SLM_E_UNSUPPORTED, "%s: q must be 16-byte aligned", name);
+    if (meet(y, n * 4, q, n * 4) || meets_cache(g, slots, half, y, n * 4))
+        return fail(c, SLM_E_INVALID, "%s: y lies in an input", name);
+    const bool few = most * group <= (uint64_t)SPAN_FEW;
+    SpanPlan want;
+    want.group = group;
+    want.heads = heads;
+    want.most = span_rows((int64_t)g->dh, few);
+    want.gap = (uint32_t)std::min<size_t>(gap, UINT32_MAX);
+    want.back = (uint32_t)std::min<size_t>(reach - 1, UINT32_MAX);
+    want.tree = tree;
+    want.born = g->born && (want.gap || want.back != UINT32_MAX);  // (positions matter to these alone)
+    SpanPlan* plan = nullptr;
+    TRY(span_plan(c, s, want, g->key_heads, &plan));
+    if (plan->slots)
+        TRY(need_pws(c, (span_ml(plan->slots, g->key_heads, (size_t)want.most) + plan->slots * g->key_heads * want.most * g->dh) * 4));
+    Op o = op(OP_PSPAN);
+    o.p[0] = y;
+    o.p[1] = q;
+    o.p[2] = g->k;
+    o.p[3] = g->v;
+    o.p[4] = want.born ? (const float*)g->born : nullptr;
+    o.p[5] = (const float*)plan->up.dev;
+    o.p[6] = (const float*)s->dev;
+    o.p[7] = tree ? (const float*)s->tree.dev : nullptr;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)s->rows;
+    o.n[2] = (int64_t)(heads | g->key_heads << 32);
+    o.n[3] = (int64_t)(g->page | g->dh << 32);
+    o.n[4] = (int64_t)((uint64_t)want.gap | (uint64_t)want.back << 32);
+    o.n[5] = (int64_t)g->pages;
+    o.n[6] = (half ? 1 : 0) | (few ? 2 : 0) | (plan->longest > 8 ? 4 : 0) | (int64_t)(tree ? s->words : 0) << 8;
+    o.n[7] = (int64_t)((uint64_t)plan->items | (uint64_t)plan->jobs << 32);
+    o.n[8] = (int64_t)plan->slots;
+    o.n[9] = (int64_t)s->width;
+    // scores in powers of two (fp16 mode: the dtype's scalar first, as slm_hip_attend)
+    o.f[0] = (float)((double)(c->fp16 ? round16(scale) : scale) * 1.4426950408889634);
+    return submit(c, o);
+}
+
+}  // namespace
+
+extern "C" {
+
+int slm_hip_paged_prompt(slm_hip* c, slm_seqs* s, const slm_pages* g, float* y, const float* q, size_t heads, size_t reach,
+                         size_t gap, float scale) {
+    return attend_new(c, "paged_prompt", false, s, g, y, q, heads, reach, gap, scale);
+}
+
+int slm_hip_paged_tree(slm_hip* c, slm_seqs* s, const slm_pages* g, float* y, const float* q, size_t heads, size_t reach,
+                       size_t gap, float scale) {
+    return attend_new(c, "paged_tree", true, s, g, y, q, heads, reach, gap, scale);
+}
+
+int slm_hip_verify(slm_hip* c, slm_seqs* s, uint32_t* count, uint32_t* path, uint32_t* next, const float* logits, size_t vocab) {
+    if (!c || !s) return SLM_E_INVALID;
+    bool live = false;
+    for (auto& q : c->seqs) live = live || q.second == s;
+    if (!live) return fail(c, SLM_E_INVALID, "verify: not a batch of this context");
+    TRY(refuse_capture(c, "verify"));
+    if (!s->has_tree || !s->has_ids)
+        return fail(c, SLM_E_INVALID, "verify: the batch's new tokens are no tree of tokens (slm_hip_seqs_tree)");
+    if (!vocab) return fail(c, SLM_E_INVALID, "verify: rows of no logits");
+    if (!s->n) return SLM_OK;
+    if (vocab > (size_t)1 << 28 || s->rows >= (size_t)1 << 22)
+        return fail(c, SLM_E_UNSUPPORTED, "verify: %zu rows of %zu logits", s->rows, vocab);
+    NEED(c, "verify", (const float*)count, s->n);
+    NEED(c, "verify", (const float*)path, s->rows);
+    NEED(c, "verify", (const float*)next, s->n);
+    NEED(c, "verify", logits, s->rows * vocab);
+    const void* outs[3] = {count, path, next};
+    const size_t bytes[3] = {s->n * 4, s->rows * 4, s->n * 4};
+    for (int i = 0; i < 3; i++) {
+        bool bad = meet(outs[i], bytes[i], logits, s->rows * vocab * 4);
+        for (int j = 0; j < i; j++) bad = bad || meet(outs[i], bytes[i], outs[j], bytes[j]);
+        if (bad) return fail(c, SLM_E_INVALID, "verify: the outputs overlap each other or the logits");
+    }
+    const size_t rows = std::max<size_t>(1, s->rows), panels = (vocab + 2047) / 2048;
+    size_t parts = std::max<size_t>(1, std::min(panels, 1024 / rows));
+    const size_t span = (panels + parts - 1) / parts * 2048;
+    parts = (vocab + span - 1) / span;
+    TRY(need_pws(c, rows * parts * 8));
+    Op o = op(OP_VERIFY);
+    o.p[0] = (const float*)count;
+    o.p[1] = (const float*)path;
+    o.p[2] = (const float*)next;
+    o.p[3] = logits;
+    o.p[4] = (const float*)s->tree.dev;
+    o.p[5] = o.p[4] + s->rows;
+    o.p[6] = (const float*)s->dev;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)s->rows;
+    o.n[2] = (int64_t)vocab;
+    o.n[3] = (int64_t)parts;
+    o.n[4] = (int64_t)span;
+    o.n[9] = (int64_t)s->width;
+    return submit(c, o);
+}
+
+int slm_hip_paged_keep(slm_hip* c, slm_seqs* s, const slm_pages* g, const uint32_t* count, const uint32_t* path) {
+    bool half = false;
+    size_t slots = 0;
+    TRY(check_pages(c, "paged_keep", s, g, &half, &slots));
+    if (!s->n || !s->rows) return SLM_OK;
+    NEED(c, "paged_keep", (const float*)count, s->n);
+    NEED(c, "paged_keep", (const float*)path, s->rows);
+    if (meets_cache(g, slots, half, count, s->n * 4) || meets_cache(g, slots, half, path, s->rows * 4))
+        return fail(c, SLM_E_INVALID, "paged_keep: the path lies in the cache");
+    if (s->fresh_shared)
+        return fail(c, SLM_E_INVALID, "paged_keep: a page that takes new tokens is in the table twice");
+    if (s->n * g->key_heads >= (size_t)1 << 22)
+        return fail(c, SLM_E_UNSUPPORTED, "paged_keep: %zu sequences of %zu key heads", s->n, g->key_heads);
+    Op o = op(OP_PKEEP);
+    o.p[0] = g->k;
+    o.p[1] = g->v;
+    o.p[2] = g->mass;
+    o.p[3] = (const float*)count;
+    o.p[4] = (const float*)path;
+    o.p[6] = (const float*)s->dev;
+    o.n[0] = (int64_t)s->n;
+    o.n[1] = (int64_t)s->rows;
+    o.n[2] = (int64_t)g->key_heads;
+    o.n[3] = (int64_t)g->page;
+    o.n[4] = (int64_t)g->dh;
+    o.n[5] = (int64_t)g->pages;
+    o.n[6] = half;
+    o.n[9] = (int64_t)s->width;
+    return submit(c, o);
+}
+
 int slm_hip_logprobs(slm_hip* c, float* lp, float* entropy, uint32_t* top_ids, float* top_lp, size_t top, const float* x,
                      const uint32_t* ids, size_t m, size_t n) {
     if (!c || (m && !ids)) return SLM_E_INVALID;
@@ -5449,7 +5976,11 @@ int slm_hip_mem_info(slm_hip* c, size_t* free_bytes, size_t* total_bytes, size_t
     direct(c->part, c->part_bytes);
     direct(c->gpart, c->gpart_bytes);
     direct(c->pws, c->pws_bytes);
-    for (auto& q : c->seqs) direct(q.second->dev, q.second->bytes());
+    for (auto& q : c->seqs) {
+        direct(q.second->dev, q.second->bytes());
+        direct(q.second->tree.dev, q.second->tree.bytes);
+        for (auto& p : q.second->plans) direct(p.up.dev, p.up.bytes);
+    }
     *held_bytes = held;
     return SLM_OK;
 }
