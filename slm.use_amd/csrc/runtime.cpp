@@ -956,10 +956,12 @@ int64_t logp_span(int64_t n, int64_t parts) {
 constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128;
 int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
 int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
-// LDS: a tile's keys, values and positions; where waves share rows, their parts as they are joined.
+// LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
+// largest; where waves share rows, their parts as they are joined.
 int64_t span_lds(int64_t dh, bool half, bool few) {
-    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = few ? (half ? 128 : 64) : dp * unit <= 256 ? 64 : 32;
-    const int64_t tile = kt * (dp + 16 / unit) * unit * 2 + kt * 4, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
+    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = few ? (half ? 128 : 64) : dp <= 64 ? 64 : 32;
+    const int64_t row = !half && !few ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
+    const int64_t tile = kt * row * 2 + kt * 4 + 64, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
     return std::max(tile, join);
 }
 size_t span_ml(size_t slots, size_t kh, size_t most) { return slots * kh * most * 2; }  // (whole 16 bytes: most is even)
