@@ -156,7 +156,7 @@ struct Kernels {
     hipFunction_t step[3];                   // one-launch one-token steps, head size classes 16, 32, 64
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
-    hipFunction_t pstore[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
+    hipFunction_t pstore[2], pstore4[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
     // several new tokens a sequence (spans.inc): fp32 and fp16 pages; head sizes to 32, 64, 128, 256; many rows and few
     hipFunction_t span[2][4][2], span_join[2], tree_pick, tree_walk, tree_keep[2];
 };
@@ -952,8 +952,9 @@ int64_t logp_span(int64_t n, int64_t parts) {
 }
 
 // Attention of several new tokens a sequence: rows of an item, by head size and whether the rows are few (a sequence has
-// at most SPAN_FEW under a key head); the slots of a stretch are a multiple of SPAN_STEP.
-constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128;
+// at most SPAN_FEW under a key head); the slots of a stretch are a multiple of SPAN_STEP; a tile's items that are
+// joined all at once.
+constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128, SPAN_SHORT = 8;
 int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
 int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
 // LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
@@ -1031,7 +1032,7 @@ int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     a.r16 = c->fp16 ? 1 : 0;
     out.push_back(mk_desc(k.span[half][span_class(a.dh)][few], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, few), a));
     if (jobs) {
-        const int64_t each = wide ? 1 : 256 / a.lanes;
+        const int64_t each = wide ? 1 : 256 / a.lanes;  // rows of a workgroup
         out.push_back(mk_desc(k.span_join[wide], (uint32_t)(jobs * a.kh * ((a.most + each - 1) / each)), 256, 0, a));
     }
     return SLM_OK;
@@ -1081,7 +1082,8 @@ int lower_batch(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     if (o.kind == OP_PSTORE) {  // p0 k, p1 v, p2 mass, p3 born, p4 and p5 new rows; n0 n, n1 rows, n2 kh, n3 page, n4 dh
         PStoreArgs a{s, (void*)p[0], (void*)p[1], (float*)p[2], (uint32_t*)p[3], p[4], p[5],
                      (int32_t)n[1], (int32_t)n[2], (int32_t)n[3], (int32_t)n[4], n[8] != 0};
-        out.push_back(mk_desc(k.pstore[half], blocks_for((size_t)(n[1] * n[2] * n[4])), 256, 0, a));
+        const bool four = aligned16(a.ksrc) && aligned16(a.vsrc);  // (head sizes are multiples of four)
+        out.push_back(mk_desc(four ? k.pstore4[half] : k.pstore[half], blocks_for((size_t)(n[1] * n[2] * n[4] / (four ? 4 : 1))), 256, 0, a));
         return SLM_OK;
     }
     if (o.kind == OP_PATTEND) {
@@ -4081,6 +4083,7 @@ int load_kernels(slm_hip* c) {
         hipFunction_t* f;
         const char* n;
     } batch[] = {{&k.pstore[0], "slm_paged_store"},  {&k.pstore[1], "slm_paged_store16"},
+                 {&k.pstore4[0], "slm_store_rows"}, {&k.pstore4[1], "slm_store_rows16"},
                  {&k.pjoin[0], "slm_paged_join_4"},  {&k.pjoin[1], "slm_paged_join_16"},
                  {&k.pselect, "slm_paged_select"},
                  {&k.pmove[0], "slm_paged_move16"},  {&k.pmove[1], "slm_paged_move8"},
@@ -5802,7 +5805,7 @@ int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_p
     o.n[3] = (int64_t)(g->page | g->dh << 32);
     o.n[4] = (int64_t)((uint64_t)want.gap | (uint64_t)want.back << 32);
     o.n[5] = (int64_t)g->pages;
-    o.n[6] = (half ? 1 : 0) | (few ? 2 : 0) | (plan->longest > 8 ? 4 : 0) | (int64_t)(tree ? s->words : 0) << 8;
+    o.n[6] = (half ? 1 : 0) | (few ? 2 : 0) | (plan->longest > SPAN_SHORT ? 4 : 0) | (int64_t)(tree ? s->words : 0) << 8;
     o.n[7] = (int64_t)((uint64_t)plan->items | (uint64_t)plan->jobs << 32);
     o.n[8] = (int64_t)plan->slots;
     o.n[9] = (int64_t)s->width;
@@ -5849,7 +5852,7 @@ int slm_hip_verify(slm_hip* c, slm_seqs* s, uint32_t* count, uint32_t* path, uin
         if (bad) return fail(c, SLM_E_INVALID, "verify: the outputs overlap each other or the logits");
     }
     const size_t rows = std::max<size_t>(1, s->rows), panels = (vocab + 2047) / 2048;
-    size_t parts = std::max<size_t>(1, std::min(panels, 1024 / rows));
+    size_t parts = std::max<size_t>(1, std::min(panels, 2048 / rows));
     const size_t span = (panels + parts - 1) / parts * 2048;
     parts = (vocab + span - 1) / span;
     TRY(need_pws(c, rows * parts * 8));
