@@ -157,8 +157,8 @@ struct Kernels {
     // several sequences over paged caches (batch.hip): fp32 and fp16 pages; attention by head sizes to
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
     hipFunction_t pstore[2], pstore4[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
-    // several new tokens a sequence (spans.inc): fp32 and fp16 pages; head sizes to 32, 64, 128, 256; many rows and few
-    hipFunction_t span[2][4][2], span_join[2], tree_pick, tree_walk, tree_keep[2];
+    // several new tokens a sequence (spans.inc): slots seen by their place, or each asked for; fp32 and fp16 pages; head sizes to 32, 64, 128, 256; many rows and few
+    hipFunction_t span[2][2][4][2], span_join[2], tree_pick, tree_walk, tree_keep[2];
 };
 
 // A block of device memory that host arrays go up into, through two pinned uploads in turn.
@@ -1030,7 +1030,8 @@ int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     while (a.lanes * 4 < a.dh) a.lanes *= 2;
     a.scale = o.f[0];
     a.r16 = c->fp16 ? 1 : 0;
-    out.push_back(mk_desc(k.span[half][span_class(a.dh)][few], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, few), a));
+    const bool slots = a.born || (a.up && (a.gap || a.back < 0x7fffffffu));
+    out.push_back(mk_desc(k.span[slots][half][span_class(a.dh)][few], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, few), a));
     if (jobs) {
         const int64_t each = wide ? 1 : 256 / a.lanes;  // rows of a workgroup
         out.push_back(mk_desc(k.span_join[wide], (uint32_t)(jobs * a.kh * ((a.most + each - 1) / each)), 256, 0, a));
@@ -4102,11 +4103,12 @@ int load_kernels(slm_hip* c) {
     TRY(get_batch(&k.tree_walk, "slm_tree_walk"));
     TRY(get_batch(&k.tree_keep[0], "slm_tree_keep16"));
     TRY(get_batch(&k.tree_keep[1], "slm_tree_keep8"));
-    for (int half = 0; half < 2; half++)
-        for (int t = 0; t < 4; t++)
-            for (int few = 0; few < 2; few++)
-                TRY(get_batch(&k.span[half][t][few], std::string("slm_span") + (half ? "16_" : "_") + std::to_string(32 << t) +
-                                                         (few ? "_1" : "_4")));
+    for (int slots = 0; slots < 2; slots++)
+        for (int half = 0; half < 2; half++)
+            for (int t = 0; t < 4; t++)
+                for (int few = 0; few < 2; few++)
+                    TRY(get_batch(&k.span[slots][half][t][few], std::string(slots ? "slm_span_slots" : "slm_span") + (half ? "16_" : "_") +
+                                                                    std::to_string(32 << t) + (few ? "_1" : "_4")));
     for (int half = 0; half < 2; half++)
         for (int t = 0; t < 3; t++)
             for (int m = 0; m < 5; m++)
