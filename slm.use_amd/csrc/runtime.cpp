@@ -5648,9 +5648,11 @@ int slm_hip_seqs_tree(slm_hip* c, slm_seqs* s, const uint32_t* parent, const uin
 namespace {
 
 // Cuts the new tokens' rows and the slots that they see into items: rows in tiles of `most` at most, of about one size;
-// slots in stretches of one length for the whole batch, such that there are about SPAN_ITEMS workgroups, each of SPAN_STEP
-// slots at least. The longest go first.
-constexpr uint64_t SPAN_ITEMS = 1024;
+// slots, where a tile sees more than a compute unit's share of the batch's work by a quarter, in stretches of that share (of
+// SPAN_STEP slots at least). The longest go first. Measured with stretches of 128 to 6016 slots, us, the rule's in brackets: 24
+// trees of 48 behind up to 6000 fp16 tokens 69 57 53 55 50 44 45 [46] 80 147, one of 25 behind 9001 [21] 21 25 29 33 .. 225,
+// windows of 1024 at 900 new tokens 152 94 84 87 86 83 [78], 16 prompts of up to 1500 246 103 92 88 82 79 78 [75], 6 chunks of
+// 256 behind 9000 58 49 45 [50] 56 46 55 70 122 197: more pieces cost their set-up and the join, fewer leave units idle.
 int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan** out) {
     SpanPlan* p = nullptr;
     for (auto& q : s->plans)
@@ -5692,17 +5694,15 @@ int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan
                 work += hi - lo;
             }
         }
-        uint64_t stretch = std::max<uint64_t>(1, work * kh / SPAN_ITEMS);
+        uint64_t stretch = std::max<uint64_t>(1, work * kh / CU_COUNT);
         stretch = (stretch + SPAN_STEP - 1) / SPAN_STEP * SPAN_STEP;
         for (const Tile& t : tiles) {
-            const uint64_t n = t.hi - t.lo, parts = std::max<uint64_t>(1, (n + stretch - 1) / stretch);
-            const uint64_t each = ((n + parts - 1) / parts + SPAN_STEP - 1) / SPAN_STEP * SPAN_STEP;
-            const uint64_t used = std::max<uint64_t>(1, each ? (n + each - 1) / each : 1);
-            if (used > 1) jobs.push_back({{t.b, t.row, t.rows, (uint32_t)slots, (uint32_t)used, 0, 0, 0}});
-            longest = std::max<size_t>(longest, used > 1 ? used : 0);
-            for (uint64_t z = 0; z < used; z++)
-                items.push_back({{t.b, t.row, t.rows, (uint32_t)(t.lo + z * each), (uint32_t)std::min<uint64_t>(t.hi, t.lo + (z + 1) * each),
-                                  used > 1 ? (uint32_t)slots++ : SLM_NO_SEQ, 0, 0}});
+            const uint64_t n = t.hi - t.lo, parts = n <= stretch + stretch / 4 ? 1 : (n + stretch - 1) / stretch;
+            if (parts > 1) jobs.push_back({{t.b, t.row, t.rows, (uint32_t)slots, (uint32_t)parts, 0, 0, 0}});
+            longest = std::max<size_t>(longest, parts > 1 ? parts : 0);
+            for (uint64_t z = 0; z < parts; z++)
+                items.push_back({{t.b, t.row, t.rows, (uint32_t)(t.lo + z * stretch), (uint32_t)(z + 1 < parts ? t.lo + (z + 1) * stretch : t.hi),
+                                  parts > 1 ? (uint32_t)slots++ : SLM_NO_SEQ, 0, 0}});
         }
         std::stable_sort(items.begin(), items.end(), [](const Item& x, const Item& y) { return x.v[4] - x.v[3] > y.v[4] - y.v[3]; });
         // (launches are sized by these counts, and a kept step is kept for its launches: they go up in steps)
