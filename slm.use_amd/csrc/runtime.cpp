@@ -960,8 +960,9 @@ int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 
 // LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
 // largest; where waves share rows, their parts as they are joined.
 int64_t span_lds(int64_t dh, bool half, bool few) {
-    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = few ? (half ? 128 : 64) : dp <= 64 ? 64 : 32;
-    const int64_t row = !half && !few ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
+    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, waves = dp > 128 ? 2 : 4,
+                  kt = few ? waves * (half ? 32 : 16) : dp <= 64 ? 64 : 32;
+    const int64_t row = !half && !few && dp <= 128 ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
     const int64_t tile = kt * row * 2 + kt * 4 + 64, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
     return std::max(tile, join);
 }
@@ -5424,7 +5425,7 @@ int slm_hip_seqs_set(slm_hip* c, slm_seqs* s, size_t n, const uint32_t* len, con
     hi[n] = item;
     for (size_t i = items; i < all; i++) ht[4 * i] = SLM_NO_SEQ;
     hipStream_t st = mstream(c);
-    s->n = 0;  // (nothing until both copies are queued)
+    s->n = s->rows = 0;  // (nothing until both copies are queued)
     s->has_tree = false;
     for (auto& p : s->plans) p.valid = false;
     HIPC(c, hipMemcpyAsync(s->dev, h, s->at_items() + 16 * all, hipMemcpyHostToDevice, st));

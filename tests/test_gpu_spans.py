@@ -128,6 +128,26 @@ def test_what_is_not_seen_may_hold_anything(hip, pkg, half, tree, heads):
     assert np.isfinite(want).any() and not np.isfinite(want).all()
 
 
+@pytest.mark.parametrize("size", [1e4, 1e6, 3e8, 1e30])
+@pytest.mark.parametrize("which", ["keys", "values", "both"])
+@pytest.mark.parametrize("seen", [False, True])
+def test_far_larger_keys_and_values_beside_others(hip, pkg, size, which, seen):
+    """Finite ones many times the others' size in the same tile: of tokens that a row does not see, and of
+    tokens that rows see (then without weight for most rows, or all of it)."""
+    lens, fresh = [300, 70], [90, 70]
+    rng = rng_of(int(np.log10(size)), seen)
+    c = Cache(rng, lens, 2, 64, 16)
+    for b, n in enumerate(lens):
+        pg, sl = c.where(b)
+        at = [3, 65, 130][:n // 60] if seen else [n - 1, n - 30]
+        for name, x in (("k", c.k), ("v", c.v)):
+            if which in ("both", "keys" if name == "k" else "values"):
+                x[pg[at], :, sl[at]] *= np.float32(size)
+    q = queries(rng, fresh, 6, 64)
+    want, bound = R.attend(c, fresh, q, 0.125)
+    check(run(hip, pkg, c, fresh, q, 0.125), want, bound)
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_infinities_and_nan_in_visible_keys(hip, pkg, half):
     lens, fresh = [600] * 7, [20] * 7
