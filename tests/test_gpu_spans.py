@@ -148,6 +148,18 @@ def test_far_larger_keys_and_values_beside_others(hip, pkg, size, which, seen):
     check(run(hip, pkg, c, fresh, q, 0.125), want, bound)
 
 
+@pytest.mark.parametrize("fresh", [3, 130])
+@pytest.mark.parametrize("n", [200, 5000])
+def test_the_largest_values(hip, pkg, fresh, n):
+    """fp32's largest: no sum of weighted ones overflows."""
+    rng = rng_of(n, fresh)
+    c = Cache(rng, [n], 1, 64, 16)
+    c.v = (np.sign(c.v) * np.float32(3.3e38)).astype(np.float32)
+    q = queries(rng, [fresh], 3, 64)
+    want, bound = R.attend(c, [fresh], q, 0.125)
+    check(run(hip, pkg, c, [fresh], q, 0.125), want, bound)
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_infinities_and_nan_in_visible_keys(hip, pkg, half):
     lens, fresh = [600] * 7, [20] * 7
