@@ -3,9 +3,10 @@
 // compiled with the same flags (expressions round as written).
 //
 // A paged cache is [pages][key heads][page][dh]: token t of a sequence lies in slot t % page of
-// page table[t / page]. The bits of a sequence's attention and eviction depend on the sequence
-// alone, not on the batch around it or on how the launch is cut. (Log probabilities add a row up in
-// an order that goes by the rows' number and alignment.)
+// page table[t / page]. The bits of a sequence's single tokens' attention and eviction depend on the
+// sequence alone, not on the batch around it or on how the launch is cut. (Log probabilities add a row up in
+// an order that goes by the rows' number and alignment; attention of several new tokens is cut by the
+// whole batch's work.)
 
 #include <float.h>
 #include <hip/hip_runtime.h>
@@ -118,8 +119,8 @@ __device__ __forceinline__ void store_body(const PStoreArgs& a) {
 KERNEL void __launch_bounds__(256) slm_paged_store(PStoreArgs a) { store_body<float>(a); }
 KERNEL void __launch_bounds__(256) slm_paged_store16(PStoreArgs a) { store_body<_Float16>(a); }
 
-// The same for new rows at whole 16 bytes, four elements a thread (1641 rows of 12 key heads of 64 into fp16 pages: 11.6 us
-// one by one, STORE4).
+// The same for new rows at whole 16 bytes, four elements a thread (some 1560 rows of 12 key heads of 64 into fp16 pages: 11.6
+// us one by one, 5.5 so).
 template <typename T>
 __device__ __forceinline__ void store4_body(const PStoreArgs& a) {
     typedef T V __attribute__((ext_vector_type(4)));

@@ -951,10 +951,15 @@ int64_t logp_span(int64_t n, int64_t parts) {
     return (panels + parts - 1) / parts * LOGP_SHORT;
 }
 
-// Attention of several new tokens a sequence: rows of an item, by head size and whether the rows are few (a sequence has
-// at most SPAN_FEW under a key head); the slots of a stretch are a multiple of SPAN_STEP; a tile's items that are
-// joined all at once.
+// Attention of several new tokens a sequence: rows of an item, by head size and whether the rows are few (span_few); the
+// slots of a stretch are a multiple of SPAN_STEP; a tile's items that are joined all at once (a join of 8 parts or less by
+// the other kernel: 6 chunks of 256 behind 9000 tokens 43 -> 51 us, 24 trees of 48 50 -> 56).
 constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128, SPAN_SHORT = 8;
+// Few rows: tiles of SPAN_FEW rows whose waves share the slots, instead of larger ones whose waves have rows of their own. With
+// tiles of SPAN_FEW -> without, us: 40 trees behind 900 tokens of 7 rows a key head 31 -> 46, of 24 34 -> 47, of 32 37 -> 47, of
+// 32 fp16 20 -> 28, heads of 128 53 -> 87; one tree of 32 behind 9001 28 -> 31, but of 48 35 -> 31; ten of 32 in fp16 heads
+// of 256 94 -> 51, of fp32 106 -> 107.
+bool span_few(int64_t dh, uint64_t rows) { return rows <= (uint64_t)(dh > 128 ? SPAN_FEW : 2 * SPAN_FEW); }
 int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
 int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
 // LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
@@ -5780,7 +5785,7 @@ int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_p
     if (!aligned16(q)) return fail(c, SLM_E_UNSUPPORTED, "%s: q must be 16-byte aligned", name);
     if (meet(y, n * 4, q, n * 4) || meets_cache(g, slots, half, y, n * 4))
         return fail(c, SLM_E_INVALID, "%s: y lies in an input", name);
-    const bool few = most * group <= (uint64_t)SPAN_FEW;
+    const bool few = span_few((int64_t)g->dh, most * group);
     SpanPlan want;
     want.group = group;
     want.heads = heads;
@@ -5854,6 +5859,8 @@ int slm_hip_verify(slm_hip* c, slm_seqs* s, uint32_t* count, uint32_t* path, uin
         for (int j = 0; j < i; j++) bad = bad || meet(outs[i], bytes[i], outs[j], bytes[j]);
         if (bad) return fail(c, SLM_E_INVALID, "verify: the outputs overlap each other or the logits");
     }
+    // parts of a row: 2048 workgroups in all, of 2048 logits at least. 24 trees of 48 over 32000 logits 17.0 us, with 1024 or 256
+    // workgroups 18.9, with 8192 16.9; one of 25 over 151936 11.1, with 512 9.4; one of 200 over 300000 50.0, with 512 78.8.
     const size_t rows = std::max<size_t>(1, s->rows), panels = (vocab + 2047) / 2048;
     size_t parts = std::max<size_t>(1, std::min(panels, 2048 / rows));
     const size_t span = (panels + parts - 1) / parts * 2048;
