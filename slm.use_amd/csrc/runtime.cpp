@@ -174,7 +174,7 @@ struct Upload {
 // is set anew: a model's layers of one kind share it.
 struct SpanPlan {
     size_t group = 0, heads = 0;
-    int64_t most = 0;
+    int64_t most = 0, step = 0;
     uint32_t gap = 0, back = 0;
     bool born = false, tree = false, valid = false;
     Upload up;
@@ -952,9 +952,9 @@ int64_t logp_span(int64_t n, int64_t parts) {
 }
 
 // Attention of several new tokens a sequence: rows of an item, by head size and whether the rows are few (span_few); the
-// slots of a stretch are a multiple of SPAN_STEP; a tile's items that are joined all at once (a join of 8 parts or less by
-// the other kernel: 6 chunks of 256 behind 9000 tokens 43 -> 51 us, 24 trees of 48 50 -> 56).
-constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128, SPAN_SHORT = 8;
+// least slots of a stretch; a tile's items that are joined all at once (a join of 8 parts or less by the other kernel: 6
+// chunks of 256 behind 9000 tokens 43 -> 51 us, 24 trees of 48 50 -> 56).
+constexpr int64_t SPAN_FEW = 16, SPAN_LEAST = 64, SPAN_SHORT = 8;
 // Few rows: tiles of SPAN_FEW rows whose waves share the slots, instead of larger ones whose waves have rows of their own. With
 // tiles of SPAN_FEW -> without, us: 40 trees behind 900 tokens of 7 rows a key head 31 -> 46, of 24 34 -> 47, of 32 37 -> 47, of
 // 32 fp16 20 -> 28, heads of 128 53 -> 87; one tree of 32 behind 9001 28 -> 31, but of 48 35 -> 31; ten of 32 in fp16 heads
@@ -962,11 +962,12 @@ constexpr int64_t SPAN_FEW = 16, SPAN_STEP = 128, SPAN_SHORT = 8;
 bool span_few(int64_t dh, uint64_t rows) { return rows <= (uint64_t)(dh > 128 ? SPAN_FEW : 2 * SPAN_FEW); }
 int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
 int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
+// Slots of a tile in LDS.
+int64_t span_tile(int64_t dh, bool half, bool few) { return few ? (dh > 128 ? 2 : 4) * (half ? 32 : 16) : dh <= 64 ? 64 : 32; }
 // LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
 // largest; where waves share rows, their parts as they are joined.
 int64_t span_lds(int64_t dh, bool half, bool few) {
-    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, waves = dp > 128 ? 2 : 4,
-                  kt = few ? waves * (half ? 32 : 16) : dp <= 64 ? 64 : 32;
+    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = span_tile(dh, half, few);
     const int64_t row = !half && !few && dp <= 128 ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
     const int64_t tile = kt * row * 2 + kt * 4 + 64, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
     return std::max(tile, join);
@@ -5654,15 +5655,17 @@ int slm_hip_seqs_tree(slm_hip* c, slm_seqs* s, const uint32_t* parent, const uin
 namespace {
 
 // Cuts the new tokens' rows and the slots that they see into items: rows in tiles of `most` at most, of about one size;
-// slots, where a tile sees more than a compute unit's share of the batch's work by a quarter, in stretches of that share (of
-// SPAN_STEP slots at least). The longest go first. Measured with stretches of 128 to 6016 slots, us, the rule's in brackets: 24
+// slots, where a tile sees more than a compute unit's share of the batch's work by a quarter, in stretches of that share, in
+// whole tiles of LDS (step), of SPAN_LEAST slots at least (trees of 25 behind 9001 tokens by 128 slots 21.5 us, by 64 20.0;
+// behind 3000 15.1, 13.7; in heads of 128 by 128 40.1, 64 37.1, 32 33.3, behind 2000 26.4, 21.5, 22.2; trees of 4 in fp16,
+// whose tiles are of 128, behind 9000 11.1, 11.2, 11.4). The longest go first. Measured with stretches of 128 to 6016 slots, us, the rule's in brackets: 24
 // trees of 48 behind up to 6000 fp16 tokens 69 57 53 55 50 44 45 [46] 80 147, one of 25 behind 9001 [21] 21 25 29 33 .. 225,
 // windows of 1024 at 900 new tokens 152 94 84 87 86 83 [78], 16 prompts of up to 1500 246 103 92 88 82 79 78 [75], 6 chunks of
 // 256 behind 9000 58 49 45 [50] 56 46 55 70 122 197: more pieces cost their set-up and the join, fewer leave units idle.
 int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan** out) {
     SpanPlan* p = nullptr;
     for (auto& q : s->plans)
-        if (q.valid && q.group == want.group && q.heads == want.heads && q.most == want.most && q.gap == want.gap &&
+        if (q.valid && q.group == want.group && q.heads == want.heads && q.most == want.most && q.step == want.step && q.gap == want.gap &&
             q.back == want.back && q.born == want.born && q.tree == want.tree)
             p = &q;
     if (p) {
@@ -5700,8 +5703,8 @@ int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan
                 work += hi - lo;
             }
         }
-        uint64_t stretch = std::max<uint64_t>(1, work * kh / CU_COUNT);
-        stretch = (stretch + SPAN_STEP - 1) / SPAN_STEP * SPAN_STEP;
+        uint64_t stretch = std::max<uint64_t>(SPAN_LEAST, work * kh / CU_COUNT);
+        stretch = (stretch + want.step - 1) / want.step * want.step;
         for (const Tile& t : tiles) {
             const uint64_t n = t.hi - t.lo, parts = n <= stretch + stretch / 4 ? 1 : (n + stretch - 1) / stretch;
             if (parts > 1) jobs.push_back({{t.b, t.row, t.rows, (uint32_t)slots, (uint32_t)parts, 0, 0, 0}});
@@ -5750,6 +5753,7 @@ int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan
     p->group = want.group;
     p->heads = want.heads;
     p->most = want.most;
+    p->step = want.step;
     p->gap = want.gap;
     p->back = want.back;
     p->born = want.born;
@@ -5790,6 +5794,7 @@ int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_p
     want.group = group;
     want.heads = heads;
     want.most = span_rows((int64_t)g->dh, few);
+    want.step = span_tile((int64_t)g->dh, half, few);
     want.gap = (uint32_t)std::min<size_t>(gap, UINT32_MAX);
     want.back = (uint32_t)std::min<size_t>(reach - 1, UINT32_MAX);
     want.tree = tree;
