@@ -158,7 +158,7 @@ struct Kernels {
     // 64, 128, 256 and 1, 2, 3, 4 or up to 16 query heads a key head
     hipFunction_t pstore[2], pstore4[2], pattn[2][3][5], pjoin[2], pselect, pmove[2], logprobs[2], logprobs_split, logprobs_join;
     // several new tokens a sequence (spans.inc): slots seen by their place, or each asked for; fp32 and fp16 pages; head sizes to 32, 64, 128, 256; many rows and few
-    hipFunction_t span[2][2][4][2], span_join[2], tree_pick, tree_walk, tree_keep[2];
+    hipFunction_t span[2][2][4][3], span_join[2], tree_pick, tree_walk, tree_keep[2];
 };
 
 // A block of device memory that host arrays go up into, through two pinned uploads in turn.
@@ -176,7 +176,7 @@ struct SpanPlan {
     size_t group = 0, heads = 0;
     int64_t most = 0, step = 0;
     uint32_t gap = 0, back = 0;
-    bool born = false, tree = false, valid = false;
+    bool born = false, tree = false, two = false, valid = false;
     Upload up;
     size_t items = 0, jobs = 0, slots = 0, longest = 0;  // counts of the launches; a job's most items
     uint64_t used = 0;
@@ -961,15 +961,27 @@ constexpr int64_t SPAN_FEW = 16, SPAN_LEAST = 64, SPAN_SHORT = 8;
 // of 256 94 -> 51, of fp32 106 -> 107.
 bool span_few(int64_t dh, uint64_t rows) { return rows <= (uint64_t)(dh > 128 ? SPAN_FEW : 2 * SPAN_FEW); }
 int span_class(int64_t dh) { return dh <= 32 ? 0 : dh <= 64 ? 1 : dh <= 128 ? 2 : 3; }
-int64_t span_rows(int64_t dh, bool few) { return few ? SPAN_FEW : dh > 128 ? 64 : 128; }
+// In heads to 64 the rows between, of short caches and of batches of few tiles: tiles of 64 rows, two pairs of waves that share the
+// slots (SPAN_TWO), instead of 128 rows (of all: a sequence's most rows a key head, its longest cache, the sequences times the key
+// heads). With SPAN_TWO -> without, us: 40 trees of 48 behind 900 tokens 44 -> 49, behind 4000 118 -> 172, one of 48 behind 9001 26
+// -> 30; in fp16 24 of 144 rows behind 6000 37 -> 50, 40 of 100 behind 900 29 -> 37, but 4 18 -> 17; in fp32 24 of 144 68 -> 80, 40
+// of 100 50 -> 57, 4 23 -> 20, one of 75 behind 9001 21 -> 20; 16 prompts of up to 300 fp16 tokens 14 -> 23, of 1000 42 -> 43, of
+// 2000 109 -> 107, one of 8001 266 -> 232; in fp32 of 300 19 -> 24, 500 29 -> 31, 800 50 -> 44. Heads of 128 spill (fp16 60 -> 45).
+enum { SPAN_MANY, SPAN_ONE, SPAN_TWO };
+int span_kind(int64_t dh, bool half, uint64_t rows, uint64_t len, uint64_t all) {
+    if (span_few(dh, rows)) return SPAN_ONE;
+    const bool two = rows <= 64 || len <= (half ? 1024u : 512u) || (rows <= 192 && (half || all * ((rows + 63) / 64) >= (uint64_t)CU_COUNT));
+    return dh <= 64 && two ? SPAN_TWO : SPAN_MANY;
+}
+int64_t span_rows(int64_t dh, int kind) { return kind == SPAN_ONE ? SPAN_FEW : kind == SPAN_TWO || dh > 128 ? 64 : 128; }
 // Slots of a tile in LDS.
-int64_t span_tile(int64_t dh, bool half, bool few) { return few ? (dh > 128 ? 2 : 4) * (half ? 32 : 16) : dh <= 64 ? 64 : 32; }
+int64_t span_tile(int64_t dh, bool half, int kind) { return kind == SPAN_ONE ? (dh > 128 ? 2 : 4) * (half ? 32 : 16) : dh <= 64 || kind == SPAN_TWO ? 64 : 32; }
 // LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
 // largest; where waves share rows, their parts as they are joined.
-int64_t span_lds(int64_t dh, bool half, bool few) {
-    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = span_tile(dh, half, few);
-    const int64_t row = !half && !few && dp <= 128 ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
-    const int64_t tile = kt * row * 2 + kt * 4 + 64, join = few ? 4 * SPAN_FEW * (dp + 4 + 2) * 4 : 0;
+int64_t span_lds(int64_t dh, bool half, int kind) {
+    const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = span_tile(dh, half, kind);
+    const int64_t row = !half && kind != SPAN_ONE && dp <= 128 ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
+    const int64_t tile = kt * row * 2 + kt * 4 + 64, join = kind ? 4 * (kind == SPAN_ONE ? SPAN_FEW : 32) * (dp + 4 + 2) * 4 : 0;
     return std::max(tile, join);
 }
 size_t span_ml(size_t slots, size_t kh, size_t most) { return slots * kh * most * 2; }  // (whole 16 bytes: most is even)
@@ -1019,7 +1031,8 @@ int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     a.dh = (int32_t)(n[3] >> 32);
     a.gap = (uint32_t)(n[4] & 0xffffffff);
     a.back = (uint32_t)((uint64_t)n[4] >> 32);
-    const bool half = n[6] & 1, few = n[6] & 2, wide = n[6] & 4;
+    const bool half = n[6] & 1, wide = n[6] & 2;
+    const int kind = n[6] >> 2 & 3;
     a.words = (int32_t)(n[6] >> 8);
     if (p[7]) {
         a.depth = (const uint32_t*)p[7] + 2 * n[1];
@@ -1028,7 +1041,7 @@ int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     const int64_t items = n[7] & 0xffffffff, jobs = n[7] >> 32;
     a.items = (const uint32_t*)p[5];
     a.jobs = a.items + 8 * items;
-    a.most = (int32_t)span_rows(a.dh, few);
+    a.most = (int32_t)span_rows(a.dh, kind);
     a.ml = c->pws;
     a.po = a.ml + span_ml((size_t)n[8], (size_t)a.kh, (size_t)a.most);
     span_divisor((uint32_t)a.page, &a.page_mul, &a.page_shift);
@@ -1038,7 +1051,7 @@ int lower_spans(slm_hip* c, const Op& o, std::vector<Rec>& out) {
     a.scale = o.f[0];
     a.r16 = c->fp16 ? 1 : 0;
     const bool slots = a.born || (a.up && (a.gap || a.back < 0x7fffffffu));
-    out.push_back(mk_desc(k.span[slots][half][span_class(a.dh)][few], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, few), a));
+    out.push_back(mk_desc(k.span[slots][half][span_class(a.dh)][kind], (uint32_t)(items * a.kh), 256, (uint32_t)span_lds(a.dh, half, kind), a));
     if (jobs) {
         const int64_t each = wide ? 1 : 256 / a.lanes;  // rows of a workgroup
         out.push_back(mk_desc(k.span_join[wide], (uint32_t)(jobs * a.kh * ((a.most + each - 1) / each)), 256, 0, a));
@@ -4113,9 +4126,10 @@ int load_kernels(slm_hip* c) {
     for (int slots = 0; slots < 2; slots++)
         for (int half = 0; half < 2; half++)
             for (int t = 0; t < 4; t++)
-                for (int few = 0; few < 2; few++)
-                    TRY(get_batch(&k.span[slots][half][t][few], std::string(slots ? "slm_span_slots" : "slm_span") + (half ? "16_" : "_") +
-                                                                    std::to_string(32 << t) + (few ? "_1" : "_4")));
+                for (int kind = 0; kind < 3; kind++)
+                    if (kind != SPAN_TWO || t < 2)
+                        TRY(get_batch(&k.span[slots][half][t][kind], std::string(slots ? "slm_span_slots" : "slm_span") + (half ? "16_" : "_") +
+                                                                         std::to_string(32 << t) + (kind == SPAN_ONE ? "_1" : kind == SPAN_TWO ? "_2" : "_4")));
     for (int half = 0; half < 2; half++)
         for (int t = 0; t < 3; t++)
             for (int m = 0; m < 5; m++)
@@ -5665,7 +5679,7 @@ namespace {
 int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan** out) {
     SpanPlan* p = nullptr;
     for (auto& q : s->plans)
-        if (q.valid && q.group == want.group && q.heads == want.heads && q.most == want.most && q.step == want.step && q.gap == want.gap &&
+        if (q.valid && q.group == want.group && q.heads == want.heads && q.most == want.most && q.step == want.step && q.two == want.two && q.gap == want.gap &&
             q.back == want.back && q.born == want.born && q.tree == want.tree)
             p = &q;
     if (p) {
@@ -5704,6 +5718,9 @@ int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan
             }
         }
         uint64_t stretch = std::max<uint64_t>(SPAN_LEAST, work * kh / CU_COUNT);
+        // (tiles of SPAN_TWO, three of which a unit holds: 24 trees of 48 in fp16 45 -> 37 us, 16 behind 6000 86 -> 72, 10 of 48 rows
+        // behind 4000 56 -> 44; where a unit has four of them, 50 -> 56, or its share is 500 slots, 24.8 -> 26.1, it does not pay)
+        if (want.two && stretch >= 1024 && tiles.size() * kh < 2 * CU_COUNT) stretch /= 2;
         stretch = (stretch + want.step - 1) / want.step * want.step;
         for (const Tile& t : tiles) {
             const uint64_t n = t.hi - t.lo, parts = n <= stretch + stretch / 4 ? 1 : (n + stretch - 1) / stretch;
@@ -5754,6 +5771,7 @@ int span_plan(slm_hip* c, slm_seqs* s, const SpanPlan& want, size_t kh, SpanPlan
     p->heads = want.heads;
     p->most = want.most;
     p->step = want.step;
+    p->two = want.two;
     p->gap = want.gap;
     p->back = want.back;
     p->born = want.born;
@@ -5789,12 +5807,13 @@ int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_p
     if (!aligned16(q)) return fail(c, SLM_E_UNSUPPORTED, "%s: q must be 16-byte aligned", name);
     if (meet(y, n * 4, q, n * 4) || meets_cache(g, slots, half, y, n * 4))
         return fail(c, SLM_E_INVALID, "%s: y lies in an input", name);
-    const bool few = span_few((int64_t)g->dh, most * group);
+    const int kind = span_kind((int64_t)g->dh, half, most * group, s->max_len, s->n * g->key_heads);
     SpanPlan want;
     want.group = group;
     want.heads = heads;
-    want.most = span_rows((int64_t)g->dh, few);
-    want.step = span_tile((int64_t)g->dh, half, few);
+    want.most = span_rows((int64_t)g->dh, kind);
+    want.two = kind == SPAN_TWO;
+    want.step = span_tile((int64_t)g->dh, half, kind);
     want.gap = (uint32_t)std::min<size_t>(gap, UINT32_MAX);
     want.back = (uint32_t)std::min<size_t>(reach - 1, UINT32_MAX);
     want.tree = tree;
@@ -5818,7 +5837,7 @@ int attend_new(slm_hip* c, const char* name, bool tree, slm_seqs* s, const slm_p
     o.n[3] = (int64_t)(g->page | g->dh << 32);
     o.n[4] = (int64_t)((uint64_t)want.gap | (uint64_t)want.back << 32);
     o.n[5] = (int64_t)g->pages;
-    o.n[6] = (half ? 1 : 0) | (few ? 2 : 0) | (plan->longest > SPAN_SHORT ? 4 : 0) | (int64_t)(tree ? s->words : 0) << 8;
+    o.n[6] = (half ? 1 : 0) | (plan->longest > SPAN_SHORT ? 2 : 0) | (int64_t)kind << 2 | (int64_t)(tree ? s->words : 0) << 8;
     o.n[7] = (int64_t)((uint64_t)plan->items | (uint64_t)plan->jobs << 32);
     o.n[8] = (int64_t)plan->slots;
     o.n[9] = (int64_t)s->width;
