@@ -497,7 +497,10 @@ class Seqs:
     def tree(self, parent, ids=None):
         """The new tokens as a tree: parent [rows], the place among the sequence's new tokens of the one that
         each follows (-1: the old tokens); ids [rows]: the tokens, for verify."""
-        parent = np.ascontiguousarray(np.asarray(parent, dtype=np.int64).astype(np.int32)).view(np.uint32)
+        parent = np.asarray(parent, dtype=np.int64)
+        if ((parent < -(1 << 31)) | (parent > 0xffffffff)).any():  # (that 32 bits would make another)
+            raise ValueError("tree: a parent is a place among the new tokens, or -1")
+        parent = np.ascontiguousarray(parent.astype(np.uint32))
         ids = None if ids is None else np.ascontiguousarray(ids, dtype=np.uint32)
         if parent.shape != (self.rows,) or (ids is not None and ids.shape != parent.shape):
             raise ValueError(f"tree: arrays of {self.rows} new tokens are wanted")

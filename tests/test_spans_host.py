@@ -200,3 +200,14 @@ def test_in_a_recorded_step(host, hip):
     t.prompt(gap=8)
     assert host.lib.stub_launches() >= before + 8
     hip.flush()
+
+
+def test_parents_of_more_than_32_bits(host, hip):
+    """Not taken for what their lower bits name."""
+    t = Set(host, hip)
+    for bad in (1 << 32, -(1 << 32)):
+        parent = t.parent.astype(np.int64)
+        parent[5] = bad
+        with pytest.raises(ValueError):
+            t.s.tree(parent, np.zeros(len(parent)))
+    t.tree(), t.verify()
