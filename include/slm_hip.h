@@ -248,10 +248,12 @@ int slm_hip_seqs_tree(slm_hip* ctx, slm_seqs* seqs, const uint32_t* parent, cons
  * key_heads). A token of position p sees those of its own sequence at p − reach + 1 to p − gap (reach
  * SIZE_MAX: all from the first on; never one behind its own): positions of old tokens by `born` where the
  * cache has it, else slot t holds position t; new ones follow them in order. A token that sees none gets zeros.
- * What of a page is not seen may hold anything. Rows of y behind the last new token stay as they were. Products
- * take elements and weights to 22 bits or more (each in two fp16 parts, where that is faster) and are added up in
- * fp32, in fp16 mode too; y is rounded there as slm_hip_attend rounds it. The slots are cut into stretches by the
- * whole batch's work: a sequence's last bits may differ in another batch. */
+ * What of a page is not seen may hold anything. Rows of y behind the last new token stay as they were. Sums are fp32, in
+ * fp16 mode too; y is rounded there as slm_hip_attend rounds it. Products take their factors in two fp16 parts, where
+ * that is faster: values to 22 bits or more, however small beside others; weights to 22 bits or to 2^-36 of their row's
+ * largest, the coarser (a weight below that may count as 0); keys and queries to 22 bits or to what a score changes by
+ * 2^-25. Sums of values below 2^-94 are off by up to 2^-118 a slot. The slots are cut into stretches by the whole batch's
+ * work: a sequence's last bits may differ in another batch. */
 int slm_hip_paged_prompt(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* y, const float* q, size_t heads,
                          size_t reach, size_t gap, float scale);
 /* The same for a tree of drafted tokens (slm_hip_seqs_tree): a token sees, of the new ones, itself and those

@@ -976,12 +976,12 @@ int span_kind(int64_t dh, bool half, uint64_t rows, uint64_t len, uint64_t all) 
 int64_t span_rows(int64_t dh, int kind) { return kind == SPAN_ONE ? SPAN_FEW : kind == SPAN_TWO || dh > 128 ? 64 : 128; }
 // Slots of a tile in LDS.
 int64_t span_tile(int64_t dh, bool half, int kind) { return kind == SPAN_ONE ? (dh > 128 ? 2 : 4) * (half ? 32 : 16) : dh <= 64 || kind == SPAN_TWO ? 64 : 32; }
-// LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where waves do not share rows), positions, the waves'
-// largest; where waves share rows, their parts as they are joined.
+// LDS: a tile's keys and values (fp32 ones cut in two fp16 parts where rows are 32 a wave), positions, the waves'
+// largest, a count and up to 32 tiles whose values are added later; where waves share rows, their parts as they are joined.
 int64_t span_lds(int64_t dh, bool half, int kind) {
     const int64_t dp = 32 << span_class(dh), unit = half ? 2 : 4, kt = span_tile(dh, half, kind);
     const int64_t row = !half && kind != SPAN_ONE && dp <= 128 ? (dp + 8) * 2 * 2 : (dp + 16 / unit) * unit;
-    const int64_t tile = kt * row * 2 + kt * 4 + 64, join = kind ? 4 * (kind == SPAN_ONE ? SPAN_FEW : 32) * (dp + 4 + 2) * 4 : 0;
+    const int64_t tile = kt * row * 2 + kt * 4 + 64 + 4 * (1 + 32), join = kind ? 4 * (kind == SPAN_ONE ? SPAN_FEW : 32) * (dp + 4 + 2) * 4 : 0;
     return std::max(tile, join);
 }
 size_t span_ml(size_t slots, size_t kh, size_t most) { return slots * kh * most * 2; }  // (whole 16 bytes: most is even)
