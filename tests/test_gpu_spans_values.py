@@ -139,3 +139,24 @@ def test_long_stretches_with_small_values(hip, pkg, dh, odd):
     q = queries(rng, fresh, 32, dh)
     want, bound = attend(c, fresh, q, dh ** -0.5)
     check(run(hip, pkg, c, fresh, q, dh ** -0.5), want, bound)
+
+
+@pytest.mark.parametrize("scale", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_scale_that_is_not_finite(hip, pkg, kind, half, scale):
+    """NaN for every row that sees a token, as paged_attend's; zeros for one that sees none."""
+    H, KH, dh, lens, fresh = kind
+    rng = rng_of(dh, lens[0], 8)
+    c = Cache(rng, lens, KH, dh, 16, half)
+    q = queries(rng, fresh, H, dh)
+    for gap in (0, 30):
+        y = run(hip, pkg, c, fresh, q, scale, gap=gap)
+        sees = np.concatenate([np.arange(n - f, n) >= gap for n, f in zip(lens, fresh)])
+        assert np.isnan(y[sees]).all() and not y[~sees].any()
+    g, up = c.upload(hip, pkg, mass=False, born=False)
+    s = c.batch(hip)
+    s.set(c.lens, c.table, fresh=np.zeros(len(lens)))
+    dq, one = hip.upload(q[:len(lens)]), hip.alloc(len(lens) * H * dh)
+    hip.paged_attend(s, g, one.ptr, dq.ptr, heads=H, scale=scale)
+    assert np.isnan(one.read()).all()
