@@ -160,3 +160,39 @@ def test_a_scale_that_is_not_finite(hip, pkg, kind, half, scale):
     dq, one = hip.upload(q[:len(lens)]), hip.alloc(len(lens) * H * dh)
     hip.paged_attend(s, g, one.ptr, dq.ptr, heads=H, scale=scale)
     assert np.isnan(one.read()).all()
+
+
+def check_by_largest_score(hip, pkg, kind, half, size):
+    """A row's result is the value of its largest score, where that lies above the others by more than scores may be off."""
+    H, KH, dh, lens, fresh = kind
+    rng = rng_of(dh, lens[0], 9)
+    c = Cache(rng, lens, KH, dh, 16, half)
+    q = (rng.standard_normal((sum(fresh), H, dh)) * size).astype(np.float32)
+    y, at, sure = run(hip, pkg, c, fresh, q, 0.125), 0, 0
+    for b, f in enumerate(fresh):
+        pg, sl = c.where(b)
+        for h in range(H):
+            k, v = (a[pg, h // (H // KH), sl] for a in (c.k, c.v))
+            qq = q[at:at + f, h].astype(np.float64)
+            s, error = qq @ k.T.astype(np.float64), U * (dh + 13) * (np.abs(qq) @ np.abs(k.T))
+            for i in range(f):
+                m = lens[b] - f + i + 1
+                first = int(s[i, :m].argmax())
+                rest = np.delete(s[i, :m] + error[i, :m], first)
+                if not rest.size or (s[i, first] - error[i, first] - rest.max()) * 0.125 > 40:  # (e^-40 of the others)
+                    err = np.abs(y[at + i, h] - v[first]).max()
+                    assert err <= 32 * U * np.abs(v[first]).max(), (b, h, i, err)
+                    sure += 1
+        at += f
+    assert sure > 0.9 * sum(fresh) * H
+
+
+ALONE = [(1, 1, 64, [50] * 24, [1] * 24), (1, 1, 200, [50] * 24, [1] * 24)]  # a row to a workgroup
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e8, 1e9, 1e10, 1e12, 1e30])
+@pytest.mark.parametrize("kind", KINDS + ALONE)
+def test_large_scores(hip, pkg, kind, half, size):
+    """Scores whose last bit is worth many powers of two."""
+    check_by_largest_score(hip, pkg, kind, half, size)
