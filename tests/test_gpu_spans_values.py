@@ -196,3 +196,11 @@ ALONE = [(1, 1, 64, [50] * 24, [1] * 24), (1, 1, 200, [50] * 24, [1] * 24)]  # a
 def test_large_scores(hip, pkg, kind, half, size):
     """Scores whose last bit is worth many powers of two."""
     check_by_largest_score(hip, pkg, kind, half, size)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("size", [1e35, 2e37])
+@pytest.mark.parametrize("kind", KINDS + ALONE)
+def test_the_largest_queries(hip, pkg, kind, half, size):
+    """Near the end of fp32, with scores that it holds."""
+    check_by_largest_score(hip, pkg, kind, half, size)
