@@ -247,7 +247,7 @@ int slm_hip_seqs_tree(slm_hip* ctx, slm_seqs* seqs, const uint32_t* parent, cons
  * [rows][heads][dh], the sequences' new tokens one after another; query head h reads key head h / (heads /
  * key_heads). A token of position p sees those of its own sequence at p − reach + 1 to p − gap (reach
  * SIZE_MAX: all from the first on; never one behind its own): positions of old tokens by `born` where the
- * cache has it, else slot t holds position t; new ones follow them in order. A token that sees none gets zeros.
+ * cache has it (looked at with a reach or a gap alone), else slot t holds position t; new ones follow them in order. A token that sees none gets zeros.
  * What of a page is not seen may hold anything. Rows of y behind the last new token stay as they were. Sums are fp32, in
  * fp16 mode too; y is rounded there as slm_hip_attend rounds it. Products take their factors in two fp16 parts, where
  * that is faster: values to 22 bits or more, however small beside others; weights to 22 bits or to 2^-36 of their row's
