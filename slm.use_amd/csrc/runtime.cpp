@@ -161,10 +161,12 @@ struct Kernels {
     hipFunction_t span[2][2][4][3], span_join[2], tree_pick, tree_walk, tree_keep[2];
 };
 
-// A block of device memory that host arrays go up into, through two pinned uploads in turn.
+// A block of device memory that host arrays go up into, through two pinned uploads in turn. Blocks that it outgrew
+// are kept with it: launched work and cached graphs may still use them.
 struct Upload {
     unsigned char* dev = nullptr;
     size_t bytes = 0;
+    std::vector<std::pair<unsigned char*, size_t>> outgrown;
     unsigned char* pin[2] = {nullptr, nullptr};
     hipEvent_t ev[2] = {nullptr, nullptr};
     int flip = 0;
@@ -3365,6 +3367,7 @@ int need_pws(slm_hip* c, size_t bytes) {
 
 void upload_free(slm_hip* c, Upload& u) {
     if (u.dev) dev_free(c, u.dev);
+    for (auto& q : u.outgrown) dev_free(c, q.first);
     for (int i = 0; i < 2; i++) {
         if (u.pin[i]) hipHostFree(u.pin[i]);
         if (u.ev[i]) hipEventDestroy(u.ev[i]);
@@ -3377,24 +3380,27 @@ int upload_begin(slm_hip* c, Upload& u, size_t bytes, unsigned char** fill) {
     if (bytes > u.bytes) {
         const size_t room = std::max(bytes, u.bytes * 2);
         unsigned char* pin[2] = {nullptr, nullptr};
+        void* dev = nullptr;
         hipError_t e = hipSuccess;
+        try {
+            u.outgrown.reserve(u.outgrown.size() + 1);
+        } catch (const std::bad_alloc&) {
+            e = hipErrorOutOfMemory;
+        }
         for (int i = 0; i < 2 && e == hipSuccess; i++) {
             e = hipHostMalloc((void**)&pin[i], room, hipHostMallocDefault);
             if (e == hipSuccess && !u.ev[i]) e = hipEventCreateWithFlags(&u.ev[i], hipEventDisableTiming);
             if (e == hipSuccess) e = hipEventSynchronize(u.ev[i]);
         }
-        int rc = SLM_OK;
+        if (e == hipSuccess) e = dev_alloc(c, room, &dev);
         if (e != hipSuccess) {
             (void)hipGetLastError();
-            rc = fail(c, SLM_E_MEMORY, "%zu bytes of a batch: %s", room, hipGetErrorString(e));
-        } else {
-            rc = internal_realloc(c, (void**)&u.dev, room);
-        }
-        if (rc) {
             for (auto* q : pin)
                 if (q) hipHostFree(q);
-            return rc;
+            return fail(c, SLM_E_MEMORY, "%zu bytes of a batch: %s", room, hipGetErrorString(e));
         }
+        if (u.dev) u.outgrown.push_back({u.dev, u.bytes});
+        u.dev = (unsigned char*)dev;
         for (int i = 0; i < 2; i++) {
             if (u.pin[i]) hipHostFree(u.pin[i]);
             u.pin[i] = pin[i];
@@ -6017,8 +6023,12 @@ int slm_hip_mem_info(slm_hip* c, size_t* free_bytes, size_t* total_bytes, size_t
     direct(c->pws, c->pws_bytes);
     for (auto& q : c->seqs) {
         direct(q.second->dev, q.second->bytes());
-        direct(q.second->tree.dev, q.second->tree.bytes);
-        for (auto& p : q.second->plans) direct(p.up.dev, p.up.bytes);
+        auto upload = [&](const Upload& u) {
+            direct(u.dev, u.bytes);
+            for (auto& p : u.outgrown) direct(p.first, p.second);
+        };
+        upload(q.second->tree);
+        for (auto& p : q.second->plans) upload(p.up);
     }
     *held_bytes = held;
     return SLM_OK;

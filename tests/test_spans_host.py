@@ -211,3 +211,21 @@ def test_parents_of_more_than_32_bits(host, hip):
         with pytest.raises(ValueError):
             t.s.tree(parent, np.zeros(len(parent)))
     t.tree(), t.verify()
+
+
+def test_batches_that_grow_and_go_leave_nothing(host, hip):
+    """What a batch's trees and plans outgrew goes back with it (memory is held in slabs of 128 MiB)."""
+    n = 1024
+    k, v = (hip.alloc_pages(n, 1, 256, 4) for _ in range(2))
+    g = host.Pages(pages=n, page=256, key_heads=1, dh=4, k=k.ptr, v=v.ptr)
+    q, y = hip.alloc(n * 256 * 4), hip.alloc(n * 256 * 4)
+    held = []
+    for _ in range(120):
+        s = hip.seqs(256, n, 1)
+        for f in (100, 256):
+            s.set([f] * n, np.arange(n)[:, None], fresh=[f] * n)
+            s.tree(np.full(n * f, -1))
+            hip.paged_tree(s, g, y.ptr, q.ptr, heads=1, scale=1.0)
+        s.free()
+        held.append(hip.mem_info()[2])
+    assert held[-1] == held[1]
