@@ -497,11 +497,14 @@ class Seqs:
     def tree(self, parent, ids=None):
         """The new tokens as a tree: parent [rows], the place among the sequence's new tokens of the one that
         each follows (-1: the old tokens); ids [rows]: the tokens, for verify."""
-        parent = np.asarray(parent, dtype=np.int64)
-        if ((parent < -(1 << 31)) | (parent > 0xffffffff)).any():  # (that 32 bits would make another)
-            raise ValueError("tree: a parent is a place among the new tokens, or -1")
-        parent = np.ascontiguousarray(parent.astype(np.uint32))
-        ids = None if ids is None else np.ascontiguousarray(ids, dtype=np.uint32)
+        def u32(a, least, what):  # (not what would become another number)
+            a = np.asarray(a)
+            if a.size and (a.min() < least or a.max() > 0xffffffff or (a.dtype.kind not in "iu" and (a != np.floor(a)).any())):
+                raise ValueError(f"tree: {what}")
+            return np.ascontiguousarray(a.astype(np.int64).astype(np.uint32))
+
+        parent = u32(parent, -(1 << 31), "a parent is a place among the new tokens, or -1")
+        ids = None if ids is None else u32(ids, 0, "a token is a whole number of 32 bits")
         if parent.shape != (self.rows,) or (ids is not None and ids.shape != parent.shape):
             raise ValueError(f"tree: arrays of {self.rows} new tokens are wanted")
         self.hip.check(lib.slm_hip_seqs_tree(self.hip.ctx, self.h, _up(parent), None if ids is None else _up(ids)))

@@ -229,3 +229,22 @@ def test_batches_that_grow_and_go_leave_nothing(host, hip):
         s.free()
         held.append(hip.mem_info()[2])
     assert held[-1] == held[1]
+
+
+def test_tokens_that_are_no_32_bits(host, hip):
+    """Not taken for what their lower bits, or their whole part, name; nor a parent for its whole part."""
+    t = Set(host, hip)
+    for bad in (1 << 32, (1 << 32) + 5, -1, 5.5, float("nan"), float("inf"), 1e30):
+        ids = np.arange(137).astype(np.float64 if isinstance(bad, float) else np.int64)
+        ids[5] = bad
+        with pytest.raises(ValueError):
+            t.s.tree(t.parent, ids)
+    for bad in (0.5, float("nan")):
+        parent = t.parent.astype(np.float64)
+        parent[5] = bad
+        with pytest.raises(ValueError):
+            t.s.tree(parent, np.arange(137))
+    t.tree(), t.verify()
+    for ids in (np.arange(137), np.arange(137.0), np.arange(137, dtype=np.uint64), [0xffffffff] * 137, np.full(137, (1 << 32) - 1, np.uint64)):
+        t.s.tree(t.parent, ids)
+    t.s.tree(t.parent.astype(np.float64), np.arange(137))
