@@ -501,7 +501,7 @@ class Seqs:
             a = np.asarray(a)
             if a.size and (a.min() < least or a.max() > 0xffffffff or (a.dtype.kind not in "iu" and (a != np.floor(a)).any())):
                 raise ValueError(f"tree: {what}")
-            return np.ascontiguousarray(a.astype(np.int64).astype(np.uint32))
+            return np.ascontiguousarray((a if a.dtype.kind in "iu" else a.astype(np.int64)).astype(np.uint32))
 
         parent = u32(parent, -(1 << 31), "a parent is a place among the new tokens, or -1")
         ids = None if ids is None else u32(ids, 0, "a token is a whole number of 32 bits")

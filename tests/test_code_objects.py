@@ -59,3 +59,14 @@ def test_the_largest_eviction_fits_in_lds(kernels):
 def test_the_paged_kernels_use_no_scratch_memory(kernels):
     own = [n for n in kernels if n.startswith(("slm_paged", "slm_logprobs"))]
     assert len(own) == 41 and [n for n in own if kernels[n][1]] == []
+
+
+def test_what_the_kernels_of_several_new_tokens_take(kernels):
+    """Scratch memory in heads above 64 alone, where rows are many, and above 128; LDS that a launch sizes from its start."""
+    span = {n: kernels[n] for n in kernels if n.startswith("slm_span") and "join" not in n}
+    assert len(span) == 40
+    spills = {n for n in span if span[n][1]}
+    assert spills == {f"slm_span{slots}{half}_{kind}" for slots in ("", "_slots") for half in ("", "16") for kind in ("128_4", "256_4", "256_1")}
+    assert [n for n in span if span[n][0] % 16] == []
+    rest = [n for n in kernels if n.startswith(("slm_span_join", "slm_tree_", "slm_store_rows"))]
+    assert len(rest) == 8 and [n for n in rest if kernels[n][1]] == []

@@ -4,6 +4,7 @@ values are."""
 import numpy as np
 import pytest
 
+import span_ref as R
 from paged_ref import U, Cache
 from test_gpu_paged import check, hip, rng_of  # noqa: F401
 from test_gpu_spans import queries, run
@@ -11,8 +12,8 @@ from test_gpu_spans import queries, run
 pytestmark = pytest.mark.gpu
 
 
-def attend(c, fresh, q, scale):
-    """A prompt's y [rows][H][dh] in 64 bits, and a bound for each element: r sum w |v| + 2^-36 sum |v| + m 2^-118, over the
+def attend(c, fresh, q, scale, reach=None, gap=0, parent=None):
+    """A prompt's (a tree's, with parents) y [rows][H][dh] in 64 bits, and a bound for each element: r sum w |v| + 2^-36 sum |v| + m 2^-118, over the
     channel's m values that the row sees.
 
     r as in span_ref.attend: a weight's relative error is the score's, twice (its own and the sum's: 2 d), the exponential's and
@@ -25,14 +26,20 @@ def attend(c, fresh, q, scale):
     y, bound, at = np.zeros((rows, H, dh)), np.zeros((rows, H, dh)), 0
     for b, f in enumerate(fresh):
         pg, sl = c.where(b)
-        sees = np.arange(len(pg)) < len(pg) - f + 1 + np.arange(f)[:, None]
+        old, step = len(pg) - f, np.arange(f)
+        sees = np.arange(len(pg)) <= old + step[:, None]
+        if parent is not None:
+            line, step = R.lines(parent[at:at + f], [f])[0]
+            sees[:, old:] = line
+        back = old + step[:, None] - np.concatenate([np.arange(old), old + step])
+        sees &= (back >= gap) & (back < (1 << 62 if reach is None else reach))
         m = sees.sum(1, keepdims=True)
         for h in range(H):
             k, v = (a[pg, h // (H // c.KH), sl].astype(np.float64) for a in (c.k, c.v))
             qq = q[at:at + f, h].astype(np.float64)
             s = np.where(sees, qq @ k.T * scale, -np.inf)
-            e = np.exp(s - s.max(1, keepdims=True))
-            w = e / e.sum(1, keepdims=True)
+            e = np.exp(s - np.where(m, s.max(1, keepdims=True), 0))
+            w = e / np.where(m, e.sum(1, keepdims=True), 1)
             largest = np.where(sees, np.abs(qq) @ np.abs(k).T * abs(scale), 0).max(1, keepdims=True)
             d = U * ((dh + 10) * largest + 3 * np.abs(np.where(sees, s, 0)).max(1, keepdims=True))
             r = 2 * d + U * (8 + 4 + 4 + 4 + m + m / 16 + 32)
@@ -204,3 +211,19 @@ def test_large_scores(hip, pkg, kind, half, size):
 def test_the_largest_queries(hip, pkg, kind, half, size):
     """Near the end of fp32, with scores that it holds."""
     check_by_largest_score(hip, pkg, kind, half, size)
+
+
+@pytest.mark.parametrize("share", [0.0002, 0.3])
+@pytest.mark.parametrize("reach,gap", [(None, 0), (90, 0), (None, 40), (70, 11)])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_small_values_in_windows_and_trees(hip, pkg, kind, tree, reach, gap, share):
+    """In some tiles or all of them, seen by some rows."""
+    H, KH, dh, lens, fresh = kind
+    rng = rng_of(dh, lens[0], gap, tree)
+    c = Cache(rng, lens, KH, dh, 16)
+    c.v = np.where(rng.random(c.v.shape) < share, c.v * np.float32(1e-12), c.v)
+    q = queries(rng, fresh, H, dh)
+    parent = R.random_tree(rng, fresh) if tree else None
+    want, bound = attend(c, fresh, q, dh ** -0.5, reach, gap, parent)
+    check(run(hip, pkg, c, fresh, q, dh ** -0.5, reach, gap, False, parent), want, bound, kind)
