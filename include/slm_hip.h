@@ -260,7 +260,8 @@ int slm_hip_paged_prompt(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, f
  * that it comes from, and its position is the old tokens' end plus its depth (0 without a parent). */
 int slm_hip_paged_tree(slm_hip* ctx, slm_seqs* seqs, const slm_pages* pages, float* y, const float* q, size_t heads,
                        size_t reach, size_t gap, float scale);
-/* The tree against the logits of its tokens ([rows][vocab]): greedy, by slm_hip_argmax's order. A sequence's
+/* The tree against the logits of its tokens ([rows][vocab]): greedy alone, by slm_hip_argmax's order (a caller that samples
+ * has to compare its own draws). A sequence's
  * first new token is one that was picked before; from it the path goes on to the first of a token's children
  * that is its pick. count[b]: the tokens of the path, the first among them (0: no new tokens); path[rows]:
  * their places among the sequence's new tokens, in order, 0xffffffff behind them; next[b]: the pick of the
